@@ -26,7 +26,7 @@ NVCC_FLAGS = ["-std=c++17", "-O3", "--fmad=false", "-lineinfo", "-Xcompiler", "-
               "-Xcompiler", "-ffp-contract=off", "--expt-relaxed-constexpr"] + ARCH
 CXX_FLAGS = ["-std=c++17", "-O2", "-fPIC", "-ffp-contract=off"]
 
-CUDA_SOURCES = ["tick.cu", "envio.cu", "env.cu"]
+CUDA_SOURCES = ["tick.cu", "envio.cu", "env.cu", "search.cu", "history.cu"]
 CXX_SOURCES = ["arena.cpp", "tables.cpp"]
 
 

@@ -5,6 +5,9 @@ constructor, `action_shape` and `mask(observation)`; the mask is one kernel
 launch (carlb_action_mask) on the current CUDA stream instead of a chain of
 torch ops.  Observations must be float32 CUDA tensors whose last dimension is
 one observation row.
+
+`beam_select` is the step of a beam search over a car's joint discrete actions;
+the reference has no counterpart.
 """
 
 from __future__ import annotations
@@ -14,6 +17,7 @@ import torch.nn as nn
 
 from . import capi
 from .carl import ACTION_LOGITS, ACTION_NVECS, OBS_PREVIOUS_CONTROLS
+from .search import BeamStep, select
 
 
 class CARLActionCodec(nn.Module):
@@ -41,6 +45,21 @@ class CARLActionCodec(nn.Module):
         stream = th.cuda.current_stream(obs.device).cuda_stream
         capi.action_mask(obs, rows, obs_dim, self._previous_controls, mask, stream)
         return mask
+
+    def beam_select(self, logits: th.Tensor, scores: th.Tensor, mask: th.Tensor | None = None, *,
+                    width: int | None = None, finished: th.Tensor | None = None) -> BeamStep:
+        """The best continuations of each group's beams over a car's 648 joint actions.
+
+        As `carl_b200.search.beam_select`, with logits [..., beams, ACTION_LOGITS]:
+        an action's log-probability is the sum over the heads of ACTION_NVECS, each
+        a softmax over its allowed logits (`mask`, as `mask()` gives it).  actions is
+        int32 [..., width, 7], what `Env.step` takes for a car; a beam without an
+        allowed action in some head has no continuation.  Of equal totals the lower
+        beam wins, then the lower action with the first head the slowest digit.
+        Up to 32 beams and a width of 32."""
+        if isinstance(logits, th.Tensor) and logits.dim() and logits.shape[-1] != ACTION_LOGITS:
+            raise ValueError(f"logits must have shape [..., beams, {ACTION_LOGITS}]")
+        return select(logits, scores, mask, width, finished, joint=True)
 
 
 __all__ = ["ACTION_NVECS", "CARLActionCodec"]

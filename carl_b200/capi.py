@@ -67,6 +67,36 @@ class Config(ctypes.Structure):
     ]
 
 
+LOGITS_F32, LOGITS_BF16, LOGITS_F16 = range(3)
+BEAM_MAX_BEAMS, BEAM_MAX_WIDTH, JOINT_MAX_BEAMS, JOINT_MAX_WIDTH = 1024, 128, 32, 32
+BEAM_MAX_CANDIDATES = 1 << 30  # beams * vocab
+
+
+class BeamArgs(ctypes.Structure):
+    """carlb_beam_args"""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "scores", "mask", "finished", "out_scores", "out_parents",
+                                               "out_actions", "workspace")] + [
+        (n, ctypes.c_int64) for n in ("workspace_bytes", "logits_group_stride", "logits_beam_stride",
+                                      "mask_group_stride", "mask_beam_stride")] + [
+        (n, ctypes.c_int32) for n in ("groups", "beams", "vocab", "width", "logit_type", "device")]
+
+
+class StateArray(ctypes.Structure):
+    """carlb_state_array"""
+
+    _fields_ = [("data", ctypes.c_void_p), ("outer", ctypes.c_int64), ("outer_stride", ctypes.c_int64),
+                ("inner_bytes", ctypes.c_int64)]
+
+
+class History(ctypes.Structure):
+    """carlb_history"""
+
+    _fields_ = [("pages", ctypes.c_void_p), ("table", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("refs", ctypes.c_void_p), ("record_bytes", ctypes.c_int64)] + [
+        (n, ctypes.c_int32) for n in ("n_rows", "row_pages", "n_pages", "page_len", "device")]
+
+
 class CarlbError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(message)
@@ -121,6 +151,18 @@ def load() -> ctypes.CDLL:
     lib.carlb_stage_times.argtypes = [vp, ctypes.POINTER(ctypes.c_float), i32, ctypes.POINTER(i32)]
     lib.carlb_stage_work.argtypes = [vp, ctypes.POINTER(i32)]
     lib.carlb_action_mask.argtypes = [vp, i64, i32, i32, vp, vp]
+    beam, hist, i64p = ctypes.POINTER(BeamArgs), ctypes.POINTER(History), ctypes.POINTER(i64)
+    lib.carlb_beam_workspace.argtypes = [beam, i64p]
+    lib.carlb_beam_select.argtypes = [beam, vp]
+    lib.carlb_joint_select.argtypes = [beam, vp]
+    lib.carlb_reorder_states.argtypes = [ctypes.POINTER(StateArray), i32, vp, i32, i32, i32, vp]
+    lib.carlb_reorder.argtypes = [vp, vp, i32]
+    lib.carlb_history_fork.argtypes = [hist, hist, vp, vp]
+    lib.carlb_history_workspace.argtypes = [hist, i64p, i64p]
+    lib.carlb_history_append.argtypes = [hist, vp, i64, vp, vp, vp, i64, vp]
+    lib.carlb_history_free.argtypes = [hist, vp, vp]
+    lib.carlb_history_compact.argtypes = [hist, vp, vp, i64, vp]
+    lib.carlb_history_read.argtypes = [hist, vp, i32, i32, vp, vp, vp]
     _lib = lib
     return lib
 
@@ -143,6 +185,14 @@ def action_mask(obs, rows: int, obs_dim: int, previous_controls: bool, mask, str
     st = lib.carlb_action_mask(_ptr(obs), rows, obs_dim, int(previous_controls), _ptr(mask), stream)
     if st != OK:
         raise CarlbError(st, lib.carlb_last_error(None).decode())
+
+
+def check(st: int) -> None:
+    """Raises the error of an entry point that has no env: ValueError for arguments,
+    CarlbError (a RuntimeError) otherwise."""
+    if st != OK:
+        msg = load().carlb_last_error(None).decode()
+        raise ValueError(msg) if st == ERR_VALUE else CarlbError(st, msg)
 
 
 class Env:
@@ -274,6 +324,12 @@ class Env:
     def reset_boost_pads(self, n, indices=None) -> None:
         keep = self._order_after_torch(indices)
         self._check(self._lib.carlb_reset_boost_pads(self._h, n, _ptr(indices)))
+        self._keep_until_read(keep)
+
+    def reorder(self, parents, beams: int) -> None:
+        """carlb_reorder: every sim becomes its parent inside its group of `beams` sims."""
+        keep = self._order_after_torch(parents)
+        self._check(self._lib.carlb_reorder(self._h, _ptr(parents), beams))
         self._keep_until_read(keep)
 
     # ---- outputs / properties ----

@@ -276,6 +276,23 @@ class Env:
         self._call(self._env.reset_boost_pads, k, idx)
         self._env.synchronize()
 
+    # ---- search ----
+    def reorder(self, parents) -> None:
+        """Moves sims inside their groups: with `parents` int64 [n_groups, beams] and
+        n_groups * beams = n_sim, sim g * beams + j takes over the whole state and the
+        output buffers of sim g * beams + parents[g, j].  A value outside [0, beams)
+        leaves its sim as it is.  What the simulator draws from a sim's index (kickoffs,
+        respawns) stays the slot's own, so copies of one sim part there."""
+        t = _as_tensor(parents)
+        if t.dtype != torch.int64:
+            raise TypeError("parents must have dtype int64")
+        self._device_ok(t, "parents")
+        if t.dim() != 2 or t.numel() != self.n_sim or not 1 <= t.shape[1] <= capi.BEAM_MAX_BEAMS:
+            raise ValueError("parents must have shape [n_groups, beams] with n_groups * beams = n_sim, beams <= 1024")
+        if not t.is_contiguous():
+            raise ValueError("parents must be contiguous")
+        self._call(self._env.reorder, t, int(t.shape[1]))
+
     # ---- outputs (non-owning views, overwritten in place) ----
     def _buffer(self, which: int) -> torch.Tensor:
         view = self._views.get(which)

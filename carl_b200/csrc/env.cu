@@ -21,6 +21,8 @@
 #include "../../include/carlb.h"
 #include "arena.hpp"
 #include "envio.cuh"
+#include "history.cuh"
+#include "search.cuh"
 #include "tick.cuh"
 
 using namespace cb;
@@ -1357,6 +1359,287 @@ carlb_status carlb_action_mask(const float* obs, int64_t rows, int32_t obsDim, i
     launchActionMask(obs, rows, obsDim, previousControls != 0, mask, (cudaStream_t)stream);
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return fail(nullptr, CARLB_ERR_CUDA, std::string("action mask: ") + cudaGetErrorString(err));
+    return CARLB_OK;
+}
+
+// ---- search and history --------------------------------------------------------
+
+// Makes `device` current for the calls of one entry point.
+struct DeviceScope
+{
+    int before = -1;
+    cudaError_t err;
+    explicit DeviceScope(int device)
+    {
+        int current = -1;
+        err = cudaGetDevice(&current);
+        if (err == cudaSuccess && current != device)
+        {
+            err = cudaSetDevice(device);
+            if (err == cudaSuccess) before = current;
+        }
+    }
+    ~DeviceScope()
+    {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+static bool misaligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
+
+// Checks the sizes; `joint` for the selection over the action heads.
+static const char* beamSizeError(const carlb_beam_args* a, bool joint)
+{
+    if (!a) return "args is null";
+    if (a->groups < 0) return "groups must be non-negative";
+    if (a->beams < 1 || a->beams > (joint ? JOINT_MAX_BEAMS : BEAM_MAX_BEAMS)) return "beams is out of range";
+    if (a->width < 1 || a->width > (joint ? JOINT_MAX_WIDTH : BEAM_MAX_WIDTH)) return "width is out of range";
+    if (a->logit_type < CARLB_LOGITS_F32 || a->logit_type > CARLB_LOGITS_F16) return "unknown logit_type";
+    if (joint ? a->vocab != ACTION_LOGITS : a->vocab < 1 || (int64_t)a->beams * a->vocab > (1ll << 30))
+        return "vocab is out of range";
+    return nullptr;
+}
+
+static BeamParams beamParams(const carlb_beam_args* a)
+{
+    BeamParams p{};
+    p.logits = a->logits;
+    p.groupStride = a->logits_group_stride;
+    p.beamStride = a->logits_beam_stride;
+    p.scores = a->scores;
+    p.mask = a->mask;
+    p.maskGroupStride = a->mask_group_stride;
+    p.maskBeamStride = a->mask_beam_stride;
+    p.finished = a->finished;
+    p.outScores = a->out_scores;
+    p.outParents = reinterpret_cast<long long*>(a->out_parents);
+    p.outActions = a->out_actions;
+    p.groups = a->groups;
+    p.beams = a->beams;
+    p.vocab = a->vocab;
+    p.width = a->width;
+    return p;
+}
+
+carlb_status carlb_beam_workspace(const carlb_beam_args* a, int64_t* bytes)
+{
+    if (const char* err = beamSizeError(a, false)) return fail(nullptr, CARLB_ERR_VALUE, err);
+    if (!bytes) return fail(nullptr, CARLB_ERR_VALUE, "bytes is null");
+    BeamParams p = beamParams(a);
+    *bytes = planBeamSelect(p, (LogitType)a->logit_type, nullptr);
+    return CARLB_OK;
+}
+
+static carlb_status beamSelect(const carlb_beam_args* a, bool joint, void* stream)
+{
+    if (const char* err = beamSizeError(a, joint)) return fail(nullptr, CARLB_ERR_VALUE, err);
+    if (a->groups == 0) return CARLB_OK;
+    if (!a->logits || !a->scores || !a->out_scores || !a->out_parents || !a->out_actions)
+        return fail(nullptr, CARLB_ERR_VALUE, "logits, scores and the outputs must not be null");
+    if (misaligned(a->logits, a->logit_type == CARLB_LOGITS_F32 ? 4 : 2) || misaligned(a->scores, 4)
+        || misaligned(a->out_scores, 4) || misaligned(a->out_parents, 8) || misaligned(a->out_actions, 4))
+        return fail(nullptr, CARLB_ERR_VALUE, "logits, scores and the outputs must be aligned to their type");
+    if (a->logits_group_stride < 0 || a->logits_beam_stride < 0 || a->mask_group_stride < 0 || a->mask_beam_stride < 0)
+        return fail(nullptr, CARLB_ERR_VALUE, "strides must be non-negative");
+    BeamParams p = beamParams(a);
+    if (!joint)
+    {
+        const long long need = planBeamSelect(p, (LogitType)a->logit_type, a->workspace);
+        if (need > 0 && (!a->workspace || misaligned(a->workspace, 16) || a->workspace_bytes < need))
+            return fail(nullptr, CARLB_ERR_VALUE, "workspace is missing, misaligned or too small");
+    }
+    DeviceScope scope(a->device);
+    if (scope.err != cudaSuccess) return cudaFail(nullptr, scope.err, "beam selection");
+    if (joint)
+        launchJointSelect(p, (LogitType)a->logit_type, (cudaStream_t)stream);
+    else
+        launchBeamSelect(p, (LogitType)a->logit_type, (cudaStream_t)stream);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return cudaFail(nullptr, err, "beam selection");
+    return CARLB_OK;
+}
+
+carlb_status carlb_beam_select(const carlb_beam_args* a, void* stream) { return beamSelect(a, false, stream); }
+carlb_status carlb_joint_select(const carlb_beam_args* a, void* stream) { return beamSelect(a, true, stream); }
+
+carlb_status carlb_reorder_states(const carlb_state_array* arrays, int32_t count, const int64_t* parents,
+                                  int32_t groups, int32_t beams, int32_t device, void* stream)
+{
+    if (count < 0 || (count > 0 && !arrays)) return fail(nullptr, CARLB_ERR_VALUE, "arrays is null");
+    if (groups < 0) return fail(nullptr, CARLB_ERR_VALUE, "groups must be non-negative");
+    if (beams < 1 || beams > BEAM_MAX_BEAMS) return fail(nullptr, CARLB_ERR_VALUE, "beams is out of range");
+    if (count == 0 || groups == 0) return CARLB_OK;
+    if (!parents || misaligned(parents, 8)) return fail(nullptr, CARLB_ERR_VALUE, "parents is null or misaligned");
+    for (int k = 0; k < count; k++)
+    {
+        const carlb_state_array& a = arrays[k];
+        if (a.outer < 0 || a.inner_bytes < 0) return fail(nullptr, CARLB_ERR_VALUE, "array sizes must be non-negative");
+        if (a.outer == 0 || a.inner_bytes == 0) continue;
+        if (!a.data) return fail(nullptr, CARLB_ERR_VALUE, "array data is null");
+        if (a.inner_bytes > (1ll << 40) / beams)
+            return fail(nullptr, CARLB_ERR_VALUE, "array rows are too long");
+        if (a.outer > 1 && a.outer_stride < (int64_t)groups * beams * a.inner_bytes)
+            return fail(nullptr, CARLB_ERR_VALUE, "array slabs overlap");
+    }
+    static_assert(sizeof(StateArray) == sizeof(carlb_state_array), "the same four words");
+    DeviceScope scope(device);
+    if (scope.err != cudaSuccess) return cudaFail(nullptr, scope.err, "state reordering");
+    launchReorder(reinterpret_cast<const StateArray*>(arrays), count, reinterpret_cast<const long long*>(parents), groups,
+                  beams, (cudaStream_t)stream);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return cudaFail(nullptr, err, "state reordering");
+    return CARLB_OK;
+}
+
+carlb_status carlb_reorder(carlb_env* e, const int64_t* parents, int32_t beams)
+{
+    if (!e) return fail(nullptr, CARLB_ERR_VALUE, "env is null");
+    const int nSim = e->cfg.n_sim;
+    if (beams < 1 || beams > BEAM_MAX_BEAMS || nSim % beams != 0)
+        return fail(e, CARLB_ERR_VALUE, "beams must divide n_sim and be at most 1024");
+    if (!parents) return fail(e, CARLB_ERR_VALUE, "parents is null");
+    DeviceScope scope(e->cfg.device);
+    if (scope.err != cudaSuccess) return cudaFail(e, scope.err, "reorder");
+    const long long cars = e->nCars, carSlab = e->carStride * 4, simSlab = e->simStride * 4;
+    const auto row = [](void* data, long long bytes) { return StateArray{ data, 1, 0, bytes }; };
+    const StateArray list[] = {
+        { e->car, NCW, carSlab, cars * 4 },
+        { e->carOut, NOW, carSlab, cars * 4 },
+        { e->sim, NSW, simSlab, 4 },
+        row(e->simOut, 4),
+        row(e->obs, cars * e->obsDim * 4),
+        row(e->tobs, cars * e->obsDim * 4),
+        row(e->packed, e->stateDim * 4ll),
+        row(e->tpacked, e->stateDim * 4ll),
+        row(e->rewards, 4),
+        row(e->dones, 1),
+        row(e->overtime, 1),
+        row(e->tovertime, 1),
+        row(e->scoreDiff, 4),
+        row(e->episodeTicks, 4),
+        row(e->tScoreDiff, 4),
+        row(e->tEpisodeTicks, 4),
+        { e->diagCar, e->diagCar ? DIAG_CAR_WORDS : 0, carSlab, cars * 4 },
+        { e->diagSim, e->diagSim ? DIAG_SIM_WORDS : 0, simSlab, 4 },
+    };
+    const long long* from = reinterpret_cast<const long long*>(parents);
+    launchReorder(list, (int)(sizeof(list) / sizeof(list[0])), from, nSim / beams, beams, e->stream);
+    launchMoveContacts(reinterpret_cast<int*>(e->car + C_CONTACT_IDX * e->carStride), from, nSim, beams, e->nCars, e->stream);
+    ECHECK(e, cudaGetLastError());
+    return CARLB_OK;
+}
+
+static const char* historyError(const carlb_history* h)
+{
+    if (!h) return "history is null";
+    if (h->n_rows < 0 || h->n_pages < 0) return "n_rows and n_pages must be non-negative";
+    if (h->row_pages < 1 || h->page_len < 1 || h->record_bytes < 1)
+        return "row_pages, page_len and record_bytes must be positive";
+    if ((int64_t)h->row_pages * h->page_len > INT32_MAX) return "rows are too long";
+    if (h->record_bytes > (1ll << 40) / h->page_len) return "pages are too large";
+    if (h->n_pages > 0 && (!h->pages || !h->refs || misaligned(h->refs, 4))) return "pages or refs is null or misaligned";
+    if (h->n_rows > 0 && (!h->table || !h->lengths || misaligned(h->table, 4) || misaligned(h->lengths, 4)))
+        return "table or lengths is null or misaligned";
+    return nullptr;
+}
+
+static HistoryView historyView(const carlb_history* h)
+{
+    return HistoryView{ static_cast<char*>(h->pages), h->table, h->lengths, h->refs, h->record_bytes,
+                        h->n_rows, h->row_pages, h->n_pages, h->page_len };
+}
+
+carlb_status carlb_history_fork(const carlb_history* from, const carlb_history* to, const int64_t* parents, void* stream)
+{
+    const char* bad = historyError(from);
+    if (!bad) bad = historyError(to);
+    if (!bad && (from->pages != to->pages || from->row_pages != to->row_pages || from->n_pages != to->n_pages
+                 || from->page_len != to->page_len || from->record_bytes != to->record_bytes || from->device != to->device))
+        bad = "both histories must have the same pages and geometry";
+    if (!bad && to->n_rows > 0 && (!parents || misaligned(parents, 8))) bad = "parents is null or misaligned";
+    if (!bad && ((to->n_pages > 0 && from->refs == to->refs)
+                 || (to->n_rows > 0 && (from->table == to->table || from->lengths == to->lengths))))
+        bad = "the forked history must not overlap its source";
+    if (bad) return fail(nullptr, CARLB_ERR_VALUE, bad);
+    DeviceScope scope(to->device);
+    if (scope.err != cudaSuccess) return cudaFail(nullptr, scope.err, "history fork");
+    const cudaError_t err = launchHistoryFork(historyView(from), historyView(to),
+                                              reinterpret_cast<const long long*>(parents), (cudaStream_t)stream);
+    if (err != cudaSuccess) return cudaFail(nullptr, err, "history fork");
+    return CARLB_OK;
+}
+
+carlb_status carlb_history_workspace(const carlb_history* h, int64_t* appendBytes, int64_t* compactBytes)
+{
+    if (const char* bad = historyError(h)) return fail(nullptr, CARLB_ERR_VALUE, bad);
+    if (appendBytes) *appendBytes = historyAppendWorkspace(historyView(h));
+    if (compactBytes) *compactBytes = historyCompactWorkspace(historyView(h));
+    return CARLB_OK;
+}
+
+carlb_status carlb_history_append(const carlb_history* h, const void* records, int64_t recordStride,
+                                  const uint8_t* mask, int32_t* dropped, void* workspace, int64_t workspaceBytes,
+                                  void* stream)
+{
+    if (const char* bad = historyError(h)) return fail(nullptr, CARLB_ERR_VALUE, bad);
+    if (h->n_rows == 0) return CARLB_OK;
+    if (!records || !dropped || misaligned(dropped, 4)) return fail(nullptr, CARLB_ERR_VALUE, "records or dropped is null or misaligned");
+    if (recordStride < 0) return fail(nullptr, CARLB_ERR_VALUE, "record_stride must be non-negative");
+    const HistoryView v = historyView(h);
+    if (!workspace || misaligned(workspace, 16) || workspaceBytes < historyAppendWorkspace(v))
+        return fail(nullptr, CARLB_ERR_VALUE, "workspace is missing, misaligned or too small");
+    DeviceScope scope(h->device);
+    if (scope.err != cudaSuccess) return cudaFail(nullptr, scope.err, "history append");
+    const cudaError_t err = launchHistoryAppend(v, static_cast<const char*>(records), recordStride, mask, dropped,
+                                                workspace, (cudaStream_t)stream);
+    if (err != cudaSuccess) return cudaFail(nullptr, err, "history append");
+    return CARLB_OK;
+}
+
+carlb_status carlb_history_free(const carlb_history* h, const uint8_t* mask, void* stream)
+{
+    if (const char* bad = historyError(h)) return fail(nullptr, CARLB_ERR_VALUE, bad);
+    if (h->n_rows == 0) return CARLB_OK;
+    if (!mask) return fail(nullptr, CARLB_ERR_VALUE, "mask is null");
+    DeviceScope scope(h->device);
+    if (scope.err != cudaSuccess) return cudaFail(nullptr, scope.err, "history free");
+    launchHistoryFree(historyView(h), mask, (cudaStream_t)stream);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return cudaFail(nullptr, err, "history free");
+    return CARLB_OK;
+}
+
+carlb_status carlb_history_compact(const carlb_history* h, int32_t* live, void* workspace, int64_t workspaceBytes,
+                                   void* stream)
+{
+    if (const char* bad = historyError(h)) return fail(nullptr, CARLB_ERR_VALUE, bad);
+    if (!live || misaligned(live, 4)) return fail(nullptr, CARLB_ERR_VALUE, "live is null or misaligned");
+    const HistoryView v = historyView(h);
+    if (!workspace || misaligned(workspace, 16) || workspaceBytes < historyCompactWorkspace(v))
+        return fail(nullptr, CARLB_ERR_VALUE, "workspace is missing, misaligned or too small");
+    DeviceScope scope(h->device);
+    if (scope.err != cudaSuccess) return cudaFail(nullptr, scope.err, "history compact");
+    const cudaError_t err = launchHistoryCompact(v, live, workspace, (cudaStream_t)stream);
+    if (err != cudaSuccess) return cudaFail(nullptr, err, "history compact");
+    return CARLB_OK;
+}
+
+carlb_status carlb_history_read(const carlb_history* h, const int64_t* rows, int32_t n, int32_t steps, void* out,
+                                int32_t* counts, void* stream)
+{
+    if (const char* bad = historyError(h)) return fail(nullptr, CARLB_ERR_VALUE, bad);
+    if (n < 0 || steps < 1) return fail(nullptr, CARLB_ERR_VALUE, "n must be non-negative and steps positive");
+    if (!rows && n != h->n_rows) return fail(nullptr, CARLB_ERR_VALUE, "n must be n_rows without row indices");
+    if ((int64_t)n * steps > (1ll << 33)) return fail(nullptr, CARLB_ERR_VALUE, "n * steps is too large");
+    if (n == 0) return CARLB_OK;
+    if (!out || !counts || misaligned(counts, 4) || misaligned(rows, 8))
+        return fail(nullptr, CARLB_ERR_VALUE, "out, counts or rows is null or misaligned");
+    DeviceScope scope(h->device);
+    if (scope.err != cudaSuccess) return cudaFail(nullptr, scope.err, "history read");
+    launchHistoryRead(historyView(h), reinterpret_cast<const long long*>(rows), n, steps, static_cast<char*>(out), counts,
+                      (cudaStream_t)stream);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return cudaFail(nullptr, err, "history read");
     return CARLB_OK;
 }
 

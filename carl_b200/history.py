@@ -1,0 +1,211 @@
+"""Paged history: records of ragged sequences in pages that forked sequences share.
+
+An env overwrites its output buffers with every step; a history keeps what they
+held.  A row is one sequence (an agent's episode, a beam's lineage), a record any
+fixed shape (an observation row, an action).  Episodes end at different times and
+lineages share their past, so records lie in pages of `page_len` that a table
+assigns to rows; a page is shared until a row writes to it::
+
+    history = PagedHistory.empty(n_rows, row_pages, n_pages, page_len, (obs_dim,))
+    history.append(env.get_obs().view(n_rows, obs_dim))     # one record per row
+    history.free(done)                                      # rows of ended episodes
+    history = history.fork(parents)                         # rows become their parents
+    history.compact()                                       # live pages to the front
+    records, counts = history.read(steps)                   # the last records, dense
+
+Everything runs on torch's current stream of the pages' device, without a host
+synchronisation, and can be captured into CUDA graphs; two calls on one history (or
+on a history and its fork) must be ordered by the caller if they run on different
+streams.  Errors are as in ``carl_b200.carl``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import capi
+
+
+class PagedHistory:
+    """Pages, table, lengths and reference counts of a paged history.
+
+    pages    any dtype [n_pages, page_len, *record], contiguous
+    table    int32 [n_rows, row_pages]: record i of row r lies in page
+             table[r, i // page_len]; entries behind the last page in use are -1
+    lengths  int32 [n_rows]
+    refs     int32 [n_pages]: how many table entries name the page; 0 = free
+
+    The constructor wraps tensors that already hold a history; `empty` makes a new one.
+    `dropped` (int32 [1]) counts the records that `append` found no place for.
+    """
+
+    def __init__(self, pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
+                 dropped: torch.Tensor | None = None):
+        for name, t in (("pages", pages), ("table", table), ("lengths", lengths), ("refs", refs)):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} must be a tensor")
+            if name != "pages" and t.dtype != torch.int32:
+                raise TypeError(f"{name} must have dtype int32")
+        for name, t in (("pages", pages), ("table", table), ("lengths", lengths), ("refs", refs)):
+            if t.device.type != "cuda":
+                raise ValueError(f"{name} must be on a CUDA device")
+            if t.device != pages.device:
+                raise ValueError(f"{name} must be on {pages.device}")
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+        if pages.requires_grad:
+            raise ValueError("pages must not require a gradient")
+        if pages.dim() < 2 or pages.shape[1] < 1 or 0 in pages.shape[2:]:
+            raise ValueError("pages must have shape [n_pages, page_len, *record] without empty dimensions")
+        if table.dim() != 2 or table.shape[1] < 1 or lengths.shape != table.shape[:1] or refs.shape != pages.shape[:1]:
+            raise ValueError("table must be [n_rows, row_pages], lengths [n_rows] and refs [n_pages]")
+        if table.shape[1] * pages.shape[1] > 0x7fffffff or max(pages.shape[0], table.shape[0]) > 0x7fffffff:
+            raise ValueError("too many rows, pages or records of a row")
+        self.pages, self.table, self.lengths, self.refs = pages, table, lengths, refs
+        self.record_shape = tuple(pages.shape[2:])
+        self._dropped = dropped
+        record_bytes = pages.element_size()
+        for n in self.record_shape:
+            record_bytes *= n
+        self._view = capi.History(pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), record_bytes,
+                                  table.shape[0], table.shape[1], pages.shape[0], pages.shape[1], pages.device.index)
+
+    @classmethod
+    def empty(cls, n_rows: int, row_pages: int, n_pages: int, page_len: int, record_shape: tuple = (),
+              dtype: torch.dtype = torch.float32, device: torch.device | str | int | None = None) -> PagedHistory:
+        """A history without records: every row empty, every page free."""
+        if min(n_rows, n_pages) < 0 or min(row_pages, page_len) < 1:
+            raise ValueError("n_rows and n_pages must be non-negative, row_pages and page_len positive")
+        if device is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        return cls(torch.zeros((n_pages, page_len, *record_shape), dtype=dtype, device=device),
+                   torch.full((n_rows, row_pages), -1, dtype=torch.int32, device=device),
+                   torch.zeros(n_rows, dtype=torch.int32, device=device),
+                   torch.zeros(n_pages, dtype=torch.int32, device=device))
+
+    @property
+    def n_rows(self) -> int:
+        return self.table.shape[0]
+
+    @property
+    def n_pages(self) -> int:
+        return self.pages.shape[0]
+
+    @property
+    def page_len(self) -> int:
+        return self.pages.shape[1]
+
+    @property
+    def dropped(self) -> torch.Tensor:
+        if self._dropped is None:
+            self._dropped = torch.zeros(1, dtype=torch.int32, device=self.pages.device)
+        return self._dropped
+
+    def _stream(self) -> int:
+        return torch.cuda.current_stream(self.pages.device).cuda_stream
+
+    def _mask(self, mask, name: str) -> torch.Tensor:
+        if not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool:
+            raise TypeError(f"{name} must be a bool tensor")
+        if mask.device != self.pages.device:
+            raise ValueError(f"{name} must be on {self.pages.device}")
+        if mask.shape != self.lengths.shape:
+            raise ValueError(f"{name} must have shape [n_rows]")
+        return mask.contiguous()
+
+    def _indices(self, indices, name: str) -> torch.Tensor:
+        if not isinstance(indices, torch.Tensor) or indices.dtype != torch.int64:
+            raise TypeError(f"{name} must be an int64 tensor")
+        if indices.device != self.pages.device:
+            raise ValueError(f"{name} must be on {self.pages.device}")
+        return indices.contiguous()
+
+    def fork(self, parents: torch.Tensor, out: PagedHistory | None = None) -> PagedHistory:
+        """The history whose row r continues row parents[r] of this one.
+
+        parents  int64 of any shape, flattened to rows; a value outside [0, n_rows)
+                 gives an empty row
+
+        Pages are shared, not copied; pages that no row of the result names are free
+        in it.  The result replaces this history, which is void once the result is
+        appended to or compacted.  `out` takes the result instead of a new history: one
+        over the same pages with a table, lengths and refs of its own (two histories
+        used in turn, for instance by captured graphs)."""
+        p = self._indices(parents, "parents").view(-1)
+        n, row_pages, n_pages = p.numel(), self.table.shape[1], self.n_pages
+        if out is None:
+            book = torch.empty(n * row_pages + n + n_pages, dtype=torch.int32, device=self.pages.device)
+            out = PagedHistory(self.pages, book[:n * row_pages].view(n, row_pages),
+                               book[n * row_pages:n * row_pages + n], book[n * row_pages + n:], self._dropped)
+        elif (out.pages.data_ptr() != self.pages.data_ptr() or out.pages.shape != self.pages.shape
+              or out.pages.dtype != self.pages.dtype or out.table.shape != (n, row_pages)):
+            raise ValueError("out must be over the same pages, with a row for every parent")
+        capi.check(capi.load().carlb_history_fork(self._view, out._view, p.data_ptr(), self._stream()))
+        return out
+
+    def append(self, records: torch.Tensor, mask: torch.Tensor | None = None) -> None:
+        """Appends records[r] to every row r, or to those with mask[r].
+
+        A row at a page's end takes a free page.  A row whose last page is shared takes
+        a free page and copies that page's records first; where all rows that share the
+        page append, the longest of them (the first of those) writes on in it instead.
+        Free pages go lowest first to the rows in order.  A row that finds no free page,
+        or has no table entry left, stays as it was and is counted in `dropped`."""
+        if not isinstance(records, torch.Tensor) or records.dtype != self.pages.dtype:
+            raise TypeError("records must be a tensor of the pages' dtype")
+        if records.device != self.pages.device:
+            raise ValueError(f"records must be on {self.pages.device}")
+        if records.shape != (self.n_rows, *self.record_shape):
+            raise ValueError("records must have shape [n_rows, *record]")
+        m = None if mask is None else self._mask(mask, "mask")
+        if self.n_rows == 0:
+            return
+        rec = records.detach()
+        if not rec[0].is_contiguous() or rec.stride(0) < 0:
+            rec = rec.contiguous()
+        size = ctypes.c_int64()
+        lib = capi.load()
+        capi.check(lib.carlb_history_workspace(self._view, size, None))
+        work = torch.empty(size.value, dtype=torch.uint8, device=self.pages.device)
+        capi.check(lib.carlb_history_append(self._view, rec.data_ptr(), rec.stride(0) * rec.element_size(),
+                                            None if m is None else m.data_ptr(), self.dropped.data_ptr(),
+                                            work.data_ptr(), size.value, self._stream()))
+
+    def free(self, mask: torch.Tensor) -> None:
+        """Empties the rows with mask[r]; a page is free when no row names it any more."""
+        m = self._mask(mask, "mask")
+        if self.n_rows:
+            capi.check(capi.load().carlb_history_free(self._view, m.data_ptr(), self._stream()))
+
+    def compact(self) -> torch.Tensor:
+        """Moves the live pages to the front and returns their number, int32 [1] on the
+        device: of L live pages, the k-th highest goes to the k-th free page below L.
+        pages[:L] is then all that the history holds."""
+        size = ctypes.c_int64()
+        lib = capi.load()
+        capi.check(lib.carlb_history_workspace(self._view, None, size))
+        work = torch.empty(max(16, size.value), dtype=torch.uint8, device=self.pages.device)
+        live = torch.empty(1, dtype=torch.int32, device=self.pages.device)
+        capi.check(lib.carlb_history_compact(self._view, live.data_ptr(), work.data_ptr(), size.value, self._stream()))
+        return live
+
+    def read(self, steps: int, rows: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The last `steps` records of the rows (all, or int64 row indices of any shape):
+        records [*rows, steps, *record], oldest first, zeros behind a row's last, and
+        their number, int32 [*rows].  A row index outside [0, n_rows) counts 0."""
+        steps = int(steps)
+        if steps < 1:
+            raise ValueError("steps must be positive")
+        r = None if rows is None else self._indices(rows, "rows")
+        shape = (self.n_rows,) if r is None else tuple(r.shape)
+        counts = torch.empty(shape, dtype=torch.int32, device=self.pages.device)
+        n = counts.numel()
+        if n * steps > 1 << 33:
+            raise ValueError("too many records")
+        out = torch.empty((*shape, steps, *self.record_shape), dtype=self.pages.dtype, device=self.pages.device)
+        if n:
+            capi.check(capi.load().carlb_history_read(self._view, None if r is None else r.data_ptr(), n, steps,
+                                                      out.data_ptr(), counts.data_ptr(), self._stream()))
+        return out, counts

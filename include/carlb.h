@@ -337,6 +337,140 @@ carlb_status carlb_stage_work(carlb_env* env, int32_t counts[4]);
 carlb_status carlb_action_mask(const float* obs, int64_t rows, int32_t obs_dim, int32_t previous_controls,
                                uint8_t* mask, void* stream);
 
+/* ---- search over simulations ------------------------------------------------
+ *
+ * A group is one planning problem, a beam one candidate of it: its score (the sum
+ * of its actions' log-probabilities so far) and, in an env, one sim.  The entry
+ * points below take device memory of `device`, enqueue on `stream` (a cudaStream_t
+ * of that device; NULL = the legacy default stream), neither allocate nor
+ * synchronise, can be captured into a CUDA graph, and leave the caller's current
+ * device as it was.  No counterpart in the reference. */
+
+typedef enum carlb_logit_type {
+    CARLB_LOGITS_F32 = 0,
+    CARLB_LOGITS_BF16 = 1,
+    CARLB_LOGITS_F16 = 2
+} carlb_logit_type;
+
+typedef struct carlb_beam_args {
+    const void* logits;            /* [groups, beams, vocab], last dimension dense */
+    const float* scores;           /* [groups, beams] dense */
+    const uint8_t* mask;           /* [groups, beams, vocab], last dimension dense, or NULL; 0 = not allowed */
+    const uint8_t* finished;       /* [groups, beams] dense, or NULL; nonzero = the beam is over */
+    float* out_scores;             /* [groups, width] */
+    int64_t* out_parents;          /* [groups, width] beam index inside the group */
+    int32_t* out_actions;          /* [groups, width]; carlb_joint_select: [groups, width, 7] */
+    void* workspace;               /* 16-byte aligned, carlb_beam_workspace bytes */
+    int64_t workspace_bytes;
+    int64_t logits_group_stride;   /* elements between groups / beams, >= 0 (0 = broadcast) */
+    int64_t logits_beam_stride;
+    int64_t mask_group_stride;
+    int64_t mask_beam_stride;
+    int32_t groups;
+    int32_t beams;                 /* 1 .. 1024 (joint: 32) */
+    int32_t vocab;                 /* >= 1, beams * vocab <= 2^30 (joint: 18 logits) */
+    int32_t width;                 /* 1 .. 128 (joint: 32) */
+    int32_t logit_type;            /* carlb_logit_type */
+    int32_t device;
+} carlb_beam_args;
+
+/* Workspace bytes of carlb_beam_select for these sizes (carlb_joint_select needs none). */
+carlb_status carlb_beam_workspace(const carlb_beam_args* args, int64_t* bytes);
+
+/* The `width` best continuations of each group, best first: the total of action v
+ * of beam k is scores[k] + logits[k][v] - log(sum over the allowed u of
+ * exp(logits[k][u])), and equal totals go to the lower k * vocab + v.  Totals are
+ * compared as if computed in 64 bits and returned rounded to float32.
+ * A finished beam has one continuation, action 0 at its own score.  Not allowed:
+ * actions with mask 0 (whatever their logit), logits of -inf, every action of a
+ * beam whose score is -inf or NaN or whose allowed logits hold a NaN or +inf.
+ * Where fewer than `width` continuations exist, the places behind them get score
+ * -inf, parent (place mod beams) and action 0. */
+carlb_status carlb_beam_select(const carlb_beam_args* args, void* stream);
+
+/* The same over the joint actions of a car: each beam has 18 logits, the heads
+ * (3, 3, 3, 2, 2, 3, 2) of the discrete action, with a softmax of its own per head;
+ * an action's total sums its seven logits, and the action index that decides ties
+ * has the first head as its slowest digit.  Actions are written as seven indices. */
+carlb_status carlb_joint_select(const carlb_beam_args* args, void* stream);
+
+/* One array of per-beam state: `outer` slabs, outer_stride bytes apart, each of
+ * groups * beams dense rows of inner_bytes.  Row-major state is one slab; state
+ * that is word-major like the simulator's has a slab per word. */
+typedef struct carlb_state_array {
+    void* data;
+    int64_t outer;
+    int64_t outer_stride;
+    int64_t inner_bytes;
+} carlb_state_array;
+
+/* Moves the parents' state to the slots of the beams they became, in place:
+ * new[g, j] = old[g, parents[g, j]] for every array (arrays must not overlap).
+ * parents: int64 [groups, beams]; a value outside [0, beams) leaves the slot as it
+ * is.  beams <= 1024. */
+carlb_status carlb_reorder_states(const carlb_state_array* arrays, int32_t count, const int64_t* parents,
+                                  int32_t groups, int32_t beams, int32_t device, void* stream);
+
+/* The same for an env: the whole state and every output buffer of sim
+ * g * beams + j become those of sim g * beams + parents[g * beams + j]; n_sim must
+ * be a multiple of beams.  Enqueued on the env's stream.  What the tick derives
+ * from a sim's index stays the slot's own (the kickoff and respawn draws). */
+carlb_status carlb_reorder(carlb_env* env, const int64_t* parents, int32_t beams);
+
+/* ---- paged history -------------------------------------------------------------
+ *
+ * Records of ragged sequences (rows) in pages of page_len records that rows may
+ * share.  Record i of row r lies in page table[r][i / page_len]; refs[p] counts the
+ * table entries that name page p, and pages with none are free.  Table entries
+ * outside [0, n_pages) name no page.  Streams, capture and devices as above. */
+typedef struct carlb_history {
+    void* pages;            /* [n_pages, page_len] records of record_bytes */
+    int32_t* table;         /* [n_rows, row_pages], -1 where unused */
+    int32_t* lengths;       /* [n_rows] */
+    int32_t* refs;          /* [n_pages] */
+    int64_t record_bytes;
+    int32_t n_rows;
+    int32_t row_pages;
+    int32_t n_pages;
+    int32_t page_len;
+    int32_t device;
+} carlb_history;
+
+/* Row r of `to` becomes row parents[r] of `from` (int64 [to->n_rows]; a value
+ * outside [0, from->n_rows) gives an empty row); the pages are shared, not copied,
+ * and to->refs counts what to->table names.  Both name the same pages; table,
+ * lengths and refs of `to` must not overlap those of `from`, which is void once
+ * `to` is appended to. */
+carlb_status carlb_history_fork(const carlb_history* from, const carlb_history* to, const int64_t* parents,
+                                void* stream);
+
+/* Workspace bytes of carlb_history_append and carlb_history_compact. */
+carlb_status carlb_history_workspace(const carlb_history* h, int64_t* append_bytes, int64_t* compact_bytes);
+
+/* Appends records[r] (record_stride bytes apart) to every row r, or to those with
+ * mask[r] != 0.  A row at a page's end takes a free page; a row whose last page is
+ * shared takes a free page and copies that page's records, except that where all
+ * rows sharing it append, the longest of them (the first of those) stays.  The k-th
+ * row in need, in row order, takes the k-th lowest free page.  A row for which no
+ * page or table column is left stays as it was and adds one to *dropped. */
+carlb_status carlb_history_append(const carlb_history* h, const void* records, int64_t record_stride,
+                                  const uint8_t* mask, int32_t* dropped, void* workspace, int64_t workspace_bytes,
+                                  void* stream);
+
+/* Empties the rows with mask[r] != 0 (u8 [n_rows]); their pages lose a reference each. */
+carlb_status carlb_history_free(const carlb_history* h, const uint8_t* mask, void* stream);
+
+/* Moves the live pages to the front: of L live pages, the k-th highest goes to the
+ * k-th free page below L, and the table follows.  *live receives L. */
+carlb_status carlb_history_compact(const carlb_history* h, int32_t* live, void* workspace, int64_t workspace_bytes,
+                                   void* stream);
+
+/* The last min(length, steps) records of rows[i] (int64 [n], NULL = all rows in
+ * order, n = n_rows) to out[i] ([n, steps] records, zeros behind them), their number
+ * to counts[i].  A row outside [0, n_rows) counts 0. */
+carlb_status carlb_history_read(const carlb_history* h, const int64_t* rows, int32_t n, int32_t steps, void* out,
+                                int32_t* counts, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,485 @@
+"""Beam selection (flat and over the action heads) and state reordering.
+
+Tolerances of the scores: an output is rounded once to float32 (2^-24 relative);
+the logarithm of the softmax sum that a beam's totals share is off by at most
+3.5e-6 (the bound derived beside the merge kernel) in the flat selection and by a
+few 2^-52 in the joint one.  Parents and actions are whole numbers and equal."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+from carl_b200 import _build, capi
+from search_oracle import HEADS, best_continuations, joint_actions
+
+SUM_ERROR = 3.5e-6
+DTYPES = ["float32", "bfloat16", "float16"]
+
+
+# ---- refusals (no GPU) -----------------------------------------------------------------
+
+
+@pytest.fixture(scope="module")
+def lib():
+    _build.build()
+    return capi.load()
+
+
+def _args(**kw):
+    a = capi.BeamArgs(logits=64, scores=64, out_scores=64, out_parents=64, out_actions=64, workspace=64,
+                      workspace_bytes=1 << 40, logits_group_stride=72, logits_beam_stride=18, groups=2, beams=4, vocab=18,
+                      width=4)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("joint", [False, True])
+@pytest.mark.parametrize("bad, needle", [
+    (dict(groups=-1), "groups"), (dict(beams=0), "beams"), (dict(beams=1025), "beams"), (dict(width=0), "width"),
+    (dict(width=129), "width"), (dict(logit_type=3), "logit_type"), (dict(vocab=0), "vocab"), (dict(logits=None), "null"),
+    (dict(out_actions=None), "null"), (dict(logits=66), "aligned"), (dict(out_parents=68), "aligned"),
+    (dict(logits_beam_stride=-1), "strides"),
+])
+def test_select_refuses_before_launch(lib, joint, bad, needle):
+    fn = lib.carlb_joint_select if joint else lib.carlb_beam_select
+    assert fn(_args(**bad), None) == capi.ERR_VALUE
+    assert needle in lib.carlb_last_error(None).decode()
+
+
+def test_select_limits_by_kind(lib):
+    assert lib.carlb_joint_select(_args(beams=33), None) == capi.ERR_VALUE
+    assert lib.carlb_joint_select(_args(width=33), None) == capi.ERR_VALUE
+    assert lib.carlb_joint_select(_args(vocab=19), None) == capi.ERR_VALUE
+    assert lib.carlb_beam_select(_args(beams=1024, vocab=1 << 21), None) == capi.ERR_VALUE
+    # Whether this selection needs a workspace is the library's choice; too little is refused.
+    size = ctypes.c_int64()
+    big = _args(groups=64, beams=64, vocab=100000)
+    assert lib.carlb_beam_workspace(big, size) == capi.OK and size.value > 0
+    big.workspace_bytes = size.value - 1
+    assert lib.carlb_beam_select(big, None) == capi.ERR_VALUE
+    assert "workspace" in lib.carlb_last_error(None).decode()
+    assert lib.carlb_beam_select(None, None) == capi.ERR_VALUE
+    assert lib.carlb_beam_select(_args(groups=0), None) == capi.OK
+
+
+def test_reorder_refuses_before_launch(lib):
+    ok = capi.StateArray(64, 1, 0, 4)
+    call = lambda arr, count, parents, groups, beams: lib.carlb_reorder_states(arr, count, parents, groups, beams, 0, None)  # noqa: E731
+    assert call(None, 1, 64, 2, 4) == capi.ERR_VALUE
+    assert call(ok, -1, 64, 2, 4) == capi.ERR_VALUE
+    assert call(ok, 1, None, 2, 4) == capi.ERR_VALUE
+    assert call(ok, 1, 64, 2, 0) == capi.ERR_VALUE
+    assert call(ok, 1, 64, 2, 1025) == capi.ERR_VALUE
+    assert call(capi.StateArray(None, 1, 0, 4), 1, 64, 2, 4) == capi.ERR_VALUE
+    assert call(capi.StateArray(64, 3, 31, 4), 1, 64, 2, 4) == capi.ERR_VALUE
+    assert "overlap" in lib.carlb_last_error(None).decode()
+    assert call(ok, 1, 64, 0, 4) == capi.OK and call(None, 0, None, 2, 4) == capi.OK
+    assert lib.carlb_reorder(None, 64, 4) == capi.ERR_VALUE
+
+
+def test_python_refuses_cpu_tensors_and_types():
+    import torch
+    from carl_b200.action import CARLActionCodec
+    from carl_b200.search import beam_select, reorder_states
+
+    x, s = torch.zeros(2, 4, 18), torch.zeros(2, 4)
+    for select in (beam_select, CARLActionCodec().beam_select):
+        with pytest.raises(ValueError, match="CUDA"):
+            select(x, s)
+        with pytest.raises(TypeError, match="logits"):
+            select([1.0], s)
+    with pytest.raises(ValueError, match="18"):
+        CARLActionCodec().beam_select(x[..., :17], s)
+    with pytest.raises(ValueError, match="CUDA"):
+        reorder_states([x], torch.zeros(2, 4, dtype=torch.int64))
+    with pytest.raises(TypeError, match="int64"):
+        reorder_states([x], s)
+    with pytest.raises(TypeError, match="sequence"):
+        reorder_states(x, torch.zeros(2, 4, dtype=torch.int64))
+
+
+# ---- selection --------------------------------------------------------------------------
+
+
+def _inputs(G, K, V, dtype, masked, finished, seed):
+    import torch
+
+    rng = np.random.default_rng(seed)
+    x = torch.from_numpy(rng.normal(0, 3, (G, K, V)).astype(np.float32)).to(getattr(torch, dtype))
+    s = torch.from_numpy((-5 * rng.random((G, K))).astype(np.float32))
+    m = torch.from_numpy(rng.random((G, K, V)) < 0.7) if masked else None
+    if masked and K > 1:
+        m[0, K - 1] = False                      # a beam without a legal action
+    f = torch.from_numpy(rng.random((G, K)) < 0.25) if finished else None
+    if finished:
+        s[:, 0] = -math.inf                      # a dead beam, finished or not
+    return x, s, m, f
+
+
+def _check(x, s, m, f, width, heads=None, fn=None, sum_error=SUM_ERROR):
+    import torch
+    from carl_b200.action import CARLActionCodec
+    from carl_b200.search import beam_select
+
+    fn = fn or (beam_select if heads is None else CARLActionCodec().beam_select)
+    cuda = lambda t: None if t is None else t.cuda()  # noqa: E731
+    best = fn(cuda(x), cuda(s), cuda(m), width=width, finished=cuda(f))
+    m3 = None if m is None else m.expand(x.shape).numpy()
+    es, ep, ea = best_continuations(x.float().numpy(), s.numpy(), m3, None if f is None else f.numpy(), width, heads)
+    assert best.parents.dtype == torch.int64 and best.actions.dtype == torch.int32 and best.scores.dtype == torch.float32
+    np.testing.assert_array_equal(best.parents.cpu().numpy(), ep)
+    np.testing.assert_array_equal(best.actions.cpu().numpy(), ea if heads is None else joint_actions(ea))
+    got = best.scores.cpu().double().numpy()
+    np.testing.assert_array_equal(np.isfinite(got), np.isfinite(es))
+    ok = np.isfinite(es)
+    assert (np.abs(got[ok] - es[ok]) <= sum_error + 2.0 ** -24 * np.abs(es[ok])).all()
+    return best
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("G, K, V, width", [
+    (1, 1, 1, 1), (1, 1, 7, 3), (3, 2, 18, 5), (5, 8, 90, 8), (7, 5, 648, 4), (2, 33, 1023, 33), (3, 8, 1025, 64),
+    (2, 3, 4099, 128), (1, 8, 50257, 8), (2, 64, 2048, 17), (1, 1024, 33, 128), (300, 4, 31, 4), (2, 2, 131072, 1),
+])
+@pytest.mark.parametrize("masked, finished", [(False, False), (True, True)])
+def test_flat_selection(dtype, G, K, V, width, masked, finished):
+    _check(*_inputs(G, K, V, dtype, masked, finished, G + K + V), width)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("G, K, width", [(1, 1, 1), (1, 8, 8), (9, 3, 5), (5, 32, 32), (40, 7, 16), (301, 8, 8), (4, 31, 2),
+                                         (1, 1, 32), (130, 2, 4)])
+@pytest.mark.parametrize("masked, finished", [(False, False), (True, True)])
+def test_joint_selection(dtype, G, K, width, masked, finished):
+    x, s, m, f = _inputs(G, K, 18, dtype, masked, finished, G + K)
+    if masked:
+        m[:, :, [0, 3, 6, 9, 11, 13, 16]] |= True     # the neutral choices
+        m[0, K - 1, 9:11] = False                     # a head without a legal choice
+    _check(x, s, m, f, width, HEADS, sum_error=1e-12)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [40, 5000])
+def test_flat_selection_edge_values(V):
+    """NaN and infinities, allowed and masked; empty rows; fewer continuations than places; -0 and +0."""
+    import torch
+
+    rng = np.random.default_rng(5)
+    x, s, m, _ = _inputs(12, 4, V, "float32", True, False, 9)
+    low = torch.finfo(torch.float32).min
+    x[0, 0, 3], m[0, 0, 3] = math.nan, True          # kills its beam
+    x[1, 1, 4], m[1, 1, 4] = math.inf, True
+    x[2, 0, :5], m[2, 0, :5] = math.nan, False       # masked: never looked at
+    x[2, 1, :5], m[2, 1, :5] = math.inf, False
+    x[3, :, 2:] = -math.inf                          # two continuations a beam at most
+    x[4] = low                                       # the type's lowest value everywhere
+    m[5] = False                                     # a group without a continuation
+    m[6] = False
+    m[6, 2, V - 1] = True                            # exactly one
+    x[7] = 0.0
+    x[7, :, ::2] = -0.0                              # equal to +0: ties by index
+    s[7] = -1.0
+    m[7] = True
+    x[8, 0], m[8, 0] = math.nan, True                # every allowed logit is NaN
+    s[9, 1], s[9, 2], s[9, 3] = math.nan, -math.inf, -1e30
+    x[10, 0, 0], m[10, 0, 0] = 1e30, True            # one logit takes all
+    x[11] = torch.from_numpy(rng.integers(0, 3, (4, V)).astype(np.float32))   # many ties
+    _check(x, s, m, None, 16)
+
+
+@pytest.mark.gpu
+def test_near_totals_are_ranked_in_64_bits():
+    """Beams whose normalisers differ by less than float32 sums can tell."""
+    import torch
+
+    rng = np.random.default_rng(11)
+    for V in (600, 20011):
+        row = rng.normal(0, 2, V).astype(np.float32)
+        x = np.tile(row, (6, 8, 1))
+        x[:, :, V // 2] = -8 - 8 * rng.random((6, 8)).astype(np.float32)     # e^-8 .. e^-16 of a sum of about e^2 V
+        x[5] = row                                                           # equal beams: ties by index
+        s = np.full((6, 8), -2.0, np.float32)
+        _check(torch.from_numpy(x), torch.from_numpy(s), None, None, 24)
+        fin = np.zeros((6, 8), bool)
+        fin[:, 3] = True                             # a finished beam right at another's best total
+        es, _, _ = best_continuations(x, s, None, None, 1)
+        s2 = s.copy()
+        s2[:, 3] = es[:, 0].astype(np.float32)
+        _check(torch.from_numpy(x), torch.from_numpy(s2), None, torch.from_numpy(fin), 24)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_joint_ties_between_heads(dtype):
+    """Small whole logits: many joint actions have exactly the same sum."""
+    import torch
+
+    rng = np.random.default_rng(3)
+    x = torch.from_numpy(rng.integers(-1, 2, (20, 6, 18)).astype(np.float32)).to(getattr(torch, dtype))
+    x[10:] = x[10:, :1]                              # equal beams too
+    s = torch.full((20, 6), -3.0)
+    _check(x, s, None, None, 32, HEADS, sum_error=1e-12)
+    x = x.float()
+    x[0, 0, 1], x[1, 1, 5], x[2, 2, 17] = math.nan, math.inf, -math.inf
+    x[3, 0, 0:3] = -math.inf
+    s[4, 0], s[5, 1] = math.nan, -math.inf
+    _check(x.to(getattr(torch, dtype)), s, None, None, 32, HEADS, sum_error=1e-12)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("joint", [False, True])
+def test_selection_layouts(joint):
+    """Broadcast masks, strided and offset logits, more leading dimensions, none, no groups."""
+    import torch
+    from carl_b200.action import CARLActionCodec
+    from carl_b200.search import beam_select
+
+    fn = CARLActionCodec().beam_select if joint else beam_select
+    heads, V = (HEADS, 18) if joint else (None, 77)
+    x, s, m, f = _inputs(6, 5, V, "bfloat16", True, True, 21)
+    _check(x, s, m[:1, :1], None, 5, heads)                        # [1, 1, V]
+    _check(x, s, m[0, 0], f, 5, heads)                             # [V]
+    _check(x, s, torch.ones(6, 5, 1, dtype=torch.bool), f, 5, heads)
+    want = fn(x.cuda(), s.cuda(), m.cuda(), finished=f.cuda())
+    wide = torch.full((6, 5, V + 9), 99.0, dtype=torch.bfloat16, device="cuda")
+    wide[..., 3:3 + V] = x.cuda()
+    wide_m = torch.zeros((6, 5, V + 5), dtype=torch.bool, device="cuda")
+    wide_m[..., 1:1 + V] = m.cuda()
+    views = [(wide[..., 3:3 + V], wide_m[..., 1:1 + V]),
+             (x.cuda().transpose(0, 1).contiguous().transpose(0, 1), m.cuda().transpose(1, 2).contiguous().transpose(1, 2)),
+             (x.cuda().transpose(1, 2).contiguous().transpose(1, 2), m.cuda())]
+    for vx, vm in views:
+        got = fn(vx, s.cuda(), vm, finished=f.cuda())
+        assert torch.equal(got.parents, want.parents) and torch.equal(got.actions, want.actions)
+        # A row's alignment decides which of its terms are summed together, so each side has the
+        # normaliser's error of its own (2 * SUM_ERROR) and its own rounding (2 * 2^-24).
+        live = torch.isfinite(want.scores)
+        assert torch.equal(live, torch.isfinite(got.scores))
+        off = (got.scores.double() - want.scores.double())[live].abs()
+        assert (off <= 2 * SUM_ERROR + 2.0 ** -23 * want.scores[live].abs()).all()
+    got = fn(x.cuda().view(2, 3, 5, V), s.cuda().view(2, 3, 5), m.cuda().view(2, 3, 5, V), finished=f.cuda().view(2, 3, 5))
+    assert got.parents.shape == (2, 3, 5) and torch.equal(got.parents.view(6, 5), want.parents)
+    one = fn(x[2].cuda(), s[2].cuda(), m[2].cuda(), finished=f[2].cuda())
+    assert torch.equal(one.parents, want.parents[2]) and torch.equal(one.actions, want.actions[2])
+    none = fn(x[:0].cuda(), s[:0].cuda())
+    assert none.scores.shape == (0, 5)
+    same = fn(x[:1].cuda().expand(4, 5, V), s[:1].cuda().expand(4, 5))   # broadcast groups
+    assert torch.equal(same.parents[0], same.parents[3])
+
+
+@pytest.mark.gpu
+def test_selection_refusals_on_the_device():
+    import torch
+    from carl_b200.search import beam_select
+
+    x, s = torch.zeros(2, 4, 9, device="cuda"), torch.zeros(2, 4, device="cuda")
+    for exc, call in [(TypeError, lambda: beam_select(x.double(), s)), (TypeError, lambda: beam_select(x, s.half())),
+                      (ValueError, lambda: beam_select(x, s[:1])), (ValueError, lambda: beam_select(x[0, 0], s[0, 0])),
+                      (TypeError, lambda: beam_select(x, s, x)), (ValueError, lambda: beam_select(x, s, s.bool())),
+                      (ValueError, lambda: beam_select(x, s, width=0)), (ValueError, lambda: beam_select(x, s, width=129)),
+                      (TypeError, lambda: beam_select(x, s, finished=s)), (ValueError, lambda: beam_select(x, s.cpu())),
+                      (ValueError, lambda: beam_select(x, s, finished=s[:, :2].bool())),
+                      (ValueError, lambda: beam_select(x[..., :0], s))]:
+        with pytest.raises(exc):
+            call()
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Rows more than 2^31 elements apart, by stride."""
+    import torch
+    from carl_b200.search import beam_select
+
+    far = 2 ** 31 + 64
+    store = torch.empty(far + 2 * 4096, dtype=torch.bfloat16, device="cuda")
+    x = torch.as_strided(store, (2, 2, 4096), (far, 4096, 1))
+    small = torch.randn(2, 2, 4096, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).bfloat16()
+    x.copy_(small)
+    s = torch.zeros(2, 2, device="cuda")
+    a, b = beam_select(x, s), beam_select(small, s)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+# ---- reordering -------------------------------------------------------------------------
+
+
+def _reordered(t, parents, dim):
+    import torch
+
+    K = parents.shape[-1]
+    p = parents.reshape(-1, K)
+    own = torch.arange(K, device=p.device)
+    p = torch.where((p >= 0) & (p < K), p, own)
+    source = (p + torch.arange(0, p.numel(), K, device=p.device)[:, None]).flatten()
+    return t.index_select(dim, source)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("G, K", [(1, 1), (1, 8), (5, 3), (64, 8), (2, 64), (1, 1024), (37, 7), (3, 1000)])
+def test_reorder_rows_and_words(G, K):
+    import torch
+    from carl_b200.search import reorder_states
+
+    g = torch.Generator("cuda").manual_seed(G * 1000 + K)
+    n = G * K
+    parents = torch.randint(-2, K + 2, (G, K), device="cuda", generator=g)     # some name no beam
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    rows = [rand(n, 6, 63), rand(n, 5).bfloat16(), rand(n) > 0, rand(n, 3).half(), rand(n, 1000), rand(n, 7, 13).to(torch.uint8),
+            rand(n, 2).double(), rand(n, 0), rand(n, 4099).bfloat16()]
+    want = [_reordered(t, parents, 0) for t in rows]
+    reorder_states(rows, parents)
+    assert all(torch.equal(a, b) for a, b in zip(rows, want))
+    words = [rand(76, n, 6), rand(33, n, 1), rand(5, n), rand(3, 2, n, 4).bfloat16().movedim(2, 1).contiguous()]
+    want = [_reordered(t, parents, 1) for t in words]
+    reorder_states(words, parents, dim=1)
+    assert all(torch.equal(a, b) for a, b in zip(words, want))
+    odd = torch.randn(n * 6 + 1, device="cuda")[1:].view(n, 6)                 # 4-byte aligned only
+    want = _reordered(odd, parents, 0)
+    reorder_states([odd], parents)
+    assert torch.equal(odd, want)
+
+
+@pytest.mark.gpu
+def test_reorder_many_arrays_and_neighbours():
+    """More arrays than one launch takes; nothing around an array is touched."""
+    import torch
+    from carl_b200.search import reorder_states
+
+    g = torch.Generator("cuda").manual_seed(3)
+    parents = torch.randint(0, 5, (4, 5), device="cuda", generator=g)
+    store = [torch.randn(22, 3 + k, device="cuda", generator=g) for k in range(60)]
+    before = [t.clone() for t in store]
+    reorder_states([t[1:21] for t in store], parents.view(2, 2, 5))
+    for t, b in zip(store, before):
+        assert torch.equal(t[0], b[0]) and torch.equal(t[21], b[21])
+        assert torch.equal(t[1:21], _reordered(b[1:21], parents, 0))
+    reorder_states([], parents)
+    reorder_states([torch.zeros(0, 4, device="cuda")], parents[:0])
+    with pytest.raises(ValueError):
+        reorder_states([store[0]], parents)                      # 22 rows
+    with pytest.raises(ValueError):
+        reorder_states([store[0][:20].t()], parents, dim=1)      # not contiguous
+    with pytest.raises(ValueError):
+        reorder_states([store[0][:20]], parents, dim=2)
+    with pytest.raises(ValueError):
+        reorder_states([torch.zeros(20, 2, device="cuda", requires_grad=True)], parents)
+    with pytest.raises(ValueError):
+        reorder_states([torch.zeros(1025, device="cuda")], torch.zeros(1, 1025, dtype=torch.int64, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_reorder_beyond_32_bits():
+    import torch
+    from carl_b200.search import reorder_states
+
+    t = torch.zeros(4, 2 ** 31 + 16, dtype=torch.uint8, device="cuda")
+    t[:, -1] = torch.arange(4, device="cuda")
+    t[:, 7] = 10 + torch.arange(4, device="cuda")
+    reorder_states([t], torch.tensor([[1, 0], [1, 1]], device="cuda"))
+    assert t[:, -1].tolist() == [1, 0, 3, 3] and t[:, 7].tolist() == [11, 10, 13, 13]
+
+
+@pytest.mark.gpu
+def test_env_reorder(tmp_path, monkeypatch):
+    """Every persistent field and output buffer of a sim becomes its parent's; copies go on alike."""
+    import torch
+    from box_arena import write_box
+    from carl_b200 import carl, workloads
+
+    monkeypatch.setenv("CARL_ARENA_OBJ", str(write_box(tmp_path / "box.obj")))
+    n, K, nc = 24, 4, 6
+    env = carl.Env(n, 3, 3, 3)
+    workloads.mixed_state(env._env, 4)
+    rng = np.random.default_rng(5)
+    act = lambda: torch.from_numpy(workloads.discrete_actions(rng, n * nc).reshape(n, nc, 7)).cuda()  # noqa: E731
+    for _ in range(3):
+        env.step(act())
+    victim = rng.integers(-1, n * nc, (n * nc, 1)).astype(np.int32)
+    env._env.write_field("CAR_CONTACT_IDX", victim)
+    parents = torch.from_numpy(rng.integers(-1, K + 1, (n // K, K))).cuda()
+    p = parents.cpu().numpy().ravel()
+    slot = np.arange(n) % K
+    source = np.where((p >= 0) & (p < K), np.arange(n) - slot + p, np.arange(n))
+    before = env._env.snapshot()
+    torch.cuda.synchronize()
+    buffers = [env._buffer(b).clone() for b in range(12)]
+    env.reorder(parents)
+    after = env._env.snapshot()
+    torch.cuda.ExternalStream(env.stream).synchronize()
+    for b in range(12):
+        assert torch.equal(env._buffer(b), buffers[b][torch.from_numpy(source).cuda()]), b
+    for name, words in before.items():
+        per = words.shape[0] // n
+        if name == "TICK_COUNT":
+            assert np.array_equal(after[name], words)
+            continue
+        want = words.reshape(n, per, -1)[source].reshape(words.shape)
+        if name == "CAR_CONTACT_IDX":
+            v = want.view(np.int32)[:, 0]
+            moved = np.repeat((np.arange(n) - source) * nc, nc)
+            want = np.where(v >= 0, v + moved, v).astype(np.int32).view(np.uint32)[:, None]
+        assert np.array_equal(after[name], want), name
+    # Copies of one parent under the same actions stay bit-identical.
+    a = act()
+    env.step(a[torch.from_numpy(source).cuda()].contiguous())
+    snap = env._env.snapshot()
+    twins = [(i, j) for i in range(n) for j in range(i) if source[i] == source[j]]
+    assert twins
+    for i, j in twins:
+        assert np.array_equal(snap["CAR_POS"].reshape(n, -1)[i], snap["CAR_POS"].reshape(n, -1)[j])
+        assert np.array_equal(snap["BALL_POS"][i], snap["BALL_POS"][j])
+    for bad in (parents.int(), parents.view(-1), parents.cpu(), parents.t(), parents[:2],
+                torch.zeros(n // 5, 5, dtype=torch.int64, device="cuda")):
+        with pytest.raises((TypeError, ValueError)):
+            env.reorder(bad)
+    env.close()
+
+
+# ---- streams and graphs ------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_selection_and_reorder_in_a_graph_and_on_a_stream():
+    import torch
+    from carl_b200.action import CARLActionCodec
+    from carl_b200.search import beam_select, reorder_states
+
+    codec = CARLActionCodec()
+    x, s, _, _ = _inputs(5, 8, 3001, "float32", False, False, 2)
+    x18 = x[..., :18].contiguous().cuda()
+    x, s = x.cuda(), s.cuda()
+    hidden = torch.randn(40, 33, device="cuda")
+
+    def step():
+        best = beam_select(x, s)
+        joint = codec.beam_select(x18, best.scores)
+        reorder_states([hidden], joint.parents)
+        return best, joint
+
+    start = hidden.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = step()
+    torch.cuda.current_stream().wait_stream(side)
+    after = hidden.clone()
+    hidden.copy_(start)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = step()
+    for k in range(3):
+        hidden.copy_(start)
+        if k == 1:
+            s.sub_(1.0)          # a uniform shift: the same choice
+        graph.replay()
+        for a, b in zip(want, got):
+            assert torch.equal(a.parents, b.parents) and torch.equal(a.actions, b.actions)
+        assert torch.equal(hidden, after)
