@@ -62,11 +62,13 @@ struct GroupKey
     unsigned i;
 };
 
+__device__ __forceinline__ bool better(unsigned a, unsigned b) { return a > b; }
 __device__ __forceinline__ bool better(RowKey a, RowKey b) { return a > b; }
 __device__ __forceinline__ bool better(const GroupKey& a, const GroupKey& b)
 {
     return a.t > b.t || (a.t == b.t && a.i > b.i);
 }
+__device__ __forceinline__ unsigned shflXor(unsigned k, int m) { return __shfl_xor_sync(FULL, k, m); }
 __device__ __forceinline__ RowKey shflXor(RowKey k, int m) { return __shfl_xor_sync(FULL, k, m); }
 __device__ __forceinline__ GroupKey shflXor(const GroupKey& k, int m)
 {
@@ -78,33 +80,37 @@ __device__ __forceinline__ GroupKey shflAt(const GroupKey& k, int l)
     return GroupKey{ __shfl_sync(FULL, k.t, l), __shfl_sync(FULL, k.i, l) };
 }
 
-// Element p of a list of 32 E keys is register p / 32 of lane p % 32.
+// Element p of a list of 32 E keys is register p / 32 of lane p % 32.  The loops over
+// strides within a warp stay rolled: unrolled they made most of the library's code.
 template <class Key, int E>
-__device__ __forceinline__ void exchange(Key (&v)[E], int stride, int size, int lane)
+__device__ __forceinline__ void exchangeLanes(Key (&v)[E], int stride, int size, int lane)
 {
-    if (stride >= 32)
+#pragma unroll
+    for (int e = 0; e < E; e++)
     {
-        const int d = stride / 32;
+        const bool down = ((e * 32 + lane) & size) == 0;
+        const Key o = shflXor(v[e], stride);
+        const bool first = (lane & stride) == 0;
+        if (better(o, v[e]) == (first == down)) v[e] = o;
+    }
+}
+
+template <class Key, int E>
+__device__ __forceinline__ void exchangeRegisters(Key (&v)[E], int size, int lane)
+{
+#pragma unroll
+    for (int d = E / 2; d > 0; d /= 2)
+    {
+        if (32 * d >= size) continue;
 #pragma unroll
         for (int e = 0; e < E; e++)
         {
             if (e & d) continue;
             const bool down = ((e * 32 + lane) & size) == 0;
-            const Key a = v[e], b = v[(e | d) < E ? (e | d) : e];
-            const bool ok = better(b, a) != down;
-            v[e] = ok ? a : b;
-            v[(e | d) < E ? (e | d) : e] = ok ? b : a;
-        }
-    }
-    else
-    {
-#pragma unroll
-        for (int e = 0; e < E; e++)
-        {
-            const bool down = ((e * 32 + lane) & size) == 0;
-            const Key o = shflXor(v[e], stride);
-            const bool first = (lane & stride) == 0;
-            if (better(o, v[e]) == (first == down)) v[e] = o;
+            const Key a = v[e], b = v[e | d];
+            const bool swap = better(b, a) == down;
+            v[e] = swap ? b : a;
+            v[e | d] = swap ? a : b;
         }
     }
 }
@@ -113,10 +119,13 @@ __device__ __forceinline__ void exchange(Key (&v)[E], int stride, int size, int 
 template <class Key, int E>
 __device__ __forceinline__ void sortDown(Key (&v)[E], int lane)
 {
-#pragma unroll
+#pragma unroll 1
     for (int size = 2; size <= 32 * E; size *= 2)
-#pragma unroll
-        for (int stride = size / 2; stride > 0; stride /= 2) exchange(v, stride, size, lane);
+    {
+        exchangeRegisters(v, size, lane);
+#pragma unroll 1
+        for (int stride = min(16, size / 2); stride > 0; stride /= 2) exchangeLanes(v, stride, size, lane);
+    }
 }
 
 // The 32 E largest of two sorted lists, sorted.
@@ -129,8 +138,9 @@ __device__ __forceinline__ void mergeDown(Key (&list)[E], const Key (&other)[E],
         const Key o = shflAt(other[E - 1 - e], 31 - lane);
         if (better(o, list[e])) list[e] = o;
     }
-#pragma unroll
-    for (int stride = 16 * E; stride > 0; stride /= 2) exchange(list, stride, 64 * E, lane);
+    exchangeRegisters(list, 64 * E, lane);
+#pragma unroll 1
+    for (int stride = 16; stride > 0; stride /= 2) exchangeLanes(list, stride, 64 * E, lane);
 }
 
 // The best keys a warp has seen: a sorted list, and a buffer of the keys that
@@ -243,64 +253,71 @@ __device__ __forceinline__ bool readsLogits(const BeamParams& p, long long row)
 
 // ---- the pass over the logits --------------------------------------------------------
 
-constexpr int ROW_WARPS = 8;
+// The `n`-th largest (n <= 32 E) of E values a lane, as an ordered image.
+template <int E>
+__device__ __forceinline__ unsigned nthLargest(unsigned (&v)[E], int n, int lane)
+{
+    if (E == 1 && n <= 12)
+    {
+        // Fewer rounds of taking the maximum out than a sort has exchanges.
+        unsigned mine = v[0], top = 0;
+        for (int left = n; left > 0;)
+        {
+            top = __reduce_max_sync(FULL, mine);
+            const bool hit = mine == top;
+            left -= __popc(__ballot_sync(FULL, hit));
+            if (hit) mine = 0;
+            if (top == 0) break;
+        }
+        return top;
+    }
+    sortDown(v, lane);
+    unsigned r = v[0];
+#pragma unroll
+    for (int e = 1; e < E; e++)
+        if ((n - 1) / 32 == e) r = v[e];
+    return __shfl_sync(FULL, r, (n - 1) & 31);
+}
 
-// One warp per segment of a row: the segment's largest logits, their maximum and
-// the sum of exp(x - maximum).
+// One warp over a segment of a row: the segment's largest logits (sorted, in `best`),
+// their maximum and, per lane, a part of the sum of exp(x - maximum).
+//
+// Tiles of 1024 elements are held in registers, 32 a lane.  A tile whose maximum
+// does not reach the list's last place costs its loads, the exponentials and one
+// vote.  The first tile has no such bar yet: the width-th largest of the lanes'
+// maxima is one, since at least `width` elements reach it.
 template <class T, int E, bool MASKED>
-__global__ void __launch_bounds__(ROW_WARPS * 32) selectRowsKernel(BeamParams p)
+__device__ __forceinline__ void scanRow(const BeamParams& p, const T* x, const uint8_t* allowed, int seg, int segs,
+                                        RowKey* wait, int lane, BestList<RowKey, E>& best, float& top, double& sum)
 {
     constexpr int VE = 16 / sizeof(T);  // elements of a 16-byte load
-    constexpr int NV = 32 / VE;         // loads of a lane per tile of 1024 elements
-    __shared__ RowKey waitS[ROW_WARPS][32 * E + 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long item = blockIdx.x * (long long)ROW_WARPS + warp;
-    if (item >= (long long)p.groups * p.beams * p.segs) return;
-    const long long row = item / p.segs;
-    const int seg = (int)(item - row * p.segs);
-    if (!readsLogits(p, row)) return;
-    const long long g = row / p.beams, k = row - g * p.beams;
-    const T* x = static_cast<const T*>(p.logits) + g * p.groupStride + k * p.beamStride;
-    const uint8_t* allowed = MASKED ? p.mask + g * p.maskGroupStride + k * p.maskBeamStride : nullptr;
-
+    constexpr int NV = 32 / VE;         // loads of a lane per tile
     const int head = min(p.vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
     const int vectors = (p.vocab - head) / VE, tail = p.vocab - head - vectors * VE;
     const int tiles = (vectors + 32 * NV - 1) / (32 * NV);
-    const int t0 = (int)((long long)tiles * seg / p.segs), t1 = (int)((long long)tiles * (seg + 1) / p.segs);
+    const int t0 = (int)((long long)tiles * seg / segs), t1 = (int)((long long)tiles * (seg + 1) / segs);
     const bool wideMask = MASKED && (reinterpret_cast<uintptr_t>(allowed + head) % VE) == 0;
 
-    BestList<RowKey, E> best;
-    best.init(waitS[warp], p.width, lane);
-    float top = NEG_INF;
-    double sum = 0.0;
+    best.init(wait, p.width, lane);
+    top = NEG_INF;
+    sum = 0.0;
+    float bar = NEG_INF;  // nothing below it can be kept
+    bool started = false;
 
+    auto raise = [&]() {
+        if (best.bar) bar = fmaxf(bar, fromOrdered((unsigned)(best.bar >> 32)));
+    };
     auto absorb = [&](float laneTop) {
         if (laneTop != laneTop) laneTop = NEG_INF;  // NaN reaches the sum, not the maximum
-        const unsigned o = __reduce_max_sync(FULL, ordered(laneTop));
-        const float t = fromOrdered(o);
+        const float t = fromOrdered(__reduce_max_sync(FULL, ordered(laneTop)));
         if (t > top)
         {
             sum *= exp((double)top - (double)t);
             top = t;
         }
-    };
-    auto offer = [&](float v, int action) {
-        const float bar = best.bar ? fromOrdered((unsigned)(best.bar >> 32)) : NEG_INF;
-        const RowKey key = ((RowKey)ordered(v) << 32) | (unsigned)~action;
-        best.push(v >= bar && v > NEG_INF && key > best.bar, key);
+        return t;
     };
 
-    // The elements before the first and behind the last whole vector.
-    if (seg == 0 && head + tail > 0)
-    {
-        const bool front = lane < head, back = lane >= 8 && lane < 8 + tail;
-        const int a = front ? lane : head + vectors * VE + lane - 8;
-        float v = NEG_INF;
-        if ((front || back) && (!MASKED || allowed[a])) v = toFloat(x[a]);
-        absorb(v);
-        sum += exp2Approx((v - (top > NEG_INF ? top : 0.f)) * LOG2E);
-        offer(v, a);
-    }
     const uint4* xv = reinterpret_cast<const uint4*>(x + head);
     for (int t = t0; t < t1; t++)
     {
@@ -312,10 +329,17 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) selectRowsKernel(BeamParams p)
             const int i = (t * NV + j) * 32 + lane;
             if (i < vectors) raw[j] = __ldcs(xv + i);
         }
+        float part[4];
 #pragma unroll
         for (int j = 0; j < NV; j++)
         {
             const int i = (t * NV + j) * 32 + lane;
+            if ((t * NV + j) * 32 >= vectors)  // the same for the whole warp
+            {
+#pragma unroll
+                for (int q = 0; q < VE; q++) v[j * VE + q] = NEG_INF;
+                continue;
+            }
             float f[VE];
             unpack(raw[j], f, T());
             bool ok[VE];
@@ -341,29 +365,103 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) selectRowsKernel(BeamParams p)
 #pragma unroll
             for (int q = 0; q < VE; q++) v[j * VE + q] = ok[q] ? f[q] : NEG_INF;
         }
-        float laneTop = v[0];
 #pragma unroll
-        for (int j = 1; j < 32; j++) laneTop = fmaxf(laneTop, v[j]);
-        absorb(laneTop);
+        for (int k = 0; k < 4; k++)
+        {
+            part[k] = v[8 * k];
+#pragma unroll
+            for (int q = 1; q < 8; q++) part[k] = fmaxf(part[k], v[8 * k + q]);
+        }
+        const float laneTop = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+        const float tileTop = absorb(laneTop);
         const float ref = top > NEG_INF ? top : 0.f;
 #pragma unroll
         for (int j = 0; j < 32; j += 8)
         {
+            if ((t * NV + j / VE) * 32 >= vectors) break;
             float s = 0.f;
 #pragma unroll
             for (int q = 0; q < 8; q++) s += exp2Approx((v[j + q] - ref) * LOG2E);
             sum += s;
         }
-        const float bar = best.bar ? fromOrdered((unsigned)(best.bar >> 32)) : NEG_INF;
-        if (__any_sync(FULL, laneTop >= bar && laneTop > NEG_INF))
+        if (!(tileTop >= bar && tileTop > NEG_INF)) continue;
+        if (!started)
         {
+            started = true;
+            unsigned tops[E];
 #pragma unroll
-            for (int j = 0; j < 32; j++) offer(v[j], head + ((t * NV + j / VE) * 32 + lane) * VE + j % VE);
+            for (int e = 0; e < E; e++)
+            {
+                float m = part[e * (4 / E)];
+#pragma unroll
+                for (int k = 1; k < 4 / E; k++) m = fmaxf(m, part[e * (4 / E) + k]);
+                tops[e] = m > NEG_INF ? ordered(m) : 0;
+            }
+            const unsigned o = nthLargest<E>(tops, p.width, lane);
+            if (o) bar = fromOrdered(o);
         }
+        unsigned bits = 0;
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+            if (v[j] >= bar && v[j] > NEG_INF) bits |= 1u << j;
+        while (__any_sync(FULL, bits != 0))
+        {
+            const bool has = bits != 0;
+            const int j = has ? __ffs(bits) - 1 : 0;
+            bits &= bits - 1;
+            const int action = head + ((t * NV + j / VE) * 32 + lane) * VE + j % VE;
+            RowKey key = 0;
+            if (has) key = (RowKey)ordered(toFloat(x[action])) << 32 | (unsigned)~action;
+            best.push(has && key > best.bar, key);
+        }
+        raise();
+    }
+    // The elements before the first and behind the last whole vector.
+    if (seg == 0 && head + tail > 0)
+    {
+        const bool front = lane < head, back = lane >= 8 && lane < 8 + tail;
+        const int a = front ? lane : head + vectors * VE + lane - 8;
+        float v = NEG_INF;
+        if ((front || back) && (!MASKED || allowed[a])) v = toFloat(x[a]);
+        absorb(v);
+        sum += exp2Approx((v - (top > NEG_INF ? top : 0.f)) * LOG2E);
+        const RowKey key = (RowKey)ordered(v) << 32 | (unsigned)~a;
+        best.push(v >= bar && v > NEG_INF && key > best.bar, key);
     }
     best.finish();
 #pragma unroll
     for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
+}
+
+template <class T>
+__device__ __forceinline__ const T* rowLogits(const BeamParams& p, long long g, int k)
+{
+    return static_cast<const T*>(p.logits) + g * p.groupStride + k * p.beamStride;
+}
+__device__ __forceinline__ const uint8_t* rowMask(const BeamParams& p, long long g, int k)
+{
+    return p.mask ? p.mask + g * p.maskGroupStride + k * p.maskBeamStride : nullptr;
+}
+
+constexpr int ROW_WARPS = 8;
+constexpr int ROW_THREADS = ROW_WARPS * 32;
+
+// One warp per segment of a row, results to the workspace.
+template <class T, int E, bool MASKED>
+__global__ void __launch_bounds__(ROW_THREADS) selectRowsKernel(BeamParams p)
+{
+    __shared__ RowKey waitS[ROW_WARPS][32 * E + 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long item = blockIdx.x * (long long)ROW_WARPS + warp;
+    if (item >= (long long)p.groups * p.beams * p.segs) return;
+    const long long row = item / p.segs, g = row / p.beams;
+    if (!readsLogits(p, row)) return;
+    const int k = (int)(row - g * p.beams);
+    BestList<RowKey, E> best;
+    float top;
+    double sum;
+    scanRow<T, E, MASKED>(p, rowLogits<T>(p, g, k), rowMask(p, g, k), (int)(item - row * p.segs), p.segs, waitS[warp], lane,
+                          best, top, sum);
     if (lane == 0)
     {
         p.top[item] = top;
@@ -376,132 +474,133 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) selectRowsKernel(BeamParams p)
 
 // ---- the merge of a group --------------------------------------------------------------
 
-constexpr int MERGE_WARPS = 8;
-constexpr int MERGE_THREADS = MERGE_WARPS * 32;
-
 // Totals of different beams are compared through normalisers that the pass above
-// has to fp32 accuracy in its terms.  Its error in the logarithm of a sum: per term
-// the rounding of x - top and of its product with log2(e) (2^-24 each, and 2^-26 for
-// the constant) times |x - top|, whose mean under the softmax is at most
-// log(vocab) <= 21.5; ex2.approx's 2^-22; seven additions of 2^-24.  Together below
-// 3.5e-6, so two totals that are further apart than twice that are in order.  Nearer
-// ones are decided by normalisers in 64 bits.
+// has to fp32 accuracy in its terms.  With u = 2^-24 and d = top - x: a term is off by
+// d u (the difference), 1.25 d u (its product with log2(e), and that constant) and 4 u
+// (ex2.approx); d averages at most log(vocab) <= 20.8 under the softmax; partial sums of
+// eight terms add 7 u.  Together 58 u = 3.5e-6, so two totals that are further apart
+// than twice that are in order.  Nearer ones are decided by normalisers in 64 bits.
 constexpr double NEAR_TOTALS = 8e-6;
 
-// Sorted best of the block's warps in listS[0] (all threads return after it is there).
 template <int E>
-__device__ void mergeWarps(BestList<GroupKey, E>& best, GroupKey (*listS)[32 * E + 32], int warp, int lane)
+struct MergeShared
 {
-    __syncthreads();  // the buffers of waiting keys become the lists
-#pragma unroll
-    for (int e = 0; e < E; e++) listS[warp][e * 32 + lane] = best.list[e];
-    __syncthreads();
-    for (int n = MERGE_WARPS / 2; n > 0; n /= 2)
-    {
-        if (warp < n)
-        {
-            GroupKey other[E];
-#pragma unroll
-            for (int e = 0; e < E; e++) other[e] = listS[warp + n][e * 32 + lane];
-            mergeDown(best.list, other, lane);
-#pragma unroll
-            for (int e = 0; e < E; e++) listS[warp][e * 32 + lane] = best.list[e];
-        }
-        __syncthreads();
-    }
-}
+    GroupKey wait[ROW_WARPS][32 * E + 32];
+    double red[ROW_WARPS];
+    unsigned near[BEAM_MAX_BEAMS / 32];
+    unsigned repair;
+};
 
+// A block merges the lists of its group's rows (`keys` [beams, segs, width], `tops`
+// and `sums` [beams, segs]) and writes the group's outputs.  base: [beams] doubles of
+// shared memory.
 template <class T, int E>
-__global__ void __launch_bounds__(MERGE_THREADS) selectMergeKernel(BeamParams p)
+__device__ void mergeGroup(const BeamParams& p, long long g, const RowKey* keys, const float* tops, const double* sums,
+                           int segs, double* base, MergeShared<E>& sh)
 {
-    __shared__ double baseS[BEAM_MAX_BEAMS];   // score minus normaliser; -inf: no candidate among the lists
-    __shared__ GroupKey waitS[MERGE_WARPS][32 * E + 32];
-    __shared__ unsigned nearS[BEAM_MAX_BEAMS / 32];
-    __shared__ double redS[MERGE_WARPS];
-    __shared__ unsigned repairS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const long long g = blockIdx.x, row0 = g * p.beams;
-    const int K = p.beams, per = p.segs * p.width;
+    const long long row0 = g * p.beams;
+    const int K = p.beams, per = segs * p.width, n = K * per;
 
-    for (int k = tid; k < K; k += MERGE_THREADS)
+    for (int k = tid; k < K; k += ROW_THREADS)
     {
-        double base = NEG_INF;
+        double b = NEG_INF;
         if (readsLogits(p, row0 + k))
         {
-            const float* top = p.top + (row0 + k) * p.segs;
-            const double* sum = p.sum + (row0 + k) * p.segs;
             float t = NEG_INF;
-            for (int s = 0; s < p.segs; s++) t = fmaxf(t, top[s]);
-            double n = 0.0;
+            for (int s = 0; s < segs; s++) t = fmaxf(t, tops[k * segs + s]);
             if (t > NEG_INF)
             {
-                for (int s = 0; s < p.segs; s++)
+                double sum = 0.0;
+                for (int s = 0; s < segs; s++)
                 {
                     // A segment without a finite logit has sum 0, or NaN where one was NaN.
-                    n += top[s] > NEG_INF ? sum[s] * exp((double)top[s] - (double)t) : sum[s];
+                    const float ts = tops[k * segs + s];
+                    sum += ts > NEG_INF && ts < t ? sums[k * segs + s] * exp((double)ts - (double)t) : sums[k * segs + s];
                 }
-                base = (double)p.scores[row0 + k] - ((double)t + log(n));
+                b = (double)p.scores[row0 + k] - ((double)t + log(sum));
             }
         }
-        baseS[k] = base;
+        base[k] = b;
     }
-    for (int k = tid; k < BEAM_MAX_BEAMS / 32; k += MERGE_THREADS) nearS[k] = 0;
-    if (tid == 0) repairS = 0;
+    for (int k = tid; k < BEAM_MAX_BEAMS / 32; k += ROW_THREADS) sh.near[k] = 0;
+    if (tid == 0) sh.repair = 0;
     __syncthreads();
 
-    auto totalOf = [&](long long c, int& beam, unsigned& index) {
-        beam = (int)(c / per);
-        const double base = baseS[beam];
-        if (!(base > NEG_INF)) return (double)NEG_INF;
-        const RowKey key = p.keys[row0 * per + c];
+    auto totalOf = [&](int c, int& beam, unsigned& index) {
+        beam = c / per;
+        const double b = base[beam];
+        if (!(b > NEG_INF)) return (double)NEG_INF;
+        const RowKey key = keys[c];
         if (!key) return (double)NEG_INF;
         index = (unsigned)beam * p.vocab + ~(unsigned)key;
-        return base + (double)fromOrdered((unsigned)(key >> 32));
+        return b + (double)fromOrdered((unsigned)(key >> 32));
     };
-    const long long n = (long long)K * per;
-    BestList<GroupKey, E> best;
+    // Few candidates are one warp's work; more are shared out and merged pairwise.
+    const int warps = n <= 256 * E ? 1 : ROW_WARPS;
     auto choose = [&]() {
-        best.init(waitS[warp], p.width, lane);
-        for (long long c0 = warp * 32; c0 < n; c0 += MERGE_THREADS)
+        BestList<GroupKey, E> best;
+        if (warp < warps)
         {
-            const long long c = c0 + lane;
-            int beam = 0;
-            unsigned index = 0;
-            const double total = c < n ? totalOf(c, beam, index) : NEG_INF;
-            const GroupKey key{ ordered64(total), ~index };
-            best.push(total > NEG_INF && better(key, best.bar), key);
+            best.init(sh.wait[warp], p.width, lane);
+            for (int c0 = warp * 32; c0 < n; c0 += warps * 32)
+            {
+                const int c = c0 + lane;
+                int beam = 0;
+                unsigned index = 0;
+                const double total = c < n ? totalOf(c, beam, index) : NEG_INF;
+                const GroupKey key{ ordered64(total), ~index };
+                best.push(total > NEG_INF && better(key, best.bar), key);
+            }
+            for (int k0 = warp * 32; p.finished && k0 < K; k0 += warps * 32)
+            {
+                const int k = k0 + lane;
+                const double total = k < K && p.finished[row0 + k] ? (double)p.scores[row0 + k] : NEG_INF;
+                const GroupKey key{ ordered64(total), ~((unsigned)k * p.vocab) };
+                best.push(total > NEG_INF && better(key, best.bar), key);
+            }
+            best.finish();
+            __syncwarp();  // the buffer of waiting keys becomes the list
+#pragma unroll
+            for (int e = 0; e < E; e++) sh.wait[warp][e * 32 + lane] = best.list[e];
         }
-        for (int k0 = warp * 32; p.finished && k0 < K; k0 += MERGE_THREADS)
+        __syncthreads();
+        for (int m = warps / 2; m > 0; m /= 2)
         {
-            const int k = k0 + lane;
-            const double total = k < K && p.finished[row0 + k] ? (double)p.scores[row0 + k] : NEG_INF;
-            const GroupKey key{ ordered64(total), ~((unsigned)k * p.vocab) };
-            best.push(total > NEG_INF && better(key, best.bar), key);
+            if (warp < m)
+            {
+                GroupKey other[E];
+#pragma unroll
+                for (int e = 0; e < E; e++) other[e] = sh.wait[warp + m][e * 32 + lane];
+                mergeDown(best.list, other, lane);
+#pragma unroll
+                for (int e = 0; e < E; e++) sh.wait[warp][e * 32 + lane] = best.list[e];
+            }
+            __syncthreads();
         }
-        best.finish();
-        mergeWarps(best, waitS, warp, lane);
     };
     choose();
 
     // Beams whose totals are too near one another's: neighbours in the list, and what
     // lies around its last place.
-    const GroupKey last = waitS[0][p.width - 1];
-    auto mark = [&](int beam) { atomicOr(&nearS[beam >> 5], 1u << (beam & 31)); };
-    for (int i = tid; i + 1 < p.width; i += MERGE_THREADS)
+    const GroupKey* list = sh.wait[0];
+    const GroupKey last = list[p.width - 1];
+    auto mark = [&](int beam) { atomicOr(&sh.near[beam >> 5], 1u << (beam & 31)); };
+    for (int i = tid; i + 1 < p.width; i += ROW_THREADS)
     {
-        const GroupKey a = waitS[0][i], b = waitS[0][i + 1];
+        const GroupKey a = list[i], b = list[i + 1];
         if (!b.t || fromOrdered64(a.t) - fromOrdered64(b.t) > NEAR_TOTALS) continue;
         const int ka = ~a.i / p.vocab, kb = ~b.i / p.vocab;
         if (ka == kb) continue;
         mark(ka);
         mark(kb);
-        repairS = 1;
+        sh.repair = 1;
     }
     if (last.t)
     {
         const double edge = fromOrdered64(last.t);
         const int kl = ~last.i / p.vocab;
-        for (long long c = tid; c < n; c += MERGE_THREADS)
+        for (int c = tid; c < n; c += ROW_THREADS)
         {
             int beam;
             unsigned index;
@@ -509,46 +608,46 @@ __global__ void __launch_bounds__(MERGE_THREADS) selectMergeKernel(BeamParams p)
             if (beam == kl || !(fabs(total - edge) <= NEAR_TOTALS)) continue;
             mark(beam);
             mark(kl);
-            repairS = 1;
+            sh.repair = 1;
         }
-        for (int k = tid; p.finished && k < K; k += MERGE_THREADS)
+        for (int k = tid; p.finished && k < K; k += ROW_THREADS)
         {
             if (!p.finished[row0 + k] || k == kl || !(fabs((double)p.scores[row0 + k] - edge) <= NEAR_TOTALS)) continue;
             mark(kl);
-            repairS = 1;
+            sh.repair = 1;
         }
     }
     __syncthreads();
-    if (repairS)
+    if (sh.repair)
     {
         for (int k = 0; k < K; k++)
         {
-            if (!(nearS[k >> 5] >> (k & 31) & 1) || !readsLogits(p, row0 + k)) continue;  // the same for the whole block
-            const T* x = static_cast<const T*>(p.logits) + g * p.groupStride + k * p.beamStride;
-            const uint8_t* allowed = p.mask ? p.mask + g * p.maskGroupStride + k * p.maskBeamStride : nullptr;
+            if (!(sh.near[k >> 5] >> (k & 31) & 1) || !readsLogits(p, row0 + k)) continue;  // the same for the whole block
+            const T* x = rowLogits<T>(p, g, k);
+            const uint8_t* allowed = rowMask(p, g, k);
             float t = NEG_INF;
-            for (int s = 0; s < p.segs; s++) t = fmaxf(t, p.top[(row0 + k) * p.segs + s]);
+            for (int s = 0; s < segs; s++) t = fmaxf(t, tops[k * segs + s]);
             double sum = 0.0;
-            for (int a = tid; a < p.vocab; a += MERGE_THREADS)
+            for (int a = tid; a < p.vocab; a += ROW_THREADS)
                 if (!allowed || allowed[a]) sum += exp((double)toFloat(x[a]) - (double)t);
 #pragma unroll
             for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
-            if (lane == 0) redS[warp] = sum;
+            if (lane == 0) sh.red[warp] = sum;
             __syncthreads();
             if (tid == 0)
             {
                 sum = 0.0;
-                for (int w = 0; w < MERGE_WARPS; w++) sum += redS[w];
-                baseS[k] = (double)p.scores[row0 + k] - ((double)t + log(sum));
+                for (int w = 0; w < ROW_WARPS; w++) sum += sh.red[w];
+                base[k] = (double)p.scores[row0 + k] - ((double)t + log(sum));
             }
             __syncthreads();
         }
         choose();
     }
 
-    for (int i = tid; i < p.width; i += MERGE_THREADS)
+    for (int i = tid; i < p.width; i += ROW_THREADS)
     {
-        const GroupKey key = waitS[0][i];
+        const GroupKey key = list[i];
         const unsigned index = ~key.i;
         const long long o = g * p.width + i;
         p.outScores[o] = key.t ? (float)fromOrdered64(key.t) : NEG_INF;
@@ -557,91 +656,238 @@ __global__ void __launch_bounds__(MERGE_THREADS) selectMergeKernel(BeamParams p)
     }
 }
 
+template <class T, int E>
+__global__ void __launch_bounds__(ROW_THREADS) selectMergeKernel(BeamParams p)
+{
+    __shared__ double baseS[BEAM_MAX_BEAMS];
+    __shared__ MergeShared<E> sh;
+    const long long g = blockIdx.x, item0 = g * p.beams * p.segs;
+    mergeGroup<T, E>(p, g, p.keys + item0 * p.width, p.top + item0, p.sum + item0, p.segs, baseS, sh);
+}
+
+// Both in one block per group, where the group's rows are short or the groups many.
+constexpr int GROUP_MAX_BEAMS = 64;
+constexpr int GROUP_MAX_KEYS = 1024;
+
+template <class T, int E, bool MASKED>
+__global__ void __launch_bounds__(ROW_THREADS) selectGroupKernel(BeamParams p)
+{
+    __shared__ RowKey keyS[GROUP_MAX_KEYS];
+    __shared__ float topS[GROUP_MAX_BEAMS];
+    __shared__ double sumS[GROUP_MAX_BEAMS], baseS[GROUP_MAX_BEAMS];
+    __shared__ union { RowKey wait[ROW_WARPS][32 * E + 32]; MergeShared<E> merge; } sh;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long g = blockIdx.x;
+    for (int k = warp; k < p.beams; k += ROW_WARPS)
+    {
+        if (!readsLogits(p, g * p.beams + k)) continue;
+        BestList<RowKey, E> best;
+        float top;
+        double sum;
+        scanRow<T, E, MASKED>(p, rowLogits<T>(p, g, k), rowMask(p, g, k), 0, 1, sh.wait[warp], lane, best, top, sum);
+        if (lane == 0)
+        {
+            topS[k] = top;
+            sumS[k] = sum;
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (e * 32 + lane < p.width) keyS[k * p.width + e * 32 + lane] = best.list[e];
+        __syncwarp();
+    }
+    __syncthreads();
+    mergeGroup<T, E>(p, g, keyS, topS, sumS, 1, baseS, sh.merge);
+}
+
 // ---- selection over the action heads ---------------------------------------------------
 
 constexpr int HEADS = 7;
 constexpr int JOINT_ACTIONS = 3 * 3 * 3 * 2 * 2 * 3 * 2;
 __host__ __device__ constexpr int headSize(int h) { return h < 3 || h == 5 ? 3 : 2; }
 
-// One block per group.  The continuations of a beam are the 648 sums of one logit
-// per head; sums and normalisers are in 64 bits.
-template <class T>
-__global__ void __launch_bounds__(MERGE_THREADS) jointSelectKernel(BeamParams p)
+struct JointKey
 {
-    __shared__ double baseS[JOINT_MAX_BEAMS];
-    __shared__ double logitS[JOINT_MAX_BEAMS][ACTION_LOGITS];
-    __shared__ GroupKey waitS[MERGE_WARPS][64];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const long long g = blockIdx.x, row0 = g * p.beams;
-    const int K = p.beams;
-    for (int k = tid; k < K; k += MERGE_THREADS)
-    {
-        double base = NEG_INF;
-        if (readsLogits(p, row0 + k))
+    double v;  // sum of logits, then total; -inf: none
+    int i;     // action, then beam * JOINT_ACTIONS + action
+};
+
+__device__ __forceinline__ bool ahead(const JointKey& a, const JointKey& b) { return a.v > b.v || (a.v == b.v && a.i < b.i); }
+
+// Sorts a bitonic list, best first.
+template <int N>
+__device__ __forceinline__ void settle(JointKey (&l)[N])
+{
+#pragma unroll
+    for (int s = N / 2; s > 0; s /= 2)
+#pragma unroll
+        for (int i = 0; i < N; i++)
         {
-            const T* x = static_cast<const T*>(p.logits) + g * p.groupStride + k * p.beamStride;
-            const uint8_t* allowed = p.mask ? p.mask + g * p.maskGroupStride + k * p.maskBeamStride : nullptr;
-            double norm = 0.0;
-            int at = 0;
-            for (int h = 0; h < HEADS; h++)
-            {
-                double top = NEG_INF, sum = 0.0;
-                for (int q = 0; q < headSize(h); q++)
-                {
-                    const double v = !allowed || allowed[at + q] ? (double)toFloat(x[at + q]) : NEG_INF;
-                    logitS[k][at + q] = v;
-                    top = v > top ? v : top;
-                }
-                for (int q = 0; q < headSize(h); q++)
-                {
-                    const double v = logitS[k][at + q];
-                    sum += exp(v - (top > NEG_INF ? top : 0.0));
-                }
-                norm += (top > NEG_INF ? top : 0.0) + log(sum);
-                at += headSize(h);
-            }
-            base = (double)p.scores[row0 + k] - norm;
+            if (i & s) continue;
+            const JointKey a = l[i], b = l[i | s];
+            const bool swap = ahead(b, a);
+            l[i] = swap ? b : a;
+            l[i | s] = swap ? a : b;
         }
-        baseS[k] = base;
-    }
-    __syncthreads();
-    BestList<GroupKey, 1> best;
-    best.init(waitS[warp], p.width, lane);
-    for (int c0 = warp * 32; c0 < K * JOINT_ACTIONS; c0 += MERGE_THREADS)
+}
+
+// As for the flat selection, for normalisers over seven heads: per head d averages at
+// most log(3), with two additions (1.1 * 2.25 + 6) u = 8.5 u; six products; and logf's
+// last place of at most 6.5, 8 u.  Together 74 u = 4.5e-6 a beam.
+constexpr double NEAR_JOINT = 1e-5;
+
+constexpr int JOINT_THREADS = 128;
+
+// A thread per beam, the beams of a group side by side in a warp (padded to a power
+// of two).  The best N joint actions of a beam are found head by head: the list of
+// the best sums so far plus each choice of the next head, merged.  A choice that is
+// the r-th best of its head (from 0) can only continue the first N / (r + 1) sums.
+// Sums of logits are in 64 bits, so they are exact for logits within 29 binades;
+// normalisers are in 32 bits first, and in 64 where two beams' totals are near.
+template <class T, int N>
+__global__ void __launch_bounds__(JOINT_THREADS) jointSelectKernel(BeamParams p, int lanes)
+{
+    const int lane = threadIdx.x & 31, K = p.beams;
+    const long long warp = (blockIdx.x * (long long)JOINT_THREADS + threadIdx.x) >> 5;
+    const long long g = warp * (32 / lanes) + lane / lanes;
+    const int k = lane % lanes;
+    const bool on = g < p.groups && k < K;
+    const long long row = g * K + k;
+    const float score = on ? p.scores[row] : NEG_INF;
+    const bool over = on && p.finished && p.finished[row];
+    const bool reads = on && !over && score > NEG_INF;
+    __shared__ float xS[ACTION_LOGITS][JOINT_THREADS];
+    const auto x = [&](int q) -> float& { return xS[q][threadIdx.x]; };  // a column of the thread's own
+    const T* from = rowLogits<T>(p, reads ? g : 0, reads ? k : 0);
+    const uint8_t* allowed = rowMask(p, reads ? g : 0, reads ? k : 0);
+#pragma unroll
+    for (int q = 0; q < ACTION_LOGITS; q++) x(q) = reads && (!allowed || allowed[q]) ? toFloat(from[q]) : NEG_INF;
+
+    JointKey best[N];
+    for (int pass = 0; pass < 2; pass++)
     {
-        const int c = c0 + lane, beam = c / JOINT_ACTIONS;
-        double total = NEG_INF;
-        if (c < K * JOINT_ACTIONS && baseS[beam] > NEG_INF)
+        // The normaliser (NaN or +inf among the logits makes it NaN, an empty head -inf),
+        // and the beam's best joint actions.
+        double tops = 0.0, base = NEG_INF;
+        float product = 1.f;
+        double product64 = 1.0;
+#pragma unroll
+        for (int i = 0; i < N; i++) best[i] = JointKey{ NEG_INF, 0 };
+        best[0].v = 0.0;
+        int at = 0;
+#pragma unroll 1
+        for (int h = 0; h < HEADS; h++)
         {
-            int rest = c - beam * JOINT_ACTIONS, at = ACTION_LOGITS;
-            double sum = 0.0;
-            for (int h = HEADS - 1; h >= 0; h--)
+            const int size = headSize(h);
+            const float v[3] = { x(at), x(at + 1), size == 3 ? x(at + 2) : NEG_INF };
+            at += size;
+            const float top = fmaxf(fmaxf(v[0], v[1]), v[2]);
+            tops += (double)top;
+            if (pass == 0)
             {
-                at -= headSize(h);
-                sum += logitS[beam][at + rest % headSize(h)];
-                rest /= headSize(h);
+                float sum = 0.f;
+#pragma unroll
+                for (int q = 0; q < 3; q++) sum += exp2Approx((v[q] - top) * LOG2E);
+                product *= sum;
             }
-            total = baseS[beam] + sum;
+            else
+            {
+                double sum = 0.0;
+#pragma unroll 1
+                for (int q = 0; q < 3; q++) sum += exp((double)(q == 0 ? v[0] : q == 1 ? v[1] : v[2]) - (double)top);
+                product64 *= sum;
+            }
+            // The head's choices, best first.
+            JointKey option[3];
+#pragma unroll
+            for (int q = 0; q < 3; q++) option[q] = JointKey{ (double)v[q], q };
+            auto order = [&](int a, int b) {
+                const JointKey l = option[a], r = option[b];
+                const bool swap = ahead(r, l);
+                option[a] = swap ? r : l;
+                option[b] = swap ? l : r;
+            };
+            order(0, 1);
+            order(1, 2);
+            order(0, 1);
+            JointKey before[N];
+#pragma unroll
+            for (int i = 0; i < N; i++)
+            {
+                before[i] = best[i];
+                best[i] = JointKey{ before[i].v + option[0].v, before[i].i * size + option[0].i };
+            }
+#pragma unroll
+            for (int r = 1; r < 3; r++)
+            {
+                if (r >= size) continue;
+#pragma unroll
+                for (int i = 0; i < N / (r + 1); i++)
+                {
+                    const JointKey c{ before[i].v + option[r].v, before[i].i * size + option[r].i };
+                    if (ahead(c, best[N - 1 - i])) best[N - 1 - i] = c;
+                }
+                settle(best);
+            }
         }
-        const GroupKey key{ ordered64(total), ~(unsigned)c };
-        best.push(total > NEG_INF && better(key, best.bar), key);
+        if (tops > NEG_INF)
+            base = (double)score - (tops + (pass == 0 ? (double)logf(product) : log(product64)));
+        const bool live = reads && base > NEG_INF;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+        {
+            best[i].v = live ? base + best[i].v : (double)NEG_INF;
+            best[i].i += k * JOINT_ACTIONS;
+        }
+        if (over) best[0] = JointKey{ score > NEG_INF ? (double)score : (double)NEG_INF, k * JOINT_ACTIONS };
+
+        // The group's: every lane of it ends with the same list.  `out` is the best that
+        // another beam lost its place with.
+        JointKey out{ NEG_INF, 0 };
+        for (int m = 1; m < lanes; m *= 2)
+        {
+            JointKey other[N];
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                other[i] = JointKey{ __shfl_xor_sync(FULL, best[N - 1 - i].v, m), __shfl_xor_sync(FULL, best[N - 1 - i].i, m) };
+            JointKey lost{ NEG_INF, 0 };
+#pragma unroll
+            for (int i = 0; i < N; i++)
+            {
+                const bool take = ahead(other[i], best[i]);
+                const JointKey drop = take ? best[i] : other[i];
+                if (take) best[i] = other[i];
+                if (drop.v > lost.v) lost = drop;
+            }
+            settle(best);
+            const JointKey theirs{ __shfl_xor_sync(FULL, out.v, m), __shfl_xor_sync(FULL, out.i, m) };
+            if (theirs.v > out.v) out = theirs;
+            if (lost.v > out.v) out = lost;
+        }
+        if (pass == 1) break;
+        bool near = false;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+        {
+            if (i >= p.width) continue;
+            const bool edge = i + 1 >= N;
+            const JointKey next = edge ? out : best[i + 1 < N ? i + 1 : i];
+            near |= best[i].v - next.v <= NEAR_JOINT && next.v > NEG_INF && best[i].i / JOINT_ACTIONS != next.i / JOINT_ACTIONS;
+        }
+        if (!__any_sync(FULL, near)) break;
     }
-    if (p.finished && warp == 0)
+
+    if (g >= p.groups) return;
+#pragma unroll
+    for (int i = 0; i < N; i++)
     {
-        const double total = lane < K && p.finished[row0 + lane] ? (double)p.scores[row0 + lane] : NEG_INF;
-        const GroupKey key{ ordered64(total), ~(unsigned)(lane * JOINT_ACTIONS) };
-        best.push(total > NEG_INF && better(key, best.bar), key);
-    }
-    best.finish();
-    mergeWarps(best, waitS, warp, lane);
-    for (int i = tid; i < p.width; i += MERGE_THREADS)
-    {
-        const GroupKey key = waitS[0][i];
-        const unsigned index = ~key.i;
+        if (i >= p.width || (i & (lanes - 1)) != k) continue;
+        const bool some = best[i].v > NEG_INF;
         const long long o = g * p.width + i;
-        p.outScores[o] = key.t ? (float)fromOrdered64(key.t) : NEG_INF;
-        p.outParents[o] = key.t ? index / JOINT_ACTIONS : i % K;
-        int rest = key.t ? index % JOINT_ACTIONS : 0;
+        const int beam = best[i].i / JOINT_ACTIONS;
+        p.outScores[o] = (float)best[i].v;
+        p.outParents[o] = some ? beam : i % K;
+        int rest = some ? best[i].i - beam * JOINT_ACTIONS : 0;
+#pragma unroll
         for (int h = HEADS - 1; h >= 0; h--)
         {
             p.outActions[o * HEADS + h] = rest % headSize(h);
@@ -741,36 +987,78 @@ __global__ void __launch_bounds__(REORDER_THREADS) moveContactsKernel(int* conta
     if (contact[car] >= 0) contact[car] += (j - (int)parent) * nCars;
 }
 
-template <class T, int E>
+template <class T, int E, bool MASKED>
 void launchSelect(const BeamParams& p, cudaStream_t s)
 {
+    if (p.segs == 0)
+    {
+        selectGroupKernel<T, E, MASKED><<<p.groups, ROW_THREADS, 0, s>>>(p);
+        return;
+    }
     const long long items = (long long)p.groups * p.beams * p.segs;
-    const unsigned blocks = (unsigned)((items + ROW_WARPS - 1) / ROW_WARPS);
+    selectRowsKernel<T, E, MASKED><<<(unsigned)((items + ROW_WARPS - 1) / ROW_WARPS), ROW_THREADS, 0, s>>>(p);
+    selectMergeKernel<T, E><<<p.groups, ROW_THREADS, 0, s>>>(p);
+}
+
+template <class T, int E>
+void launchSelectMasked(const BeamParams& p, cudaStream_t s)
+{
     if (p.mask)
-        selectRowsKernel<T, E, true><<<blocks, ROW_WARPS * 32, 0, s>>>(p);
+        launchSelect<T, E, true>(p, s);
     else
-        selectRowsKernel<T, E, false><<<blocks, ROW_WARPS * 32, 0, s>>>(p);
-    selectMergeKernel<T, E><<<p.groups, MERGE_THREADS, 0, s>>>(p);
+        launchSelect<T, E, false>(p, s);
 }
 
 template <class T>
 void launchSelectWidth(const BeamParams& p, cudaStream_t s)
 {
     if (p.width <= 32)
-        launchSelect<T, 1>(p, s);
+        launchSelectMasked<T, 1>(p, s);
     else if (p.width <= 64)
-        launchSelect<T, 2>(p, s);
+        launchSelectMasked<T, 2>(p, s);
     else
-        launchSelect<T, 4>(p, s);
+        launchSelectMasked<T, 4>(p, s);
+}
+
+template <class T, int N>
+void launchJoint(const BeamParams& p, cudaStream_t s)
+{
+    int lanes = 1;
+    while (lanes < p.beams) lanes *= 2;
+    const long long threads = ((long long)p.groups * lanes + 31) / 32 * 32;
+    jointSelectKernel<T, N><<<(unsigned)((threads + JOINT_THREADS - 1) / JOINT_THREADS), JOINT_THREADS, 0, s>>>(p, lanes);
+}
+
+template <class T>
+void launchJointWidth(const BeamParams& p, cudaStream_t s)
+{
+    if (p.width <= 4)
+        launchJoint<T, 4>(p, s);
+    else if (p.width <= 8)
+        launchJoint<T, 8>(p, s);
+    else if (p.width <= 16)
+        launchJoint<T, 16>(p, s);
+    else
+        launchJoint<T, 32>(p, s);
 }
 
 }  // namespace
 
 long long planBeamSelect(BeamParams& p, LogitType type, void* base)
 {
+    const long long rows = (long long)p.groups * p.beams;
+    const int tiles = (p.vocab + 1023) / 1024;
+    // Warps the card holds at a time, at the pass's register use.
+    constexpr long long WARPS = 148 * 24;
     (void)type;
-    p.segs = 1;
-    const long long items = (long long)p.groups * p.beams * p.segs;
+    const bool fits = p.beams <= GROUP_MAX_BEAMS && p.beams * p.width <= GROUP_MAX_KEYS;
+    if (fits && (tiles * ((p.beams + ROW_WARPS - 1) / ROW_WARPS) <= 2 || p.groups * ROW_WARPS >= 2 * WARPS))
+    {
+        p.segs = 0;
+        return 0;
+    }
+    p.segs = (int)std::max<long long>(1, std::min<long long>(tiles, WARPS / std::max<long long>(1, rows)));
+    const long long items = rows * p.segs;
     char* c = static_cast<char*>(base);
     p.sum = reinterpret_cast<double*>(c);
     p.keys = reinterpret_cast<unsigned long long*>(c + items * 8);
@@ -791,11 +1079,11 @@ void launchBeamSelect(const BeamParams& p, LogitType type, cudaStream_t s)
 void launchJointSelect(const BeamParams& p, LogitType type, cudaStream_t s)
 {
     if (type == LOGITS_F32)
-        jointSelectKernel<float><<<p.groups, MERGE_THREADS, 0, s>>>(p);
+        launchJointWidth<float>(p, s);
     else if (type == LOGITS_BF16)
-        jointSelectKernel<__nv_bfloat16><<<p.groups, MERGE_THREADS, 0, s>>>(p);
+        launchJointWidth<__nv_bfloat16>(p, s);
     else
-        jointSelectKernel<__half><<<p.groups, MERGE_THREADS, 0, s>>>(p);
+        launchJointWidth<__half>(p, s);
 }
 
 void launchReorder(const StateArray* arrays, int count, const long long* parents, int groups, int beams, cudaStream_t s)
