@@ -11,6 +11,7 @@
 #include "search.cuh"
 
 #include <algorithm>
+#include <cfloat>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -208,35 +209,6 @@ __device__ __forceinline__ float toFloat(float x) { return x; }
 __device__ __forceinline__ float toFloat(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float toFloat(__half x) { return __half2float(x); }
 
-__device__ __forceinline__ void unpack(const uint4& r, float (&v)[4], float)
-{
-    v[0] = __uint_as_float(r.x);
-    v[1] = __uint_as_float(r.y);
-    v[2] = __uint_as_float(r.z);
-    v[3] = __uint_as_float(r.w);
-}
-__device__ __forceinline__ void unpack(const uint4& r, float (&v)[8], __nv_bfloat16)
-{
-    const unsigned w[4] = { r.x, r.y, r.z, r.w };
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-    {
-        v[2 * k] = __uint_as_float(w[k] << 16);
-        v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ void unpack(const uint4& r, float (&v)[8], __half)
-{
-    const unsigned w[4] = { r.x, r.y, r.z, r.w };
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-    {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-        v[2 * k] = f.x;
-        v[2 * k + 1] = f.y;
-    }
-}
-
 __device__ __forceinline__ float exp2Approx(float x)
 {
     float y;
@@ -250,8 +222,165 @@ __device__ __forceinline__ bool readsLogits(const BeamParams& p, long long row)
 {
     return p.scores[row] > NEG_INF && !(p.finished && p.finished[row]);
 }
+template <class T>
+__device__ __forceinline__ const T* rowLogits(const BeamParams& p, long long g, int k)
+{
+    return static_cast<const T*>(p.logits) + g * p.groupStride + k * p.beamStride;
+}
+__device__ __forceinline__ const uint8_t* rowMask(const BeamParams& p, long long g, int k)
+{
+    return p.mask ? p.mask + g * p.maskGroupStride + k * p.maskBeamStride : nullptr;
+}
 
-// ---- the pass over the logits --------------------------------------------------------
+// 32-bit words of logits: one float32, or two of the 16-bit types.
+template <class T>
+struct Words;
+template <>
+struct Words<float>
+{
+    static constexpr int PER = 1;
+    static constexpr unsigned NONE = 0xff800000u;
+    static __device__ __forceinline__ float at(unsigned w, int) { return __uint_as_float(w); }
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b)
+    {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }
+};
+template <>
+struct Words<__nv_bfloat16>
+{
+    static constexpr int PER = 2;
+    static constexpr unsigned NONE = 0xff80ff80u;
+    static __device__ __forceinline__ float at(unsigned w, int q) { return __uint_as_float(q ? w & 0xffff0000u : w << 16); }
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b)
+    {
+        const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+        return *reinterpret_cast<const unsigned*>(&m);
+    }
+};
+template <>
+struct Words<__half>
+{
+    static constexpr int PER = 2;
+    static constexpr unsigned NONE = 0xfc00fc00u;
+    static __device__ __forceinline__ float at(unsigned w, int q)
+    {
+        const __half2 h = *reinterpret_cast<__half2*>(&w);
+        return q ? __high2float(h) : __low2float(h);
+    }
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b)
+    {
+        const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+        return *reinterpret_cast<const unsigned*>(&m);
+    }
+};
+
+// A row of logits as a warp reads it: whole 16-byte vectors in tiles of 32 elements a
+// lane, and one more element a lane for those before the first and behind the last
+// vector (at most 7 each).
+template <class T>
+struct Row
+{
+    static constexpr int VE = 16 / sizeof(T);   // elements of a vector
+    static constexpr int NV = 32 / VE;          // vectors of a lane per tile
+    static constexpr int WORDS = 32 / Words<T>::PER;
+    const T* x;
+    const uint8_t* allowed;
+    int head, vectors, tail, tiles, lane;
+    bool wideMask;
+
+    __device__ Row(const T* logits, const uint8_t* mask, int vocab, int l)
+        : x(logits), allowed(mask), lane(l)
+    {
+        head = min(vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
+        vectors = (vocab - head) / VE;
+        tail = vocab - head - vectors * VE;
+        tiles = (vectors + 32 * NV - 1) / (32 * NV);
+        wideMask = (reinterpret_cast<uintptr_t>(mask + head) & 3) == 0;
+    }
+    // Element j (0 .. 31) of this lane's part of tile t, as an action.
+    __device__ int action(int t, int j) const { return head + ((t * NV + j / VE) * 32 + lane) * VE + j % VE; }
+
+    template <bool MASKED>
+    __device__ __forceinline__ void load(int t, unsigned (&w)[WORDS], unsigned (&m)[8]) const
+    {
+        const uint4* v = reinterpret_cast<const uint4*>(x + head);
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+        {
+            const int i = (t * NV + j) * 32 + lane;
+            uint4 r = make_uint4(Words<T>::NONE, Words<T>::NONE, Words<T>::NONE, Words<T>::NONE);
+            if (i < vectors) r = __ldcs(v + i);
+            w[4 * j] = r.x;
+            w[4 * j + 1] = r.y;
+            w[4 * j + 2] = r.z;
+            w[4 * j + 3] = r.w;
+            if (MASKED)
+            {
+                const uint8_t* a = allowed + head + (long long)i * VE;
+#pragma unroll
+                for (int q = 0; q < VE / 4; q++)
+                {
+                    unsigned b = 0;
+                    if (i < vectors)
+                    {
+                        if (wideMask)
+                            b = __ldcs(reinterpret_cast<const unsigned*>(a + 4 * q));
+                        else
+                            b = a[4 * q] | a[4 * q + 1] << 8 | a[4 * q + 2] << 16 | (unsigned)a[4 * q + 3] << 24;
+                    }
+                    m[j * VE / 4 + q] = b;
+                }
+            }
+        }
+    }
+    // What is not allowed becomes -inf.
+    __device__ __forceinline__ static void hide(unsigned (&w)[WORDS], const unsigned (&m)[8])
+    {
+#pragma unroll
+        for (int q = 0; q < 8; q++)
+        {
+            if (Words<T>::PER == 1)
+            {
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (!(m[q] >> (8 * k) & 0xff)) w[(4 * q + k) % WORDS] = Words<T>::NONE;
+            }
+            else
+            {
+                const unsigned z = __vcmpeq4(m[q], 0);
+                const unsigned lo = __byte_perm(z, 0, 0x1100), hi = __byte_perm(z, 0, 0x3322);
+                w[(2 * q) % WORDS] = (w[(2 * q) % WORDS] & ~lo) | (Words<T>::NONE & lo);
+                w[(2 * q + 1) % WORDS] = (w[(2 * q + 1) % WORDS] & ~hi) | (Words<T>::NONE & hi);
+            }
+        }
+    }
+    __device__ static float element(const unsigned (&w)[WORDS], int j)
+    {
+        return Words<T>::at(w[j / Words<T>::PER], j % Words<T>::PER);
+    }
+    // Largest of elements 8 k .. 8 k + 7, NaN passed over (-inf if there is nothing else).
+    __device__ static float largest8(const unsigned (&w)[WORDS], int k)
+    {
+        constexpr int N = 8 / Words<T>::PER;
+        unsigned m = w[N * k];
+#pragma unroll
+        for (int i = 1; i < N; i++) m = Words<T>::larger(m, w[N * k + i]);
+        float f = Words<T>::at(m, 0);
+        if (Words<T>::PER == 2) f = fmaxf(f, Words<T>::at(m, 1));
+        return fmaxf(f, NEG_INF);
+    }
+    // The lane's element outside the vectors; returns its action, or -1 for none.
+    __device__ int edge(float& v) const
+    {
+        v = NEG_INF;
+        int a = -1;
+        if (lane < head) a = lane;
+        else if (lane >= 8 && lane < 8 + tail) a = head + vectors * VE + lane - 8;
+        if (a >= 0 && (!allowed || allowed[a])) v = toFloat(x[a]);
+        return a;
+    }
+};
 
 // The `n`-th largest (n <= 32 E) of E values a lane, as an ordered image.
 template <int E>
@@ -279,36 +408,15 @@ __device__ __forceinline__ unsigned nthLargest(unsigned (&v)[E], int n, int lane
     return __shfl_sync(FULL, r, (n - 1) & 31);
 }
 
-// One warp over a segment of a row: the segment's largest logits (sorted, in `best`),
-// their maximum and, per lane, a part of the sum of exp(x - maximum).
-//
-// Tiles of 1024 elements are held in registers, 32 a lane.  A tile whose maximum
-// does not reach the list's last place costs its loads, the exponentials and one
-// vote.  The first tile has no such bar yet: the width-th largest of the lanes'
-// maxima is one, since at least `width` elements reach it.
-template <class T, int E, bool MASKED>
-__device__ __forceinline__ void scanRow(const BeamParams& p, const T* x, const uint8_t* allowed, int seg, int segs,
-                                        RowKey* wait, int lane, BestList<RowKey, E>& best, float& top, double& sum)
+// Running maximum of a row (over the warp) and, per lane, a part of the sum of
+// exp(x - maximum).
+struct RowSum
 {
-    constexpr int VE = 16 / sizeof(T);  // elements of a 16-byte load
-    constexpr int NV = 32 / VE;         // loads of a lane per tile
-    const int head = min(p.vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-    const int vectors = (p.vocab - head) / VE, tail = p.vocab - head - vectors * VE;
-    const int tiles = (vectors + 32 * NV - 1) / (32 * NV);
-    const int t0 = (int)((long long)tiles * seg / segs), t1 = (int)((long long)tiles * (seg + 1) / segs);
-    const bool wideMask = MASKED && (reinterpret_cast<uintptr_t>(allowed + head) % VE) == 0;
+    float top = NEG_INF;
+    double sum = 0.0;
 
-    best.init(wait, p.width, lane);
-    top = NEG_INF;
-    sum = 0.0;
-    float bar = NEG_INF;  // nothing below it can be kept
-    bool started = false;
-
-    auto raise = [&]() {
-        if (best.bar) bar = fmaxf(bar, fromOrdered((unsigned)(best.bar >> 32)));
-    };
-    auto absorb = [&](float laneTop) {
-        if (laneTop != laneTop) laneTop = NEG_INF;  // NaN reaches the sum, not the maximum
+    __device__ __forceinline__ float raise(float laneTop)
+    {
         const float t = fromOrdered(__reduce_max_sync(FULL, ordered(laneTop)));
         if (t > top)
         {
@@ -316,75 +424,61 @@ __device__ __forceinline__ void scanRow(const BeamParams& p, const T* x, const u
             top = t;
         }
         return t;
-    };
+    }
+    __device__ __forceinline__ void add(float v) { sum += exp2Approx((v - (top > NEG_INF ? top : 0.f)) * LOG2E); }
+    template <class T>
+    __device__ __forceinline__ void add8(const unsigned (&w)[Row<T>::WORDS], int k)
+    {
+        const float ref = top > NEG_INF ? top : 0.f;
+        float s = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; q++) s += exp2Approx((Row<T>::element(w, 8 * k + q) - ref) * LOG2E);
+        sum += s;
+    }
+    // Over the warp.
+    __device__ __forceinline__ void gather()
+    {
+#pragma unroll
+        for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
+    }
+};
 
-    const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+// ---- long rows: the best of each segment ----------------------------------------------
+
+// One warp over a segment of a row: the segment's largest logits, sorted, and its sum.
+//
+// A tile whose maximum does not reach the list's last place costs its loads, the
+// exponentials and one vote.  The first tile has no such bar yet: the width-th largest
+// of the lanes' maxima is one, since at least `width` elements reach it.
+template <class T, int E, bool MASKED>
+__device__ __forceinline__ void scanRow(const Row<T>& row, int width, int seg, int segs, RowKey* wait,
+                                        BestList<RowKey, E>& best, RowSum& sum)
+{
+    const int t0 = (int)((long long)row.tiles * seg / segs), t1 = (int)((long long)row.tiles * (seg + 1) / segs);
+    best.init(wait, width, row.lane);
+    float bar = -FLT_MAX;  // nothing below it can be kept
+    bool started = false;
+    unsigned next[Row<T>::WORDS], nextMask[8];
+    if (t0 < t1) row.template load<MASKED>(t0, next, nextMask);
     for (int t = t0; t < t1; t++)
     {
-        float v[32];
-        uint4 raw[NV];
+        unsigned w[Row<T>::WORDS], m[8];
 #pragma unroll
-        for (int j = 0; j < NV; j++)
+        for (int i = 0; i < Row<T>::WORDS; i++) w[i] = next[i];
+        if (MASKED)
         {
-            const int i = (t * NV + j) * 32 + lane;
-            if (i < vectors) raw[j] = __ldcs(xv + i);
+#pragma unroll
+            for (int i = 0; i < 8; i++) m[i] = nextMask[i];
         }
+        if (t + 1 < t1) row.template load<MASKED>(t + 1, next, nextMask);
+        if (MASKED) Row<T>::hide(w, m);
         float part[4];
 #pragma unroll
-        for (int j = 0; j < NV; j++)
-        {
-            const int i = (t * NV + j) * 32 + lane;
-            if ((t * NV + j) * 32 >= vectors)  // the same for the whole warp
-            {
+        for (int k = 0; k < 4; k++) part[k] = Row<T>::largest8(w, k);
+        const float tileTop = sum.raise(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
 #pragma unroll
-                for (int q = 0; q < VE; q++) v[j * VE + q] = NEG_INF;
-                continue;
-            }
-            float f[VE];
-            unpack(raw[j], f, T());
-            bool ok[VE];
-#pragma unroll
-            for (int q = 0; q < VE; q++) ok[q] = i < vectors;
-            if (MASKED && i < vectors)
-            {
-                const uint8_t* m = allowed + head + i * VE;
-                if (wideMask)
-                {
-                    unsigned w[2];
-                    w[0] = __ldcs(reinterpret_cast<const unsigned*>(m));
-                    if (VE == 8) w[1] = __ldcs(reinterpret_cast<const unsigned*>(m) + 1);
-#pragma unroll
-                    for (int q = 0; q < VE; q++) ok[q] = (w[q / 4] >> (8 * (q & 3)) & 0xffu) != 0;
-                }
-                else
-                {
-#pragma unroll
-                    for (int q = 0; q < VE; q++) ok[q] = m[q] != 0;
-                }
-            }
-#pragma unroll
-            for (int q = 0; q < VE; q++) v[j * VE + q] = ok[q] ? f[q] : NEG_INF;
-        }
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-        {
-            part[k] = v[8 * k];
-#pragma unroll
-            for (int q = 1; q < 8; q++) part[k] = fmaxf(part[k], v[8 * k + q]);
-        }
-        const float laneTop = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-        const float tileTop = absorb(laneTop);
-        const float ref = top > NEG_INF ? top : 0.f;
-#pragma unroll
-        for (int j = 0; j < 32; j += 8)
-        {
-            if ((t * NV + j / VE) * 32 >= vectors) break;
-            float s = 0.f;
-#pragma unroll
-            for (int q = 0; q < 8; q++) s += exp2Approx((v[j + q] - ref) * LOG2E);
-            sum += s;
-        }
-        if (!(tileTop >= bar && tileTop > NEG_INF)) continue;
+        for (int k = 0; k < 4; k++) sum.template add8<T>(w, k);
+        if (!(tileTop >= bar)) continue;
         if (!started)
         {
             started = true;
@@ -392,55 +486,45 @@ __device__ __forceinline__ void scanRow(const BeamParams& p, const T* x, const u
 #pragma unroll
             for (int e = 0; e < E; e++)
             {
-                float m = part[e * (4 / E)];
+                float top = part[e * (4 / E)];
 #pragma unroll
-                for (int k = 1; k < 4 / E; k++) m = fmaxf(m, part[e * (4 / E) + k]);
-                tops[e] = m > NEG_INF ? ordered(m) : 0;
+                for (int k = 1; k < 4 / E; k++) top = fmaxf(top, part[e * (4 / E) + k]);
+                tops[e] = top > NEG_INF ? ordered(top) : 0;
             }
-            const unsigned o = nthLargest<E>(tops, p.width, lane);
+            const unsigned o = nthLargest<E>(tops, width, row.lane);
             if (o) bar = fromOrdered(o);
         }
         unsigned bits = 0;
 #pragma unroll
-        for (int j = 0; j < 32; j++)
-            if (v[j] >= bar && v[j] > NEG_INF) bits |= 1u << j;
+        for (int k = 0; k < 4; k++)
+        {
+            if (!__any_sync(FULL, part[k] >= bar)) continue;
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+                if (Row<T>::element(w, 8 * k + q) >= bar) bits |= 1u << (8 * k + q);
+        }
         while (__any_sync(FULL, bits != 0))
         {
             const bool has = bits != 0;
-            const int j = has ? __ffs(bits) - 1 : 0;
+            const int action = row.action(t, has ? __ffs(bits) - 1 : 0);
             bits &= bits - 1;
-            const int action = head + ((t * NV + j / VE) * 32 + lane) * VE + j % VE;
             RowKey key = 0;
-            if (has) key = (RowKey)ordered(toFloat(x[action])) << 32 | (unsigned)~action;
+            if (has) key = (RowKey)ordered(toFloat(row.x[action])) << 32 | (unsigned)~action;
             best.push(has && key > best.bar, key);
         }
-        raise();
+        if (best.bar) bar = fmaxf(bar, fromOrdered((unsigned)(best.bar >> 32)));
     }
-    // The elements before the first and behind the last whole vector.
-    if (seg == 0 && head + tail > 0)
+    if (seg == 0 && row.head + row.tail > 0)
     {
-        const bool front = lane < head, back = lane >= 8 && lane < 8 + tail;
-        const int a = front ? lane : head + vectors * VE + lane - 8;
-        float v = NEG_INF;
-        if ((front || back) && (!MASKED || allowed[a])) v = toFloat(x[a]);
-        absorb(v);
-        sum += exp2Approx((v - (top > NEG_INF ? top : 0.f)) * LOG2E);
+        float v;
+        const int a = row.edge(v);
+        sum.raise(fmaxf(v, NEG_INF));
+        sum.add(v);
         const RowKey key = (RowKey)ordered(v) << 32 | (unsigned)~a;
-        best.push(v >= bar && v > NEG_INF && key > best.bar, key);
+        best.push(v >= bar && key > best.bar, key);
     }
     best.finish();
-#pragma unroll
-    for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
-}
-
-template <class T>
-__device__ __forceinline__ const T* rowLogits(const BeamParams& p, long long g, int k)
-{
-    return static_cast<const T*>(p.logits) + g * p.groupStride + k * p.beamStride;
-}
-__device__ __forceinline__ const uint8_t* rowMask(const BeamParams& p, long long g, int k)
-{
-    return p.mask ? p.mask + g * p.maskGroupStride + k * p.maskBeamStride : nullptr;
+    sum.gather();
 }
 
 constexpr int ROW_WARPS = 8;
@@ -458,32 +542,31 @@ __global__ void __launch_bounds__(ROW_THREADS) selectRowsKernel(BeamParams p)
     if (!readsLogits(p, row)) return;
     const int k = (int)(row - g * p.beams);
     BestList<RowKey, E> best;
-    float top;
-    double sum;
-    scanRow<T, E, MASKED>(p, rowLogits<T>(p, g, k), rowMask(p, g, k), (int)(item - row * p.segs), p.segs, waitS[warp], lane,
-                          best, top, sum);
+    RowSum sum;
+    scanRow<T, E, MASKED>(Row<T>(rowLogits<T>(p, g, k), rowMask(p, g, k), p.vocab, lane), p.width,
+                          (int)(item - row * p.segs), p.segs, waitS[warp], best, sum);
     if (lane == 0)
     {
-        p.top[item] = top;
-        p.sum[item] = sum;
+        p.top[item] = sum.top;
+        p.sum[item] = sum.sum;
     }
 #pragma unroll
     for (int e = 0; e < E; e++)
         if (e * 32 + lane < p.width) p.keys[item * p.width + e * 32 + lane] = best.list[e];
 }
 
-// ---- the merge of a group --------------------------------------------------------------
+// ---- the best of a group -----------------------------------------------------------------
 
-// Totals of different beams are compared through normalisers that the pass above
-// has to fp32 accuracy in its terms.  With u = 2^-24 and d = top - x: a term is off by
-// d u (the difference), 1.25 d u (its product with log2(e), and that constant) and 4 u
-// (ex2.approx); d averages at most log(vocab) <= 20.8 under the softmax; partial sums of
-// eight terms add 7 u.  Together 58 u = 3.5e-6, so two totals that are further apart
+// Totals of different beams are compared through normalisers that the passes over the
+// logits have to fp32 accuracy in their terms.  With u = 2^-24 and d = top - x: a term is
+// off by d u (the difference), 1.25 d u (its product with log2(e), and that constant) and
+// 4 u (ex2.approx); d averages at most log(vocab) <= 20.8 under the softmax; partial sums
+// of eight terms add 7 u.  Together 58 u = 3.5e-6, so two totals that are further apart
 // than twice that are in order.  Nearer ones are decided by normalisers in 64 bits.
 constexpr double NEAR_TOTALS = 8e-6;
 
 template <int E>
-struct MergeShared
+struct GroupShared
 {
     GroupKey wait[ROW_WARPS][32 * E + 32];
     double red[ROW_WARPS];
@@ -491,50 +574,23 @@ struct MergeShared
     unsigned repair;
 };
 
-// A block merges the lists of its group's rows (`keys` [beams, segs, width], `tops`
-// and `sums` [beams, segs]) and writes the group's outputs.  base: [beams] doubles of
-// shared memory.
-template <class T, int E>
-__device__ void mergeGroup(const BeamParams& p, long long g, const RowKey* keys, const float* tops, const double* sums,
-                           int segs, double* base, MergeShared<E>& sh)
+// A block orders its group's candidates and writes the group's outputs.  candidate(c,
+// beam, index) gives candidate c < n: its logit, beam and beam * vocab + action (-inf for
+// none); topOf(k) is the largest allowed logit of beam k; base[k] is the score minus the
+// normaliser, -inf where beam k has no candidate; finished beams come on top.
+template <class T, int E, class Candidate, class TopOf>
+__device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, int n, Candidate candidate, TopOf topOf,
+                                            double* base, GroupShared<E>& sh)
 {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long row0 = g * p.beams;
-    const int K = p.beams, per = segs * p.width, n = K * per;
-
-    for (int k = tid; k < K; k += ROW_THREADS)
-    {
-        double b = NEG_INF;
-        if (readsLogits(p, row0 + k))
-        {
-            float t = NEG_INF;
-            for (int s = 0; s < segs; s++) t = fmaxf(t, tops[k * segs + s]);
-            if (t > NEG_INF)
-            {
-                double sum = 0.0;
-                for (int s = 0; s < segs; s++)
-                {
-                    // A segment without a finite logit has sum 0, or NaN where one was NaN.
-                    const float ts = tops[k * segs + s];
-                    sum += ts > NEG_INF && ts < t ? sums[k * segs + s] * exp((double)ts - (double)t) : sums[k * segs + s];
-                }
-                b = (double)p.scores[row0 + k] - ((double)t + log(sum));
-            }
-        }
-        base[k] = b;
-    }
+    const int K = p.beams;
     for (int k = tid; k < BEAM_MAX_BEAMS / 32; k += ROW_THREADS) sh.near[k] = 0;
     if (tid == 0) sh.repair = 0;
-    __syncthreads();
 
     auto totalOf = [&](int c, int& beam, unsigned& index) {
-        beam = c / per;
-        const double b = base[beam];
-        if (!(b > NEG_INF)) return (double)NEG_INF;
-        const RowKey key = keys[c];
-        if (!key) return (double)NEG_INF;
-        index = (unsigned)beam * p.vocab + ~(unsigned)key;
-        return b + (double)fromOrdered((unsigned)(key >> 32));
+        const float x = candidate(c, beam, index);
+        return x > NEG_INF ? base[beam] + (double)x : (double)NEG_INF;
     };
     // Few candidates are one warp's work; more are shared out and merged pairwise.
     const int warps = n <= 256 * E ? 1 : ROW_WARPS;
@@ -545,10 +601,9 @@ __device__ void mergeGroup(const BeamParams& p, long long g, const RowKey* keys,
             best.init(sh.wait[warp], p.width, lane);
             for (int c0 = warp * 32; c0 < n; c0 += warps * 32)
             {
-                const int c = c0 + lane;
                 int beam = 0;
                 unsigned index = 0;
-                const double total = c < n ? totalOf(c, beam, index) : NEG_INF;
+                const double total = c0 + lane < n ? totalOf(c0 + lane, beam, index) : NEG_INF;
                 const GroupKey key{ ordered64(total), ~index };
                 best.push(total > NEG_INF && better(key, best.bar), key);
             }
@@ -602,8 +657,8 @@ __device__ void mergeGroup(const BeamParams& p, long long g, const RowKey* keys,
         const int kl = ~last.i / p.vocab;
         for (int c = tid; c < n; c += ROW_THREADS)
         {
-            int beam;
-            unsigned index;
+            int beam = 0;
+            unsigned index = 0;
             const double total = totalOf(c, beam, index);
             if (beam == kl || !(fabs(total - edge) <= NEAR_TOTALS)) continue;
             mark(beam);
@@ -625,11 +680,10 @@ __device__ void mergeGroup(const BeamParams& p, long long g, const RowKey* keys,
             if (!(sh.near[k >> 5] >> (k & 31) & 1) || !readsLogits(p, row0 + k)) continue;  // the same for the whole block
             const T* x = rowLogits<T>(p, g, k);
             const uint8_t* allowed = rowMask(p, g, k);
-            float t = NEG_INF;
-            for (int s = 0; s < segs; s++) t = fmaxf(t, tops[k * segs + s]);
+            const double t = (double)topOf(k);
             double sum = 0.0;
             for (int a = tid; a < p.vocab; a += ROW_THREADS)
-                if (!allowed || allowed[a]) sum += exp((double)toFloat(x[a]) - (double)t);
+                if (!allowed || allowed[a]) sum += exp((double)toFloat(x[a]) - t);
 #pragma unroll
             for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
             if (lane == 0) sh.red[warp] = sum;
@@ -638,7 +692,7 @@ __device__ void mergeGroup(const BeamParams& p, long long g, const RowKey* keys,
             {
                 sum = 0.0;
                 for (int w = 0; w < ROW_WARPS; w++) sum += sh.red[w];
-                base[k] = (double)p.scores[row0 + k] - ((double)t + log(sum));
+                base[k] = (double)p.scores[row0 + k] - (t + log(sum));
             }
             __syncthreads();
         }
@@ -656,47 +710,217 @@ __device__ void mergeGroup(const BeamParams& p, long long g, const RowKey* keys,
     }
 }
 
+// From the segments' lists.
 template <class T, int E>
 __global__ void __launch_bounds__(ROW_THREADS) selectMergeKernel(BeamParams p)
 {
     __shared__ double baseS[BEAM_MAX_BEAMS];
-    __shared__ MergeShared<E> sh;
-    const long long g = blockIdx.x, item0 = g * p.beams * p.segs;
-    mergeGroup<T, E>(p, g, p.keys + item0 * p.width, p.top + item0, p.sum + item0, p.segs, baseS, sh);
+    __shared__ GroupShared<E> sh;
+    const long long g = blockIdx.x, row0 = g * p.beams;
+    const int segs = p.segs, per = segs * p.width;
+    const RowKey* keys = p.keys + row0 * per;
+    const float* tops = p.top + row0 * segs;
+    const double* sums = p.sum + row0 * segs;
+    auto topOf = [&](int k) {
+        float t = NEG_INF;
+        for (int s = 0; s < segs; s++) t = fmaxf(t, tops[k * segs + s]);
+        return t;
+    };
+    for (int k = threadIdx.x; k < p.beams; k += ROW_THREADS)
+    {
+        double b = NEG_INF;
+        const float t = readsLogits(p, row0 + k) ? topOf(k) : NEG_INF;
+        if (t > NEG_INF)
+        {
+            double sum = 0.0;
+            for (int s = 0; s < segs; s++)
+            {
+                // A segment without a finite logit has sum 0, or NaN where one was NaN.
+                const float ts = tops[k * segs + s];
+                sum += ts > NEG_INF && ts < t ? sums[k * segs + s] * exp((double)ts - (double)t) : sums[k * segs + s];
+            }
+            b = (double)p.scores[row0 + k] - ((double)t + log(sum));
+        }
+        baseS[k] = b;
+    }
+    __syncthreads();
+    auto candidate = [&](int c, int& beam, unsigned& index) {
+        beam = c / per;
+        if (!(baseS[beam] > NEG_INF)) return NEG_INF;
+        const RowKey key = keys[c];
+        if (!key) return NEG_INF;
+        index = (unsigned)beam * p.vocab + ~(unsigned)key;
+        return fromOrdered((unsigned)(key >> 32));
+    };
+    finishGroup<T, E>(p, g, p.beams * per, candidate, topOf, baseS, sh);
 }
 
-// Both in one block per group, where the group's rows are short or the groups many.
+// ---- short rows: a block per group ------------------------------------------------------
+
+// A group's rows are read by the warps of one block.  The lanes' largest totals give a
+// bar for the whole group, the width-th largest of them; the few elements that reach it
+// (with a margin for rounding) are the group's candidates.  Where more reach it than
+// there is room for (rows of equal logits), the rows' own best take their place.
 constexpr int GROUP_MAX_BEAMS = 64;
 constexpr int GROUP_MAX_KEYS = 1024;
 
-template <class T, int E, bool MASKED>
-__global__ void __launch_bounds__(ROW_THREADS) selectGroupKernel(BeamParams p)
+template <class T, bool MASKED>
+__global__ void __launch_bounds__(ROW_THREADS, 3) selectGroupKernel(BeamParams p)
 {
-    __shared__ RowKey keyS[GROUP_MAX_KEYS];
+    __shared__ RowKey keyS[GROUP_MAX_KEYS];        // ordered logit, beam * vocab + action
     __shared__ float topS[GROUP_MAX_BEAMS];
-    __shared__ double sumS[GROUP_MAX_BEAMS], baseS[GROUP_MAX_BEAMS];
-    __shared__ union { RowKey wait[ROW_WARPS][32 * E + 32]; MergeShared<E> merge; } sh;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ double baseS[GROUP_MAX_BEAMS];
+    __shared__ unsigned laneS[ROW_THREADS];
+    __shared__ float barS;
+    __shared__ int countS;
+    __shared__ union { RowKey wait[ROW_WARPS][64]; GroupShared<1> group; } sh;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = p.beams;
     const long long g = blockIdx.x;
-    for (int k = warp; k < p.beams; k += ROW_WARPS)
+    if (threadIdx.x == 0) countS = 0;
+
+    unsigned w[Row<T>::WORDS], m[8];
+    int held = -1, heldTile = 0;                   // the tile in registers
+    float laneBest = NEG_INF;                      // largest total of the lane
+    for (int k = warp; k < K; k += ROW_WARPS)
     {
-        if (!readsLogits(p, g * p.beams + k)) continue;
-        BestList<RowKey, E> best;
-        float top;
-        double sum;
-        scanRow<T, E, MASKED>(p, rowLogits<T>(p, g, k), rowMask(p, g, k), 0, 1, sh.wait[warp], lane, best, top, sum);
+        double b = NEG_INF;
+        RowSum sum;
+        if (readsLogits(p, g * K + k))
+        {
+            const Row<T> row(rowLogits<T>(p, g, k), rowMask(p, g, k), p.vocab, lane);
+            float laneTop = NEG_INF;
+            for (int t = 0; t < row.tiles; t++)
+            {
+                row.template load<MASKED>(t, w, m);
+                if (MASKED) Row<T>::hide(w, m);
+                held = k;
+                heldTile = t;
+                const float tileTop = fmaxf(fmaxf(Row<T>::largest8(w, 0), Row<T>::largest8(w, 1)),
+                                            fmaxf(Row<T>::largest8(w, 2), Row<T>::largest8(w, 3)));
+                laneTop = fmaxf(laneTop, tileTop);
+                sum.raise(tileTop);
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    if ((t * Row<T>::NV + q * Row<T>::NV / 4) * 32 < row.vectors) sum.template add8<T>(w, q);
+            }
+            if (row.head + row.tail > 0)
+            {
+                float v;
+                row.edge(v);
+                laneTop = fmaxf(laneTop, v);
+                sum.raise(fmaxf(v, NEG_INF));
+                sum.add(v);
+            }
+            sum.gather();
+            if (sum.top > NEG_INF) b = (double)p.scores[g * K + k] - ((double)sum.top + log(sum.sum));
+            if (b > NEG_INF && laneTop > NEG_INF) laneBest = fmaxf(laneBest, (float)(b + (double)laneTop));
+        }
         if (lane == 0)
         {
-            topS[k] = top;
-            sumS[k] = sum;
+            topS[k] = sum.top;
+            baseS[k] = b;
         }
+    }
+    laneS[threadIdx.x] = laneBest > NEG_INF ? ordered(laneBest) : 0;
+    __syncthreads();
+    if (warp == 0)
+    {
+        unsigned v[ROW_WARPS], top = 0;
 #pragma unroll
-        for (int e = 0; e < E; e++)
-            if (e * 32 + lane < p.width) keyS[k * p.width + e * 32 + lane] = best.list[e];
-        __syncwarp();
+        for (int i = 0; i < ROW_WARPS; i++) v[i] = laneS[i * 32 + lane];
+        for (int left = p.width; left > 0;)
+        {
+            unsigned mine = v[0];
+#pragma unroll
+            for (int i = 1; i < ROW_WARPS; i++) mine = max(mine, v[i]);
+            top = __reduce_max_sync(FULL, mine);
+            if (top == 0) break;
+            int hits = 0;
+#pragma unroll
+            for (int i = 0; i < ROW_WARPS; i++)
+            {
+                hits += v[i] == top;
+                if (v[i] == top) v[i] = 0;
+            }
+            left -= __reduce_add_sync(FULL, hits);
+        }
+        if (lane == 0)
+        {
+            // Lower by twice NEAR_TOTALS and by eight roundings to float32.
+            const float t = fromOrdered(top);
+            barS = top && fabsf(t) < FLT_MAX ? t - (2.f * (float)NEAR_TOTALS + 8.f * 0x1p-24f * fabsf(t)) : NEG_INF;
+        }
     }
     __syncthreads();
-    mergeGroup<T, E>(p, g, keyS, topS, sumS, 1, baseS, sh.merge);
+    const float bar = barS;
+    auto offer = [&](float v, int k, int action) {
+        const int at = atomicAdd(&countS, 1);
+        if (at < GROUP_MAX_KEYS) keyS[at] = (RowKey)ordered(v) << 32 | ((unsigned)k * p.vocab + action);
+    };
+    for (int k = (K - 1 - warp) / ROW_WARPS * ROW_WARPS + warp; k >= 0 && warp < K; k -= ROW_WARPS)
+    {
+        const double b = baseS[k];
+        if (!(b > NEG_INF)) continue;
+        // Logits of this row that can reach the bar.
+        const float need = b < (double)INFINITY && bar > NEG_INF ? fmaxf((float)((double)bar - b), -FLT_MAX) : -FLT_MAX;
+        const float margin = need > -FLT_MAX ? need - 2.f * 0x1p-24f * fabsf(need) : need;
+        if (!(topS[k] >= margin)) continue;
+        const Row<T> row(rowLogits<T>(p, g, k), rowMask(p, g, k), p.vocab, lane);
+        for (int t = row.tiles - 1; t >= 0; t--)
+        {
+            if (held != k || heldTile != t)
+            {
+                row.template load<MASKED>(t, w, m);
+                if (MASKED) Row<T>::hide(w, m);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+            {
+                if (!(Row<T>::largest8(w, q) >= margin)) continue;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                {
+                    const float v = Row<T>::element(w, 8 * q + i);
+                    if (v >= margin) offer(v, k, row.action(t, 8 * q + i));
+                }
+            }
+        }
+        if (row.head + row.tail > 0)
+        {
+            float v;
+            const int a = row.edge(v);
+            if (v >= margin) offer(v, k, a);
+        }
+    }
+    __syncthreads();
+    int n = countS;
+    if (n > GROUP_MAX_KEYS)
+    {
+        for (int k = warp; k < K; k += ROW_WARPS)
+        {
+            BestList<RowKey, 1> best;
+            best.init(sh.wait[warp], p.width, lane);
+            RowSum sum;
+            if (baseS[k] > NEG_INF)
+                scanRow<T, 1, MASKED>(Row<T>(rowLogits<T>(p, g, k), rowMask(p, g, k), p.vocab, lane), p.width, 0, 1,
+                                      sh.wait[warp], best, sum);
+            const RowKey key = best.list[0];
+            if (lane < p.width)
+                keyS[k * p.width + lane] = key ? (key & ~0xffffffffull) | ((unsigned)k * p.vocab + ~(unsigned)key) : 0;
+            __syncwarp();
+        }
+        n = K * p.width;
+        __syncthreads();
+    }
+    auto candidate = [&](int c, int& beam, unsigned& index) {
+        const RowKey key = keyS[c];
+        if (!key) return NEG_INF;
+        index = (unsigned)key;
+        beam = index / p.vocab;
+        return fromOrdered((unsigned)(key >> 32));
+    };
+    auto topOf = [&](int k) { return topS[k]; };
+    finishGroup<T, 1>(p, g, n, candidate, topOf, baseS, sh.group);
 }
 
 // ---- selection over the action heads ---------------------------------------------------
@@ -990,34 +1214,31 @@ __global__ void __launch_bounds__(REORDER_THREADS) moveContactsKernel(int* conta
 template <class T, int E, bool MASKED>
 void launchSelect(const BeamParams& p, cudaStream_t s)
 {
-    if (p.segs == 0)
-    {
-        selectGroupKernel<T, E, MASKED><<<p.groups, ROW_THREADS, 0, s>>>(p);
-        return;
-    }
     const long long items = (long long)p.groups * p.beams * p.segs;
     selectRowsKernel<T, E, MASKED><<<(unsigned)((items + ROW_WARPS - 1) / ROW_WARPS), ROW_THREADS, 0, s>>>(p);
     selectMergeKernel<T, E><<<p.groups, ROW_THREADS, 0, s>>>(p);
 }
 
-template <class T, int E>
-void launchSelectMasked(const BeamParams& p, cudaStream_t s)
+template <class T, bool MASKED>
+void launchSelectWidth(const BeamParams& p, cudaStream_t s)
 {
-    if (p.mask)
-        launchSelect<T, E, true>(p, s);
+    if (p.segs == 0)
+        selectGroupKernel<T, MASKED><<<p.groups, ROW_THREADS, 0, s>>>(p);
+    else if (p.width <= 32)
+        launchSelect<T, 1, MASKED>(p, s);
+    else if (p.width <= 64)
+        launchSelect<T, 2, MASKED>(p, s);
     else
-        launchSelect<T, E, false>(p, s);
+        launchSelect<T, 4, MASKED>(p, s);
 }
 
 template <class T>
-void launchSelectWidth(const BeamParams& p, cudaStream_t s)
+void launchSelectMasked(const BeamParams& p, cudaStream_t s)
 {
-    if (p.width <= 32)
-        launchSelectMasked<T, 1>(p, s);
-    else if (p.width <= 64)
-        launchSelectMasked<T, 2>(p, s);
+    if (p.mask)
+        launchSelectWidth<T, true>(p, s);
     else
-        launchSelectMasked<T, 4>(p, s);
+        launchSelectWidth<T, false>(p, s);
 }
 
 template <class T, int N>
@@ -1049,10 +1270,14 @@ long long planBeamSelect(BeamParams& p, LogitType type, void* base)
     const long long rows = (long long)p.groups * p.beams;
     const int tiles = (p.vocab + 1023) / 1024;
     // Warps the card holds at a time, at the pass's register use.
-    constexpr long long WARPS = 148 * 24;
+    constexpr long long WARPS = 148 * 16;
     (void)type;
-    const bool fits = p.beams <= GROUP_MAX_BEAMS && p.beams * p.width <= GROUP_MAX_KEYS;
-    if (fits && (tiles * ((p.beams + ROW_WARPS - 1) / ROW_WARPS) <= 2 || p.groups * ROW_WARPS >= 2 * WARPS))
+    // A block per group re-reads rows of more than one tile, and its warps take the rows
+    // of more than eight beams in turn.
+    const bool fits = p.width <= 32 && p.width <= 16 * p.beams && p.beams <= GROUP_MAX_BEAMS
+                      && p.beams * p.width <= GROUP_MAX_KEYS;
+    const int turns = tiles * ((p.beams + ROW_WARPS - 1) / ROW_WARPS);
+    if (fits && (turns <= 2 || (tiles <= 4 && p.groups >= 2 * 148)))
     {
         p.segs = 0;
         return 0;
@@ -1069,11 +1294,11 @@ long long planBeamSelect(BeamParams& p, LogitType type, void* base)
 void launchBeamSelect(const BeamParams& p, LogitType type, cudaStream_t s)
 {
     if (type == LOGITS_F32)
-        launchSelectWidth<float>(p, s);
+        launchSelectMasked<float>(p, s);
     else if (type == LOGITS_BF16)
-        launchSelectWidth<__nv_bfloat16>(p, s);
+        launchSelectMasked<__nv_bfloat16>(p, s);
     else
-        launchSelectWidth<__half>(p, s);
+        launchSelectMasked<__half>(p, s);
 }
 
 void launchJointSelect(const BeamParams& p, LogitType type, cudaStream_t s)
