@@ -4,10 +4,9 @@
 // Beam selection.  With s_k the score of beam k and x_kv its logits, the total of
 // a continuation is s_k + x_kv - log(sum of exp(x_ku) over the allowed u), and a
 // step keeps the `width` largest of a group, ties to the lowest k * vocab + v.
-// Within a beam the order is that of the logits, so the pass over the logits needs
-// no normaliser: a warp keeps the largest of its part of a row in a sorted list
-// across its lanes while it accumulates the sum.  The lists of a group's rows are
-// then merged on 64-bit totals.
+// The logits are read once, for the sums and for the maxima of short runs of them
+// (chunks); the totals of those maxima say which few chunks can hold one of the
+// best, and these are read again and ordered on 64-bit totals.
 #include "search.cuh"
 
 #include <algorithm>
@@ -52,30 +51,22 @@ __device__ __forceinline__ double fromOrdered64(u64 o)
 
 // ---- sorted lists across a warp --------------------------------------------------------
 
-// A candidate of a row: ordered logit, complement of the action (greater is better,
-// a lower action wins a tie); 0 is none.
-using RowKey = u64;
-
-// A candidate of a group: ordered 64-bit total, complement of beam * vocab + action.
+// A candidate of a group: ordered 64-bit total, complement of beam * vocab + action
+// (greater is better, a lower index wins a tie); t = 0 is none.
 struct GroupKey
 {
     u64 t;
     unsigned i;
 };
 
-__device__ __forceinline__ bool better(unsigned a, unsigned b) { return a > b; }
-__device__ __forceinline__ bool better(RowKey a, RowKey b) { return a > b; }
 __device__ __forceinline__ bool better(const GroupKey& a, const GroupKey& b)
 {
     return a.t > b.t || (a.t == b.t && a.i > b.i);
 }
-__device__ __forceinline__ unsigned shflXor(unsigned k, int m) { return __shfl_xor_sync(FULL, k, m); }
-__device__ __forceinline__ RowKey shflXor(RowKey k, int m) { return __shfl_xor_sync(FULL, k, m); }
 __device__ __forceinline__ GroupKey shflXor(const GroupKey& k, int m)
 {
     return GroupKey{ __shfl_xor_sync(FULL, k.t, m), __shfl_xor_sync(FULL, k.i, m) };
 }
-__device__ __forceinline__ RowKey shflAt(RowKey k, int l) { return __shfl_sync(FULL, k, l); }
 __device__ __forceinline__ GroupKey shflAt(const GroupKey& k, int l)
 {
     return GroupKey{ __shfl_sync(FULL, k.t, l), __shfl_sync(FULL, k.i, l) };
@@ -275,46 +266,72 @@ struct Words<__half>
     }
 };
 
-// A row of logits as a warp reads it: whole 16-byte vectors in tiles of 32 elements a
-// lane, and one more element a lane for those before the first and behind the last
-// vector (at most 7 each).
+// Sum of exp(v - ref) over eight values, two at a time (the packed fp32 instructions).
+__device__ __forceinline__ u64 pack2(float a, float b)
+{
+    u64 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float sumExp8(const float (&v)[8], float ref)
+{
+    const u64 minus = pack2(-ref, -ref), scale = pack2(LOG2E, LOG2E);
+    u64 total = 0;
+#pragma unroll
+    for (int q = 0; q < 8; q += 2)
+    {
+        u64 d;
+        float a, b;
+        asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pack2(v[q], v[q + 1])), "l"(minus));
+        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(d), "l"(scale));
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
+        asm("add.rn.f32x2 %0, %1, %2;" : "=l"(total) : "l"(total), "l"(pack2(exp2Approx(a), exp2Approx(b))));
+    }
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(total));
+    return a + b;
+}
+
+// A row of logits as a warp reads it: 16-byte vectors, lane l those with index l mod 32,
+// and one more element a lane for those before the first and behind the last vector (at
+// most 7 each).  A segment is a range of vectors (a multiple of 32 but for the last); a
+// lane's elements of a segment, the edges counted to the first, are a chunk.
 template <class T>
 struct Row
 {
     static constexpr int VE = 16 / sizeof(T);   // elements of a vector
-    static constexpr int NV = 32 / VE;          // vectors of a lane per tile
-    static constexpr int WORDS = 32 / Words<T>::PER;
+    static constexpr int NV = 4;                // vectors of a lane per tile
+    static constexpr int MASKS = NV * VE / 4;   // 32-bit words of mask bytes
     const T* x;
     const uint8_t* allowed;
-    int head, vectors, tail, tiles, lane;
+    int head, vectors, tail, lane;
     bool wideMask;
 
-    __device__ Row(const T* logits, const uint8_t* mask, int vocab, int l)
-        : x(logits), allowed(mask), lane(l)
+    __device__ Row(const BeamParams& p, long long g, int k, int l)
+        : x(rowLogits<T>(p, g, k)), allowed(rowMask(p, g, k)), lane(l)
     {
-        head = min(vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-        vectors = (vocab - head) / VE;
-        tail = vocab - head - vectors * VE;
-        tiles = (vectors + 32 * NV - 1) / (32 * NV);
-        wideMask = (reinterpret_cast<uintptr_t>(mask + head) & 3) == 0;
+        head = min(p.vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
+        vectors = (p.vocab - head) / VE;
+        tail = p.vocab - head - vectors * VE;
+        wideMask = (reinterpret_cast<uintptr_t>(allowed + head) & 3) == 0;
     }
-    // Element j (0 .. 31) of this lane's part of tile t, as an action.
-    __device__ int action(int t, int j) const { return head + ((t * NV + j / VE) * 32 + lane) * VE + j % VE; }
+    __device__ static int segmentStart(int vectors, int seg, int segs)
+    {
+        const int blocks = (vectors + 31) / 32;
+        return (int)((long long)blocks * seg / segs) * 32;
+    }
 
+    // Vectors v0 + lane + 32 j, those below `end`; the others are -inf.
     template <bool MASKED>
-    __device__ __forceinline__ void load(int t, unsigned (&w)[WORDS], unsigned (&m)[8]) const
+    __device__ __forceinline__ void load(int v0, int end, uint4 (&w)[NV], unsigned (&m)[MASKS]) const
     {
         const uint4* v = reinterpret_cast<const uint4*>(x + head);
 #pragma unroll
         for (int j = 0; j < NV; j++)
         {
-            const int i = (t * NV + j) * 32 + lane;
-            uint4 r = make_uint4(Words<T>::NONE, Words<T>::NONE, Words<T>::NONE, Words<T>::NONE);
-            if (i < vectors) r = __ldcs(v + i);
-            w[4 * j] = r.x;
-            w[4 * j + 1] = r.y;
-            w[4 * j + 2] = r.z;
-            w[4 * j + 3] = r.w;
+            const int i = v0 + 32 * j + lane;
+            w[j] = make_uint4(Words<T>::NONE, Words<T>::NONE, Words<T>::NONE, Words<T>::NONE);
+            if (i < end) w[j] = __ldcs(v + i);
             if (MASKED)
             {
                 const uint8_t* a = allowed + head + (long long)i * VE;
@@ -322,7 +339,7 @@ struct Row
                 for (int q = 0; q < VE / 4; q++)
                 {
                     unsigned b = 0;
-                    if (i < vectors)
+                    if (i < end)
                     {
                         if (wideMask)
                             b = __ldcs(reinterpret_cast<const unsigned*>(a + 4 * q));
@@ -335,40 +352,26 @@ struct Row
         }
     }
     // What is not allowed becomes -inf.
-    __device__ __forceinline__ static void hide(unsigned (&w)[WORDS], const unsigned (&m)[8])
+    __device__ __forceinline__ static void hide(uint4& w, const unsigned* m)
     {
+        unsigned* r = reinterpret_cast<unsigned*>(&w);
 #pragma unroll
-        for (int q = 0; q < 8; q++)
+        for (int q = 0; q < VE / 4; q++)
         {
-            if (Words<T>::PER == 1)
+            if (VE == 4)
             {
 #pragma unroll
                 for (int k = 0; k < 4; k++)
-                    if (!(m[q] >> (8 * k) & 0xff)) w[(4 * q + k) % WORDS] = Words<T>::NONE;
+                    if (!(m[q] & 0xffu << (8 * k))) r[k] = Words<T>::NONE;
             }
             else
             {
                 const unsigned z = __vcmpeq4(m[q], 0);
                 const unsigned lo = __byte_perm(z, 0, 0x1100), hi = __byte_perm(z, 0, 0x3322);
-                w[(2 * q) % WORDS] = (w[(2 * q) % WORDS] & ~lo) | (Words<T>::NONE & lo);
-                w[(2 * q + 1) % WORDS] = (w[(2 * q + 1) % WORDS] & ~hi) | (Words<T>::NONE & hi);
+                r[2 * q] = (r[2 * q] & ~lo) | (Words<T>::NONE & lo);
+                r[2 * q + 1] = (r[2 * q + 1] & ~hi) | (Words<T>::NONE & hi);
             }
         }
-    }
-    __device__ static float element(const unsigned (&w)[WORDS], int j)
-    {
-        return Words<T>::at(w[j / Words<T>::PER], j % Words<T>::PER);
-    }
-    // Largest of elements 8 k .. 8 k + 7, NaN passed over (-inf if there is nothing else).
-    __device__ static float largest8(const unsigned (&w)[WORDS], int k)
-    {
-        constexpr int N = 8 / Words<T>::PER;
-        unsigned m = w[N * k];
-#pragma unroll
-        for (int i = 1; i < N; i++) m = Words<T>::larger(m, w[N * k + i]);
-        float f = Words<T>::at(m, 0);
-        if (Words<T>::PER == 2) f = fmaxf(f, Words<T>::at(m, 1));
-        return fmaxf(f, NEG_INF);
     }
     // The lane's element outside the vectors; returns its action, or -1 for none.
     __device__ int edge(float& v) const
@@ -382,244 +385,303 @@ struct Row
     }
 };
 
-// The `n`-th largest (n <= 32 E) of E values a lane, as an ordered image.
-template <int E>
-__device__ __forceinline__ unsigned nthLargest(unsigned (&v)[E], int n, int lane)
+// Largest of the elements of a word's worth of logits, NaN passed over.
+template <class T>
+__device__ __forceinline__ float largestOf(unsigned w)
 {
-    if (E == 1 && n <= 12)
-    {
-        // Fewer rounds of taking the maximum out than a sort has exchanges.
-        unsigned mine = v[0], top = 0;
-        for (int left = n; left > 0;)
-        {
-            top = __reduce_max_sync(FULL, mine);
-            const bool hit = mine == top;
-            left -= __popc(__ballot_sync(FULL, hit));
-            if (hit) mine = 0;
-            if (top == 0) break;
-        }
-        return top;
-    }
-    sortDown(v, lane);
-    unsigned r = v[0];
-#pragma unroll
-    for (int e = 1; e < E; e++)
-        if ((n - 1) / 32 == e) r = v[e];
-    return __shfl_sync(FULL, r, (n - 1) & 31);
+    const float f = Words<T>::at(w, 0);
+    return Words<T>::PER == 2 ? fmaxf(f, Words<T>::at(w, 1)) : f;
 }
 
-// Running maximum of a row (over the warp) and, per lane, a part of the sum of
-// exp(x - maximum).
-struct RowSum
+// What one pass over a segment keeps: its maximum (over the warp), the sum of
+// exp(x - maximum), and every lane's largest logit.
+struct Scan
 {
-    float top = NEG_INF;
+    float top = NEG_INF, laneTop = NEG_INF;
     double sum = 0.0;
 
-    __device__ __forceinline__ float raise(float laneTop)
+    __device__ __forceinline__ void raise(float v)
     {
+        laneTop = fmaxf(laneTop, v);  // NaN is passed over: it reaches the sum alone
         const float t = fromOrdered(__reduce_max_sync(FULL, ordered(laneTop)));
         if (t > top)
         {
-            sum *= exp((double)top - (double)t);
+            if (top > NEG_INF) sum *= exp((double)top - (double)t);  // otherwise it is 0, or NaN
             top = t;
         }
-        return t;
     }
-    __device__ __forceinline__ void add(float v) { sum += exp2Approx((v - (top > NEG_INF ? top : 0.f)) * LOG2E); }
-    template <class T>
-    __device__ __forceinline__ void add8(const unsigned (&w)[Row<T>::WORDS], int k)
-    {
-        const float ref = top > NEG_INF ? top : 0.f;
-        float s = 0.f;
-#pragma unroll
-        for (int q = 0; q < 8; q++) s += exp2Approx((Row<T>::element(w, 8 * k + q) - ref) * LOG2E);
-        sum += s;
-    }
-    // Over the warp.
-    __device__ __forceinline__ void gather()
-    {
-#pragma unroll
-        for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
-    }
+    __device__ __forceinline__ float ref() const { return top > NEG_INF ? top : 0.f; }
 };
 
-// ---- long rows: the best of each segment ----------------------------------------------
-
-// One warp over a segment of a row: the segment's largest logits, sorted, and its sum.
-//
-// A tile whose maximum does not reach the list's last place costs its loads, the
-// exponentials and one vote.  The first tile has no such bar yet: the width-th largest
-// of the lanes' maxima is one, since at least `width` elements reach it.
-template <class T, int E, bool MASKED>
-__device__ __forceinline__ void scanRow(const Row<T>& row, int width, int seg, int segs, RowKey* wait,
-                                        BestList<RowKey, E>& best, RowSum& sum)
+// One warp over segment `seg` of a row.  Nothing is selected here: the lanes' maxima
+// tell later which chunks can hold one of the best, and only those are read again.
+template <class T, bool MASKED>
+__device__ __forceinline__ Scan scanRow(const Row<T>& row, int seg, int segs)
 {
-    const int t0 = (int)((long long)row.tiles * seg / segs), t1 = (int)((long long)row.tiles * (seg + 1) / segs);
-    best.init(wait, width, row.lane);
-    float bar = -FLT_MAX;  // nothing below it can be kept
-    bool started = false;
-    unsigned next[Row<T>::WORDS], nextMask[8];
-    if (t0 < t1) row.template load<MASKED>(t0, next, nextMask);
-    for (int t = t0; t < t1; t++)
+    constexpr int NV = Row<T>::NV, VE = Row<T>::VE;
+    Scan scan;
+    const int begin = Row<T>::segmentStart(row.vectors, seg, segs);
+    const int end = min(row.vectors, Row<T>::segmentStart(row.vectors, seg + 1, segs));
+    uint4 next[NV];
+    unsigned nextMask[Row<T>::MASKS];
+    if (begin < end) row.template load<MASKED>(begin, end, next, nextMask);
+    for (int v0 = begin; v0 < end; v0 += 32 * NV)
     {
-        unsigned w[Row<T>::WORDS], m[8];
+        uint4 w[NV];
+        unsigned m[Row<T>::MASKS];
 #pragma unroll
-        for (int i = 0; i < Row<T>::WORDS; i++) w[i] = next[i];
-        if (MASKED)
+        for (int j = 0; j < NV; j++) w[j] = next[j];
+#pragma unroll
+        for (int j = 0; j < Row<T>::MASKS; j++) m[j] = nextMask[j];
+        if (v0 + 32 * NV < end) row.template load<MASKED>(v0 + 32 * NV, end, next, nextMask);
+        unsigned most = Words<T>::NONE;
+#pragma unroll
+        for (int j = 0; j < NV; j++)
         {
-#pragma unroll
-            for (int i = 0; i < 8; i++) m[i] = nextMask[i];
+            if (MASKED) Row<T>::hide(w[j], m + j * VE / 4);
+            most = Words<T>::larger(most, Words<T>::larger(Words<T>::larger(w[j].x, w[j].y), Words<T>::larger(w[j].z, w[j].w)));
         }
-        if (t + 1 < t1) row.template load<MASKED>(t + 1, next, nextMask);
-        if (MASKED) Row<T>::hide(w, m);
-        float part[4];
+        scan.raise(largestOf<T>(most));
+        const float ref = scan.ref();
 #pragma unroll
-        for (int k = 0; k < 4; k++) part[k] = Row<T>::largest8(w, k);
-        const float tileTop = sum.raise(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
-#pragma unroll
-        for (int k = 0; k < 4; k++) sum.template add8<T>(w, k);
-        if (!(tileTop >= bar)) continue;
-        if (!started)
+        for (int j = 0; j < NV; j += 8 / VE)
         {
-            started = true;
-            unsigned tops[E];
+            if (v0 + 32 * j >= end) break;  // the same for the whole warp
+            float v[8];
 #pragma unroll
-            for (int e = 0; e < E; e++)
+            for (int i = 0; i < 8; i++)
             {
-                float top = part[e * (4 / E)];
-#pragma unroll
-                for (int k = 1; k < 4 / E; k++) top = fmaxf(top, part[e * (4 / E) + k]);
-                tops[e] = top > NEG_INF ? ordered(top) : 0;
+                const uint4& r = w[j + i / VE];
+                const int e = i % VE / Words<T>::PER;
+                v[i] = Words<T>::at(e == 0 ? r.x : e == 1 ? r.y : e == 2 ? r.z : r.w, i % Words<T>::PER);
             }
-            const unsigned o = nthLargest<E>(tops, width, row.lane);
-            if (o) bar = fromOrdered(o);
+            scan.sum += sumExp8(v, ref);
         }
-        unsigned bits = 0;
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-        {
-            if (!__any_sync(FULL, part[k] >= bar)) continue;
-#pragma unroll
-            for (int q = 0; q < 8; q++)
-                if (Row<T>::element(w, 8 * k + q) >= bar) bits |= 1u << (8 * k + q);
-        }
-        while (__any_sync(FULL, bits != 0))
-        {
-            const bool has = bits != 0;
-            const int action = row.action(t, has ? __ffs(bits) - 1 : 0);
-            bits &= bits - 1;
-            RowKey key = 0;
-            if (has) key = (RowKey)ordered(toFloat(row.x[action])) << 32 | (unsigned)~action;
-            best.push(has && key > best.bar, key);
-        }
-        if (best.bar) bar = fmaxf(bar, fromOrdered((unsigned)(best.bar >> 32)));
     }
     if (seg == 0 && row.head + row.tail > 0)
     {
         float v;
-        const int a = row.edge(v);
-        sum.raise(fmaxf(v, NEG_INF));
-        sum.add(v);
-        const RowKey key = (RowKey)ordered(v) << 32 | (unsigned)~a;
-        best.push(v >= bar && key > best.bar, key);
+        row.edge(v);
+        scan.raise(v);
+        scan.sum += exp2Approx((v - scan.ref()) * LOG2E);
     }
-    best.finish();
-    sum.gather();
+#pragma unroll
+    for (int m = 16; m > 0; m /= 2) scan.sum += __shfl_xor_sync(FULL, scan.sum, m);
+    return scan;
 }
 
 constexpr int ROW_WARPS = 8;
 constexpr int ROW_THREADS = ROW_WARPS * 32;
 
 // One warp per segment of a row, results to the workspace.
-template <class T, int E, bool MASKED>
+template <class T, bool MASKED>
 __global__ void __launch_bounds__(ROW_THREADS) selectRowsKernel(BeamParams p)
 {
-    __shared__ RowKey waitS[ROW_WARPS][32 * E + 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long item = blockIdx.x * (long long)ROW_WARPS + warp;
+    const int lane = threadIdx.x & 31;
+    const long long item = blockIdx.x * (long long)ROW_WARPS + (threadIdx.x >> 5);
     if (item >= (long long)p.groups * p.beams * p.segs) return;
-    const long long row = item / p.segs, g = row / p.beams;
-    if (!readsLogits(p, row)) return;
-    const int k = (int)(row - g * p.beams);
-    BestList<RowKey, E> best;
-    RowSum sum;
-    scanRow<T, E, MASKED>(Row<T>(rowLogits<T>(p, g, k), rowMask(p, g, k), p.vocab, lane), p.width,
-                          (int)(item - row * p.segs), p.segs, waitS[warp], best, sum);
+    const long long r = item / p.segs, g = r / p.beams;
+    if (!readsLogits(p, r)) return;
+    const Scan scan = scanRow<T, MASKED>(Row<T>(p, g, (int)(r - g * p.beams), lane), (int)(item - r * p.segs), p.segs);
+    p.chunks[item * 32 + lane] = scan.laneTop;
     if (lane == 0)
     {
-        p.top[item] = sum.top;
-        p.sum[item] = sum.sum;
+        p.top[item] = scan.top;
+        p.sum[item] = scan.sum;
     }
-#pragma unroll
-    for (int e = 0; e < E; e++)
-        if (e * 32 + lane < p.width) p.keys[item * p.width + e * 32 + lane] = best.list[e];
 }
 
 // ---- the best of a group -----------------------------------------------------------------
 
-// Totals of different beams are compared through normalisers that the passes over the
-// logits have to fp32 accuracy in their terms.  With u = 2^-24 and d = top - x: a term is
-// off by d u (the difference), 1.25 d u (its product with log2(e), and that constant) and
-// 4 u (ex2.approx); d averages at most log(vocab) <= 20.8 under the softmax; partial sums
-// of eight terms add 7 u.  Together 58 u = 3.5e-6, so two totals that are further apart
-// than twice that are in order.  Nearer ones are decided by normalisers in 64 bits.
+// Totals of different beams are compared through normalisers that the pass over the
+// logits has to fp32 accuracy in its terms.  With u = 2^-24 and d = top - x: a term is off
+// by d u (the difference), 1.25 d u (its product with log2(e), and that constant) and 4 u
+// (ex2.approx); d averages at most log(vocab) <= 20.8 under the softmax; partial sums of
+// eight terms add 7 u.  Together 58 u = 3.5e-6, so two totals that are further apart than
+// twice that are in order.  Nearer ones are decided by normalisers in 64 bits.
 constexpr double NEAR_TOTALS = 8e-6;
+
+constexpr int MAX_CHUNKS = 512;       // chunks of a group that are read again
+constexpr int MAX_CANDIDATES = 1024;  // and their elements that reach the bar
 
 template <int E>
 struct GroupShared
 {
     GroupKey wait[ROW_WARPS][32 * E + 32];
+    u64 found[MAX_CANDIDATES];        // ordered logit, beam * vocab + action
+    int chunk[MAX_CHUNKS];
+    unsigned tops[ROW_THREADS];       // the threads' largest totals
     double red[ROW_WARPS];
     unsigned near[BEAM_MAX_BEAMS / 32];
-    unsigned repair;
+    unsigned bar;
+    int chunks, candidates, repair;
 };
 
-// A block orders its group's candidates and writes the group's outputs.  candidate(c,
-// beam, index) gives candidate c < n: its logit, beam and beam * vocab + action (-inf for
-// none); topOf(k) is the largest allowed logit of beam k; base[k] is the score minus the
-// normaliser, -inf where beam k has no candidate; finished beams come on top.
-template <class T, int E, class Candidate, class TopOf>
-__device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, int n, Candidate candidate, TopOf topOf,
+// The n-th largest (n <= 128) of the values that the block's threads hold (0: none), to
+// sh.bar.
+template <int E>
+__device__ __forceinline__ void nthLargest(unsigned mine, int n, GroupShared<E>& sh)
+{
+    const int tid = threadIdx.x, lane = tid & 31;
+    sh.tops[tid] = mine;
+    if (tid == 0) sh.bar = n <= 12 ? 0 : 0xffffffffu;
+    __syncthreads();
+    if (n <= 12)
+    {
+        // One warp takes the maximum out n times.
+        if (tid < 32)
+        {
+            unsigned v[ROW_WARPS], top = 0;
+#pragma unroll
+            for (int i = 0; i < ROW_WARPS; i++) v[i] = sh.tops[i * 32 + lane];
+            for (int left = n; left > 0;)
+            {
+                unsigned most = v[0];
+#pragma unroll
+                for (int i = 1; i < ROW_WARPS; i++) most = max(most, v[i]);
+                top = __reduce_max_sync(FULL, most);
+                if (top == 0) break;
+                int hits = 0;
+#pragma unroll
+                for (int i = 0; i < ROW_WARPS; i++)
+                {
+                    hits += v[i] == top;
+                    if (v[i] == top) v[i] = 0;
+                }
+                left -= __reduce_add_sync(FULL, hits);
+            }
+            if (lane == 0) sh.bar = top;
+        }
+    }
+    else
+    {
+        // The smallest of the values with fewer than n above them.
+        int above = 0;
+        for (int i = 0; i < ROW_THREADS; i++) above += sh.tops[i] > mine;
+        const unsigned least = __reduce_min_sync(FULL, above < n ? mine : 0xffffffffu);
+        if (lane == 0) atomicMin(&sh.bar, least);
+    }
+    __syncthreads();
+}
+
+// A block finds its group's best and writes them.  chunkTop(c) is the largest logit of
+// chunk c = (beam * segs + segment) * 32 + lane, topOf(k) that of beam k; base[k] is the
+// score minus the normaliser, -inf where beam k has no continuation.
+//
+// The width-th largest of the threads' largest totals is a bar that `width` elements
+// reach; the chunks that reach it (lowered by the margin of the comparison) are read
+// again, and their elements that do are the candidates.  Where there are too many of
+// either (rows of equal logits), every element is one.
+template <class T, int E, class ChunkTop, class TopOf>
+__device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, int segs, ChunkTop chunkTop, TopOf topOf,
                                             double* base, GroupShared<E>& sh)
 {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long row0 = g * p.beams;
-    const int K = p.beams;
-    for (int k = tid; k < BEAM_MAX_BEAMS / 32; k += ROW_THREADS) sh.near[k] = 0;
-    if (tid == 0) sh.repair = 0;
+    const int K = p.beams, all = K * segs * 32;
 
-    auto totalOf = [&](int c, int& beam, unsigned& index) {
-        const float x = candidate(c, beam, index);
-        return x > NEG_INF ? base[beam] + (double)x : (double)NEG_INF;
-    };
-    // Few candidates are one warp's work; more are shared out and merged pairwise.
-    const int warps = n <= 256 * E ? 1 : ROW_WARPS;
-    auto choose = [&]() {
-        BestList<GroupKey, E> best;
-        if (warp < warps)
+    if (tid == 0) sh.chunks = sh.candidates = sh.repair = 0;
+    if (tid < BEAM_MAX_BEAMS / 32) sh.near[tid] = 0;
+    float best = NEG_INF;
+    for (int c = tid; c < all; c += ROW_THREADS)
+    {
+        const double b = base[c / (32 * segs)];
+        if (b > NEG_INF) best = fmaxf(best, (float)(b + (double)chunkTop(c)));
+    }
+    nthLargest(best > NEG_INF ? ordered(best) : 0u, p.width, sh);
+    // Lower by twice NEAR_TOTALS and by eight roundings to float32.
+    float bar = sh.bar && sh.bar != 0xffffffffu ? fromOrdered(sh.bar) : NEG_INF;
+    bar = fabsf(bar) < FLT_MAX ? bar - (2.f * (float)NEAR_TOTALS + 8.f * 0x1p-24f * fabsf(bar)) : NEG_INF;
+    for (int c = tid; c < all; c += ROW_THREADS)
+    {
+        const double b = base[c / (32 * segs)];
+        const float top = b > NEG_INF ? chunkTop(c) : NEG_INF;
+        if (!(top > NEG_INF && b + (double)top >= (double)bar)) continue;
+        const int at = atomicAdd(&sh.chunks, 1);
+        if (at < MAX_CHUNKS) sh.chunk[at] = c;
+    }
+    __syncthreads();
+    const int chunks = sh.chunks;
+    for (int i = warp; i < chunks && chunks <= MAX_CHUNKS; i += ROW_WARPS)
+    {
+        const int c = sh.chunk[i], k = c / (32 * segs), seg = c / 32 - k * segs;
+        const double b = base[k];
+        Row<T> row(p, g, k, c & 31);
+        const int begin = Row<T>::segmentStart(row.vectors, seg, segs) + row.lane;
+        const int end = min(row.vectors, Row<T>::segmentStart(row.vectors, seg + 1, segs));
+        auto offer = [&](float v, int action) {
+            if (!(v > NEG_INF && b + (double)v >= (double)bar)) return;
+            const int at = atomicAdd(&sh.candidates, 1);
+            if (at < MAX_CANDIDATES) sh.found[at] = (u64)ordered(v) << 32 | ((unsigned)k * p.vocab + action);
+        };
+        for (int e = lane;; e += 32)
         {
-            best.init(sh.wait[warp], p.width, lane);
-            for (int c0 = warp * 32; c0 < n; c0 += warps * 32)
-            {
-                int beam = 0;
-                unsigned index = 0;
-                const double total = c0 + lane < n ? totalOf(c0 + lane, beam, index) : NEG_INF;
-                const GroupKey key{ ordered64(total), ~index };
-                best.push(total > NEG_INF && better(key, best.bar), key);
-            }
-            for (int k0 = warp * 32; p.finished && k0 < K; k0 += warps * 32)
-            {
-                const int k = k0 + lane;
-                const double total = k < K && p.finished[row0 + k] ? (double)p.scores[row0 + k] : NEG_INF;
-                const GroupKey key{ ordered64(total), ~((unsigned)k * p.vocab) };
-                best.push(total > NEG_INF && better(key, best.bar), key);
-            }
-            best.finish();
-            __syncwarp();  // the buffer of waiting keys becomes the list
-#pragma unroll
-            for (int e = 0; e < E; e++) sh.wait[warp][e * 32 + lane] = best.list[e];
+            const int v = begin + e / Row<T>::VE * 32;
+            if (v >= end) break;
+            const int action = row.head + v * Row<T>::VE + e % Row<T>::VE;
+            if (!row.allowed || row.allowed[action]) offer(toFloat(row.x[action]), action);
         }
-        __syncthreads();
+        if (seg == 0 && lane == 0)
+        {
+            float v;
+            const int action = row.edge(v);
+            if (action >= 0) offer(v, action);
+        }
+    }
+    __syncthreads();
+    const bool every = chunks > MAX_CHUNKS || sh.candidates > MAX_CANDIDATES;
+    const int n = every ? K * p.vocab : sh.candidates;
+
+    // Candidate c: its total, beam and index; -inf for none.
+    auto totalOf = [&](int c, int& beam, unsigned& index) {
+        if (every)
+        {
+            index = c;
+            beam = c / p.vocab;
+            if (!(base[beam] > NEG_INF)) return (double)NEG_INF;
+            const int action = c - beam * p.vocab;
+            const uint8_t* allowed = rowMask(p, g, beam);
+            const float x = !allowed || allowed[action] ? toFloat(rowLogits<T>(p, g, beam)[action]) : NEG_INF;
+            return x > NEG_INF ? base[beam] + (double)x : (double)NEG_INF;
+        }
+        const u64 key = sh.found[c];
+        index = (unsigned)key;
+        beam = index / p.vocab;
+        return base[beam] + (double)fromOrdered((unsigned)(key >> 32));
+    };
+    // Few candidates are one warp's work, and the others are done; more are shared out
+    // and merged pairwise.
+    const int warps = n <= 128 * E ? 1 : ROW_WARPS, threads = warps * 32;
+    if (warp >= warps) return;
+    auto sync = [&]() {
+        if (warps == 1)
+            __syncwarp();
+        else
+            __syncthreads();
+    };
+    auto choose = [&]() {
+        BestList<GroupKey, E> list;
+        list.init(sh.wait[warp], p.width, lane);
+        for (int c0 = warp * 32; c0 < n; c0 += threads)
+        {
+            int beam = 0;
+            unsigned index = 0;
+            const double total = c0 + lane < n ? totalOf(c0 + lane, beam, index) : NEG_INF;
+            const GroupKey key{ ordered64(total), ~index };
+            list.push(total > NEG_INF && better(key, list.bar), key);
+        }
+        for (int k0 = warp * 32; p.finished && k0 < K; k0 += threads)
+        {
+            const int k = k0 + lane;
+            const double total = k < K && p.finished[row0 + k] ? (double)p.scores[row0 + k] : NEG_INF;
+            const GroupKey key{ ordered64(total), ~((unsigned)k * p.vocab) };
+            list.push(total > NEG_INF && better(key, list.bar), key);
+        }
+        list.finish();
+        __syncwarp();  // the buffer of waiting keys becomes the list
+#pragma unroll
+        for (int e = 0; e < E; e++) sh.wait[warp][e * 32 + lane] = list.list[e];
+        sync();
         for (int m = warps / 2; m > 0; m /= 2)
         {
             if (warp < m)
@@ -627,11 +689,11 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
                 GroupKey other[E];
 #pragma unroll
                 for (int e = 0; e < E; e++) other[e] = sh.wait[warp + m][e * 32 + lane];
-                mergeDown(best.list, other, lane);
+                mergeDown(list.list, other, lane);
 #pragma unroll
-                for (int e = 0; e < E; e++) sh.wait[warp][e * 32 + lane] = best.list[e];
+                for (int e = 0; e < E; e++) sh.wait[warp][e * 32 + lane] = list.list[e];
             }
-            __syncthreads();
+            sync();
         }
     };
     choose();
@@ -640,8 +702,11 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
     // lies around its last place.
     const GroupKey* list = sh.wait[0];
     const GroupKey last = list[p.width - 1];
-    auto mark = [&](int beam) { atomicOr(&sh.near[beam >> 5], 1u << (beam & 31)); };
-    for (int i = tid; i + 1 < p.width; i += ROW_THREADS)
+    auto mark = [&](int beam) {
+        atomicOr(&sh.near[beam >> 5], 1u << (beam & 31));
+        sh.repair = 1;
+    };
+    for (int i = tid; i + 1 < p.width; i += threads)
     {
         const GroupKey a = list[i], b = list[i + 1];
         if (!b.t || fromOrdered64(a.t) - fromOrdered64(b.t) > NEAR_TOTALS) continue;
@@ -649,13 +714,12 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
         if (ka == kb) continue;
         mark(ka);
         mark(kb);
-        sh.repair = 1;
     }
     if (last.t)
     {
         const double edge = fromOrdered64(last.t);
         const int kl = ~last.i / p.vocab;
-        for (int c = tid; c < n; c += ROW_THREADS)
+        for (int c = tid; c < n; c += threads)
         {
             int beam = 0;
             unsigned index = 0;
@@ -663,43 +727,41 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
             if (beam == kl || !(fabs(total - edge) <= NEAR_TOTALS)) continue;
             mark(beam);
             mark(kl);
-            sh.repair = 1;
         }
-        for (int k = tid; p.finished && k < K; k += ROW_THREADS)
+        for (int k = tid; p.finished && k < K; k += threads)
         {
             if (!p.finished[row0 + k] || k == kl || !(fabs((double)p.scores[row0 + k] - edge) <= NEAR_TOTALS)) continue;
             mark(kl);
-            sh.repair = 1;
         }
     }
-    __syncthreads();
+    sync();
     if (sh.repair)
     {
         for (int k = 0; k < K; k++)
         {
-            if (!(sh.near[k >> 5] >> (k & 31) & 1) || !readsLogits(p, row0 + k)) continue;  // the same for the whole block
+            if (!(sh.near[k >> 5] >> (k & 31) & 1) || !readsLogits(p, row0 + k)) continue;  // the same for all threads
             const T* x = rowLogits<T>(p, g, k);
             const uint8_t* allowed = rowMask(p, g, k);
             const double t = (double)topOf(k);
             double sum = 0.0;
-            for (int a = tid; a < p.vocab; a += ROW_THREADS)
+            for (int a = tid; a < p.vocab; a += threads)
                 if (!allowed || allowed[a]) sum += exp((double)toFloat(x[a]) - t);
 #pragma unroll
             for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
             if (lane == 0) sh.red[warp] = sum;
-            __syncthreads();
+            sync();
             if (tid == 0)
             {
                 sum = 0.0;
-                for (int w = 0; w < ROW_WARPS; w++) sum += sh.red[w];
+                for (int w = 0; w < warps; w++) sum += sh.red[w];
                 base[k] = (double)p.scores[row0 + k] - (t + log(sum));
             }
-            __syncthreads();
+            sync();
         }
         choose();
     }
 
-    for (int i = tid; i < p.width; i += ROW_THREADS)
+    for (int i = tid; i < p.width; i += threads)
     {
         const GroupKey key = list[i];
         const unsigned index = ~key.i;
@@ -710,217 +772,74 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
     }
 }
 
-// From the segments' lists.
+// Long rows: from the segments' results.
 template <class T, int E>
 __global__ void __launch_bounds__(ROW_THREADS) selectMergeKernel(BeamParams p)
 {
     __shared__ double baseS[BEAM_MAX_BEAMS];
     __shared__ GroupShared<E> sh;
     const long long g = blockIdx.x, row0 = g * p.beams;
-    const int segs = p.segs, per = segs * p.width;
-    const RowKey* keys = p.keys + row0 * per;
+    const int segs = p.segs;
     const float* tops = p.top + row0 * segs;
     const double* sums = p.sum + row0 * segs;
+    const float* chunks = p.chunks + row0 * segs * 32;
     auto topOf = [&](int k) {
         float t = NEG_INF;
         for (int s = 0; s < segs; s++) t = fmaxf(t, tops[k * segs + s]);
         return t;
     };
-    for (int k = threadIdx.x; k < p.beams; k += ROW_THREADS)
+    // A warp per beam, its lanes over the segments.
+    for (int k = threadIdx.x >> 5; k < p.beams; k += ROW_WARPS)
     {
+        const int lane = threadIdx.x & 31;
         double b = NEG_INF;
-        const float t = readsLogits(p, row0 + k) ? topOf(k) : NEG_INF;
-        if (t > NEG_INF)
+        if (readsLogits(p, row0 + k))
         {
+            float t = NEG_INF;
+            for (int s = lane; s < segs; s += 32) t = fmaxf(t, tops[k * segs + s]);
+            t = fromOrdered(__reduce_max_sync(FULL, ordered(t)));
             double sum = 0.0;
-            for (int s = 0; s < segs; s++)
+            for (int s = lane; s < segs; s += 32)
             {
                 // A segment without a finite logit has sum 0, or NaN where one was NaN.
                 const float ts = tops[k * segs + s];
                 sum += ts > NEG_INF && ts < t ? sums[k * segs + s] * exp((double)ts - (double)t) : sums[k * segs + s];
             }
-            b = (double)p.scores[row0 + k] - ((double)t + log(sum));
+#pragma unroll
+            for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
+            if (t > NEG_INF) b = (double)p.scores[row0 + k] - ((double)t + log(sum));
+        }
+        if (lane == 0) baseS[k] = b;
+    }
+    __syncthreads();
+    finishGroup<T, E>(p, g, segs, [&](int c) { return chunks[c]; }, topOf, baseS, sh);
+}
+
+// Short rows: a block per group for both.
+constexpr int GROUP_MAX_BEAMS = 64;
+
+template <class T, bool MASKED>
+__global__ void __launch_bounds__(ROW_THREADS, 4) selectGroupKernel(BeamParams p)
+{
+    __shared__ float chunkS[GROUP_MAX_BEAMS * 32], topS[GROUP_MAX_BEAMS];
+    __shared__ double baseS[GROUP_MAX_BEAMS];
+    __shared__ GroupShared<1> sh;
+    const int lane = threadIdx.x & 31;
+    const long long g = blockIdx.x;
+    for (int k = threadIdx.x >> 5; k < p.beams; k += ROW_WARPS)
+    {
+        double b = NEG_INF;
+        if (readsLogits(p, g * p.beams + k))
+        {
+            const Scan scan = scanRow<T, MASKED>(Row<T>(p, g, k, lane), 0, 1);
+            if (scan.top > NEG_INF) b = (double)p.scores[g * p.beams + k] - ((double)scan.top + log(scan.sum));
+            chunkS[k * 32 + lane] = scan.laneTop;
+            topS[k] = scan.top;
         }
         baseS[k] = b;
     }
     __syncthreads();
-    auto candidate = [&](int c, int& beam, unsigned& index) {
-        beam = c / per;
-        if (!(baseS[beam] > NEG_INF)) return NEG_INF;
-        const RowKey key = keys[c];
-        if (!key) return NEG_INF;
-        index = (unsigned)beam * p.vocab + ~(unsigned)key;
-        return fromOrdered((unsigned)(key >> 32));
-    };
-    finishGroup<T, E>(p, g, p.beams * per, candidate, topOf, baseS, sh);
-}
-
-// ---- short rows: a block per group ------------------------------------------------------
-
-// A group's rows are read by the warps of one block.  The lanes' largest totals give a
-// bar for the whole group, the width-th largest of them; the few elements that reach it
-// (with a margin for rounding) are the group's candidates.  Where more reach it than
-// there is room for (rows of equal logits), the rows' own best take their place.
-constexpr int GROUP_MAX_BEAMS = 64;
-constexpr int GROUP_MAX_KEYS = 1024;
-
-template <class T, bool MASKED>
-__global__ void __launch_bounds__(ROW_THREADS, 3) selectGroupKernel(BeamParams p)
-{
-    __shared__ RowKey keyS[GROUP_MAX_KEYS];        // ordered logit, beam * vocab + action
-    __shared__ float topS[GROUP_MAX_BEAMS];
-    __shared__ double baseS[GROUP_MAX_BEAMS];
-    __shared__ unsigned laneS[ROW_THREADS];
-    __shared__ float barS;
-    __shared__ int countS;
-    __shared__ union { RowKey wait[ROW_WARPS][64]; GroupShared<1> group; } sh;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = p.beams;
-    const long long g = blockIdx.x;
-    if (threadIdx.x == 0) countS = 0;
-
-    unsigned w[Row<T>::WORDS], m[8];
-    int held = -1, heldTile = 0;                   // the tile in registers
-    float laneBest = NEG_INF;                      // largest total of the lane
-    for (int k = warp; k < K; k += ROW_WARPS)
-    {
-        double b = NEG_INF;
-        RowSum sum;
-        if (readsLogits(p, g * K + k))
-        {
-            const Row<T> row(rowLogits<T>(p, g, k), rowMask(p, g, k), p.vocab, lane);
-            float laneTop = NEG_INF;
-            for (int t = 0; t < row.tiles; t++)
-            {
-                row.template load<MASKED>(t, w, m);
-                if (MASKED) Row<T>::hide(w, m);
-                held = k;
-                heldTile = t;
-                const float tileTop = fmaxf(fmaxf(Row<T>::largest8(w, 0), Row<T>::largest8(w, 1)),
-                                            fmaxf(Row<T>::largest8(w, 2), Row<T>::largest8(w, 3)));
-                laneTop = fmaxf(laneTop, tileTop);
-                sum.raise(tileTop);
-#pragma unroll
-                for (int q = 0; q < 4; q++)
-                    if ((t * Row<T>::NV + q * Row<T>::NV / 4) * 32 < row.vectors) sum.template add8<T>(w, q);
-            }
-            if (row.head + row.tail > 0)
-            {
-                float v;
-                row.edge(v);
-                laneTop = fmaxf(laneTop, v);
-                sum.raise(fmaxf(v, NEG_INF));
-                sum.add(v);
-            }
-            sum.gather();
-            if (sum.top > NEG_INF) b = (double)p.scores[g * K + k] - ((double)sum.top + log(sum.sum));
-            if (b > NEG_INF && laneTop > NEG_INF) laneBest = fmaxf(laneBest, (float)(b + (double)laneTop));
-        }
-        if (lane == 0)
-        {
-            topS[k] = sum.top;
-            baseS[k] = b;
-        }
-    }
-    laneS[threadIdx.x] = laneBest > NEG_INF ? ordered(laneBest) : 0;
-    __syncthreads();
-    if (warp == 0)
-    {
-        unsigned v[ROW_WARPS], top = 0;
-#pragma unroll
-        for (int i = 0; i < ROW_WARPS; i++) v[i] = laneS[i * 32 + lane];
-        for (int left = p.width; left > 0;)
-        {
-            unsigned mine = v[0];
-#pragma unroll
-            for (int i = 1; i < ROW_WARPS; i++) mine = max(mine, v[i]);
-            top = __reduce_max_sync(FULL, mine);
-            if (top == 0) break;
-            int hits = 0;
-#pragma unroll
-            for (int i = 0; i < ROW_WARPS; i++)
-            {
-                hits += v[i] == top;
-                if (v[i] == top) v[i] = 0;
-            }
-            left -= __reduce_add_sync(FULL, hits);
-        }
-        if (lane == 0)
-        {
-            // Lower by twice NEAR_TOTALS and by eight roundings to float32.
-            const float t = fromOrdered(top);
-            barS = top && fabsf(t) < FLT_MAX ? t - (2.f * (float)NEAR_TOTALS + 8.f * 0x1p-24f * fabsf(t)) : NEG_INF;
-        }
-    }
-    __syncthreads();
-    const float bar = barS;
-    auto offer = [&](float v, int k, int action) {
-        const int at = atomicAdd(&countS, 1);
-        if (at < GROUP_MAX_KEYS) keyS[at] = (RowKey)ordered(v) << 32 | ((unsigned)k * p.vocab + action);
-    };
-    for (int k = (K - 1 - warp) / ROW_WARPS * ROW_WARPS + warp; k >= 0 && warp < K; k -= ROW_WARPS)
-    {
-        const double b = baseS[k];
-        if (!(b > NEG_INF)) continue;
-        // Logits of this row that can reach the bar.
-        const float need = b < (double)INFINITY && bar > NEG_INF ? fmaxf((float)((double)bar - b), -FLT_MAX) : -FLT_MAX;
-        const float margin = need > -FLT_MAX ? need - 2.f * 0x1p-24f * fabsf(need) : need;
-        if (!(topS[k] >= margin)) continue;
-        const Row<T> row(rowLogits<T>(p, g, k), rowMask(p, g, k), p.vocab, lane);
-        for (int t = row.tiles - 1; t >= 0; t--)
-        {
-            if (held != k || heldTile != t)
-            {
-                row.template load<MASKED>(t, w, m);
-                if (MASKED) Row<T>::hide(w, m);
-            }
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-            {
-                if (!(Row<T>::largest8(w, q) >= margin)) continue;
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                {
-                    const float v = Row<T>::element(w, 8 * q + i);
-                    if (v >= margin) offer(v, k, row.action(t, 8 * q + i));
-                }
-            }
-        }
-        if (row.head + row.tail > 0)
-        {
-            float v;
-            const int a = row.edge(v);
-            if (v >= margin) offer(v, k, a);
-        }
-    }
-    __syncthreads();
-    int n = countS;
-    if (n > GROUP_MAX_KEYS)
-    {
-        for (int k = warp; k < K; k += ROW_WARPS)
-        {
-            BestList<RowKey, 1> best;
-            best.init(sh.wait[warp], p.width, lane);
-            RowSum sum;
-            if (baseS[k] > NEG_INF)
-                scanRow<T, 1, MASKED>(Row<T>(rowLogits<T>(p, g, k), rowMask(p, g, k), p.vocab, lane), p.width, 0, 1,
-                                      sh.wait[warp], best, sum);
-            const RowKey key = best.list[0];
-            if (lane < p.width)
-                keyS[k * p.width + lane] = key ? (key & ~0xffffffffull) | ((unsigned)k * p.vocab + ~(unsigned)key) : 0;
-            __syncwarp();
-        }
-        n = K * p.width;
-        __syncthreads();
-    }
-    auto candidate = [&](int c, int& beam, unsigned& index) {
-        const RowKey key = keyS[c];
-        if (!key) return NEG_INF;
-        index = (unsigned)key;
-        beam = index / p.vocab;
-        return fromOrdered((unsigned)(key >> 32));
-    };
-    auto topOf = [&](int k) { return topS[k]; };
-    finishGroup<T, 1>(p, g, n, candidate, topOf, baseS, sh.group);
+    finishGroup<T, 1>(p, g, 1, [&](int c) { return chunkS[c]; }, [&](int k) { return topS[k]; }, baseS, sh);
 }
 
 // ---- selection over the action heads ---------------------------------------------------
@@ -1211,34 +1130,29 @@ __global__ void __launch_bounds__(REORDER_THREADS) moveContactsKernel(int* conta
     if (contact[car] >= 0) contact[car] += (j - (int)parent) * nCars;
 }
 
-template <class T, int E, bool MASKED>
+template <class T>
 void launchSelect(const BeamParams& p, cudaStream_t s)
 {
-    const long long items = (long long)p.groups * p.beams * p.segs;
-    selectRowsKernel<T, E, MASKED><<<(unsigned)((items + ROW_WARPS - 1) / ROW_WARPS), ROW_THREADS, 0, s>>>(p);
-    selectMergeKernel<T, E><<<p.groups, ROW_THREADS, 0, s>>>(p);
-}
-
-template <class T, bool MASKED>
-void launchSelectWidth(const BeamParams& p, cudaStream_t s)
-{
     if (p.segs == 0)
-        selectGroupKernel<T, MASKED><<<p.groups, ROW_THREADS, 0, s>>>(p);
-    else if (p.width <= 32)
-        launchSelect<T, 1, MASKED>(p, s);
-    else if (p.width <= 64)
-        launchSelect<T, 2, MASKED>(p, s);
-    else
-        launchSelect<T, 4, MASKED>(p, s);
-}
-
-template <class T>
-void launchSelectMasked(const BeamParams& p, cudaStream_t s)
-{
+    {
+        if (p.mask)
+            selectGroupKernel<T, true><<<p.groups, ROW_THREADS, 0, s>>>(p);
+        else
+            selectGroupKernel<T, false><<<p.groups, ROW_THREADS, 0, s>>>(p);
+        return;
+    }
+    const long long items = (long long)p.groups * p.beams * p.segs;
+    const unsigned blocks = (unsigned)((items + ROW_WARPS - 1) / ROW_WARPS);
     if (p.mask)
-        launchSelectWidth<T, true>(p, s);
+        selectRowsKernel<T, true><<<blocks, ROW_THREADS, 0, s>>>(p);
     else
-        launchSelectWidth<T, false>(p, s);
+        selectRowsKernel<T, false><<<blocks, ROW_THREADS, 0, s>>>(p);
+    if (p.width <= 32)
+        selectMergeKernel<T, 1><<<p.groups, ROW_THREADS, 0, s>>>(p);
+    else if (p.width <= 64)
+        selectMergeKernel<T, 2><<<p.groups, ROW_THREADS, 0, s>>>(p);
+    else
+        selectMergeKernel<T, 4><<<p.groups, ROW_THREADS, 0, s>>>(p);
 }
 
 template <class T, int N>
@@ -1268,37 +1182,33 @@ void launchJointWidth(const BeamParams& p, cudaStream_t s)
 long long planBeamSelect(BeamParams& p, LogitType type, void* base)
 {
     const long long rows = (long long)p.groups * p.beams;
-    const int tiles = (p.vocab + 1023) / 1024;
-    // Warps the card holds at a time, at the pass's register use.
-    constexpr long long WARPS = 148 * 16;
-    (void)type;
-    // A block per group re-reads rows of more than one tile, and its warps take the rows
-    // of more than eight beams in turn.
-    const bool fits = p.width <= 32 && p.width <= 16 * p.beams && p.beams <= GROUP_MAX_BEAMS
-                      && p.beams * p.width <= GROUP_MAX_KEYS;
+    const int tiles = (int)(((long long)p.vocab * (type == LOGITS_F32 ? 4 : 2) + 2047) / 2048);  // of a warp's pass
+    // Short rows are one block's work per group.
     const int turns = tiles * ((p.beams + ROW_WARPS - 1) / ROW_WARPS);
-    if (fits && (turns <= 2 || (tiles <= 4 && p.groups >= 2 * 148)))
+    if (p.width <= 32 && p.beams <= GROUP_MAX_BEAMS && (turns <= 4 || (tiles <= 16 && p.groups >= 4 * 148)))
     {
         p.segs = 0;
         return 0;
     }
+    // Warps the card holds at a time, at the pass's register use.
+    constexpr long long WARPS = 148 * 32;
     p.segs = (int)std::max<long long>(1, std::min<long long>(tiles, WARPS / std::max<long long>(1, rows)));
     const long long items = rows * p.segs;
     char* c = static_cast<char*>(base);
     p.sum = reinterpret_cast<double*>(c);
-    p.keys = reinterpret_cast<unsigned long long*>(c + items * 8);
-    p.top = reinterpret_cast<float*>(c + items * 8 * (1 + p.width));
-    return items * (8 * (1 + p.width) + 4);
+    p.top = reinterpret_cast<float*>(c + items * 8);
+    p.chunks = reinterpret_cast<float*>(c + items * 12);
+    return items * (12 + 128);
 }
 
 void launchBeamSelect(const BeamParams& p, LogitType type, cudaStream_t s)
 {
     if (type == LOGITS_F32)
-        launchSelectMasked<float>(p, s);
+        launchSelect<float>(p, s);
     else if (type == LOGITS_BF16)
-        launchSelectMasked<__nv_bfloat16>(p, s);
+        launchSelect<__nv_bfloat16>(p, s);
     else
-        launchSelectMasked<__half>(p, s);
+        launchSelect<__half>(p, s);
 }
 
 void launchJointSelect(const BeamParams& p, LogitType type, cudaStream_t s)

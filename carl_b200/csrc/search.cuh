@@ -26,10 +26,11 @@ struct BeamParams
     float* outScores;                   // [groups, width]
     long long* outParents;
     int* outActions;                    // [groups, width] (joint: [groups, width, 7])
-    unsigned long long* keys;           // workspace: [rows, segs, width] best of each row segment
+    double* sum;                        // workspace: [rows, segs] sum of exp(logit - top)
     float* top;                         // [rows, segs] largest logit
-    double* sum;                        // [rows, segs] sum of exp(logit - top)
-    int groups, beams, vocab, width, segs;
+    float* chunks;                      // [rows, segs, 32] largest logit of each lane's part
+    int groups, beams, vocab, width;
+    int segs;                           // warps to a row; 0: a block to a group
 };
 
 // Workspace bytes of a flat selection, and its pointers into `base`; sets p.segs.
