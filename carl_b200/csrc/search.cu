@@ -300,8 +300,6 @@ template <class T>
 struct Row
 {
     static constexpr int VE = 16 / sizeof(T);   // elements of a vector
-    static constexpr int NV = 4;                // vectors of a lane per tile
-    static constexpr int MASKS = NV * VE / 4;   // 32-bit words of mask bytes
     const T* x;
     const uint8_t* allowed;
     int head, vectors, tail, lane;
@@ -315,39 +313,39 @@ struct Row
         tail = p.vocab - head - vectors * VE;
         wideMask = (reinterpret_cast<uintptr_t>(allowed + head) & 3) == 0;
     }
-    __device__ static int segmentStart(int vectors, int seg, int segs)
+    // Vectors v0 + lane + 32 j below `end`; beyond it they are -inf.  A j with nothing below
+    // `end` for the whole warp is left out, here and by what follows.
+    template <bool MASKED, int NV>
+    __device__ __forceinline__ void load(int v0, int end, uint4 (&w)[NV], unsigned (&m)[NV * VE / 4]) const
     {
-        const int blocks = (vectors + 31) / 32;
-        return (int)((long long)blocks * seg / segs) * 32;
-    }
-
-    // Vectors v0 + lane + 32 j, those below `end`; the others are -inf.
-    template <bool MASKED>
-    __device__ __forceinline__ void load(int v0, int end, uint4 (&w)[NV], unsigned (&m)[MASKS]) const
-    {
-        const uint4* v = reinterpret_cast<const uint4*>(x + head);
+        const uint4* v = reinterpret_cast<const uint4*>(x + head) + lane;
+        const uint8_t* a = allowed + head + lane * VE;
 #pragma unroll
         for (int j = 0; j < NV; j++)
         {
-            const int i = v0 + 32 * j + lane;
-            w[j] = make_uint4(Words<T>::NONE, Words<T>::NONE, Words<T>::NONE, Words<T>::NONE);
-            if (i < end) w[j] = __ldcs(v + i);
-            if (MASKED)
+            const int i = v0 + 32 * j;
+            if (i >= end) break;
+            if (i + lane < end)
             {
-                const uint8_t* a = allowed + head + (long long)i * VE;
-#pragma unroll
-                for (int q = 0; q < VE / 4; q++)
+                w[j] = __ldcs(v + i);
+                if (MASKED)
                 {
-                    unsigned b = 0;
-                    if (i < end)
+#pragma unroll
+                    for (int q = 0; q < VE / 4; q++)
                     {
+                        const uint8_t* b = a + (long long)i * VE + 4 * q;
                         if (wideMask)
-                            b = __ldcs(reinterpret_cast<const unsigned*>(a + 4 * q));
+                            m[j * VE / 4 + q] = __ldcs(reinterpret_cast<const unsigned*>(b));
                         else
-                            b = a[4 * q] | a[4 * q + 1] << 8 | a[4 * q + 2] << 16 | (unsigned)a[4 * q + 3] << 24;
+                            m[j * VE / 4 + q] = b[0] | b[1] << 8 | b[2] << 16 | (unsigned)b[3] << 24;
                     }
-                    m[j * VE / 4 + q] = b;
                 }
+            }
+            else
+            {
+                w[j] = make_uint4(Words<T>::NONE, Words<T>::NONE, Words<T>::NONE, Words<T>::NONE);
+#pragma unroll
+                for (int q = 0; MASKED && q < VE / 4; q++) m[j * VE / 4 + q] = 0;
             }
         }
     }
@@ -413,31 +411,36 @@ struct Scan
     __device__ __forceinline__ float ref() const { return top > NEG_INF ? top : 0.f; }
 };
 
-// One warp over segment `seg` of a row.  Nothing is selected here: the lanes' maxima
-// tell later which chunks can hold one of the best, and only those are read again.
-template <class T, bool MASKED>
-__device__ __forceinline__ Scan scanRow(const Row<T>& row, int seg, int segs)
+// One warp over vectors [begin, end) of a row, NV vectors a lane at a time.  Nothing is selected
+// here: the lanes' maxima tell later which chunks can hold one of the best, and only
+// those are read again.  AHEAD: the next vectors are loaded before these are used.
+template <class T, bool MASKED, int NV, bool AHEAD>
+__device__ __forceinline__ Scan scanRow(const Row<T>& row, int begin, int end)
 {
-    constexpr int NV = Row<T>::NV, VE = Row<T>::VE;
+    constexpr int VE = Row<T>::VE, MASKS = NV * VE / 4;
     Scan scan;
-    const int begin = Row<T>::segmentStart(row.vectors, seg, segs);
-    const int end = min(row.vectors, Row<T>::segmentStart(row.vectors, seg + 1, segs));
-    uint4 next[NV];
-    unsigned nextMask[Row<T>::MASKS];
-    if (begin < end) row.template load<MASKED>(begin, end, next, nextMask);
+    uint4 w[NV], next[AHEAD ? NV : 1];
+    unsigned m[MASKS], nextMask[AHEAD ? MASKS : 1];
+    if constexpr (AHEAD) row.template load<MASKED, NV>(begin, end, next, nextMask);
     for (int v0 = begin; v0 < end; v0 += 32 * NV)
     {
-        uint4 w[NV];
-        unsigned m[Row<T>::MASKS];
+        if constexpr (AHEAD)
+        {
 #pragma unroll
-        for (int j = 0; j < NV; j++) w[j] = next[j];
+            for (int j = 0; j < NV; j++) w[j] = next[j];
 #pragma unroll
-        for (int j = 0; j < Row<T>::MASKS; j++) m[j] = nextMask[j];
-        if (v0 + 32 * NV < end) row.template load<MASKED>(v0 + 32 * NV, end, next, nextMask);
+            for (int j = 0; MASKED && j < MASKS; j++) m[j] = nextMask[j];
+            row.template load<MASKED, NV>(v0 + 32 * NV, end, next, nextMask);
+        }
+        else
+        {
+            row.template load<MASKED, NV>(v0, end, w, m);
+        }
         unsigned most = Words<T>::NONE;
 #pragma unroll
         for (int j = 0; j < NV; j++)
         {
+            if (v0 + 32 * j >= end) break;  // the same for the whole warp
             if (MASKED) Row<T>::hide(w[j], m + j * VE / 4);
             most = Words<T>::larger(most, Words<T>::larger(Words<T>::larger(w[j].x, w[j].y), Words<T>::larger(w[j].z, w[j].w)));
         }
@@ -446,7 +449,7 @@ __device__ __forceinline__ Scan scanRow(const Row<T>& row, int seg, int segs)
 #pragma unroll
         for (int j = 0; j < NV; j += 8 / VE)
         {
-            if (v0 + 32 * j >= end) break;  // the same for the whole warp
+            if (v0 + 32 * j >= end) break;
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -455,10 +458,15 @@ __device__ __forceinline__ Scan scanRow(const Row<T>& row, int seg, int segs)
                 const int e = i % VE / Words<T>::PER;
                 v[i] = Words<T>::at(e == 0 ? r.x : e == 1 ? r.y : e == 2 ? r.z : r.w, i % Words<T>::PER);
             }
+            if (VE == 4 && v0 + 32 * (j + 1) >= end)
+            {
+#pragma unroll
+                for (int i = 4; i < 8; i++) v[i] = NEG_INF;
+            }
             scan.sum += sumExp8(v, ref);
         }
     }
-    if (seg == 0 && row.head + row.tail > 0)
+    if (begin == 0 && row.head + row.tail > 0)
     {
         float v;
         row.edge(v);
@@ -466,7 +474,7 @@ __device__ __forceinline__ Scan scanRow(const Row<T>& row, int seg, int segs)
         scan.sum += exp2Approx((v - scan.ref()) * LOG2E);
     }
 #pragma unroll
-    for (int m = 16; m > 0; m /= 2) scan.sum += __shfl_xor_sync(FULL, scan.sum, m);
+    for (int d = 16; d > 0; d /= 2) scan.sum += __shfl_xor_sync(FULL, scan.sum, d);
     return scan;
 }
 
@@ -482,7 +490,9 @@ __global__ void __launch_bounds__(ROW_THREADS) selectRowsKernel(BeamParams p)
     if (item >= (long long)p.groups * p.beams * p.segs) return;
     const long long r = item / p.segs, g = r / p.beams;
     if (!readsLogits(p, r)) return;
-    const Scan scan = scanRow<T, MASKED>(Row<T>(p, g, (int)(r - g * p.beams), lane), (int)(item - r * p.segs), p.segs);
+    const Row<T> row(p, g, (int)(r - g * p.beams), lane);
+    const int begin = (int)(item - r * p.segs) * p.segVectors;
+    const Scan scan = scanRow<T, MASKED, 4, true>(row, begin, min(row.vectors, begin + p.segVectors));
     p.chunks[item * 32 + lane] = scan.laneTop;
     if (lane == 0)
     {
@@ -501,168 +511,325 @@ __global__ void __launch_bounds__(ROW_THREADS) selectRowsKernel(BeamParams p)
 // twice that are in order.  Nearer ones are decided by normalisers in 64 bits.
 constexpr double NEAR_TOTALS = 8e-6;
 
-constexpr int MAX_CHUNKS = 512;       // chunks of a group that are read again
-constexpr int MAX_CANDIDATES = 1024;  // and their elements that reach the bar
-
-template <int E>
-struct GroupShared
+// A continuation that reaches the group's bar.
+struct Candidate
 {
-    GroupKey wait[ROW_WARPS][32 * E + 32];
-    u64 found[MAX_CANDIDATES];        // ordered logit, beam * vocab + action
-    int chunk[MAX_CHUNKS];
-    unsigned tops[ROW_THREADS];       // the threads' largest totals
-    double red[ROW_WARPS];
+    double total;
+    unsigned index;  // beam * vocab + action
+    int beam;
+};
+
+// THREADS: a block's, or one warp's.
+template <int THREADS, int E>
+struct alignas(16) GroupShared
+{
+    static constexpr int WARPS = THREADS / 32;
+    static constexpr int CHUNKS = THREADS == 32 ? 128 : 512;       // chunks that are read again
+    static constexpr int CANDIDATES = THREADS == 32 ? 128 : 1024;  // and their elements that reach the bar
+    GroupKey wait[WARPS][32 * E + 32];
+    Candidate found[CANDIDATES];
+    int chunk[CHUNKS];
+    unsigned tops[THREADS];
+    double red[WARPS];
     unsigned near[BEAM_MAX_BEAMS / 32];
     unsigned bar;
     int chunks, candidates, repair;
 };
 
-// The n-th largest (n <= 128) of the values that the block's threads hold (0: none), to
-// sh.bar.
-template <int E>
-__device__ __forceinline__ void nthLargest(unsigned mine, int n, GroupShared<E>& sh)
+template <int THREADS>
+__device__ __forceinline__ void groupSync()
 {
-    const int tid = threadIdx.x, lane = tid & 31;
-    sh.tops[tid] = mine;
-    if (tid == 0) sh.bar = n <= 12 ? 0 : 0xffffffffu;
-    __syncthreads();
-    if (n <= 12)
-    {
-        // One warp takes the maximum out n times.
-        if (tid < 32)
-        {
-            unsigned v[ROW_WARPS], top = 0;
-#pragma unroll
-            for (int i = 0; i < ROW_WARPS; i++) v[i] = sh.tops[i * 32 + lane];
-            for (int left = n; left > 0;)
-            {
-                unsigned most = v[0];
-#pragma unroll
-                for (int i = 1; i < ROW_WARPS; i++) most = max(most, v[i]);
-                top = __reduce_max_sync(FULL, most);
-                if (top == 0) break;
-                int hits = 0;
-#pragma unroll
-                for (int i = 0; i < ROW_WARPS; i++)
-                {
-                    hits += v[i] == top;
-                    if (v[i] == top) v[i] = 0;
-                }
-                left -= __reduce_add_sync(FULL, hits);
-            }
-            if (lane == 0) sh.bar = top;
-        }
-    }
+    if (THREADS == 32)
+        __syncwarp();
     else
-    {
-        // The smallest of the values with fewer than n above them.
-        int above = 0;
-        for (int i = 0; i < ROW_THREADS; i++) above += sh.tops[i] > mine;
-        const unsigned least = __reduce_min_sync(FULL, above < n ? mine : 0xffffffffu);
-        if (lane == 0) atomicMin(&sh.bar, least);
-    }
-    __syncthreads();
+        __syncthreads();
 }
 
-// A block finds its group's best and writes them.  chunkTop(c) is the largest logit of
-// chunk c = (beam * segs + segment) * 32 + lane, topOf(k) that of beam k; base[k] is the
-// score minus the normaliser, -inf where beam k has no continuation.
+// A value that at least n of the threads' `mine` reach, the n-th largest where it can be
+// told quickly (0: there are none).
+template <int THREADS, int E>
+__device__ __forceinline__ unsigned nthLargest(unsigned mine, int n, int tid, GroupShared<THREADS, E>& sh)
+{
+    const int lane = tid & 31;
+    unsigned top = 0;
+    if (THREADS == 32 && n <= 12)
+    {
+        // The maximum is taken out n times.
+        for (int left = n; left > 0;)
+        {
+            top = __reduce_max_sync(FULL, mine);
+            const bool hit = mine == top;
+            left -= __popc(__ballot_sync(FULL, hit));
+            if (hit) mine = 0;
+            if (top == 0) break;
+        }
+        return top;
+    }
+    // The smallest of the values with fewer than n above them.
+    sh.tops[tid] = mine;
+    if (tid == 0) sh.bar = 0xffffffffu;
+    groupSync<THREADS>();
+    int above = 0;
+    const uint4* t = reinterpret_cast<const uint4*>(sh.tops);
+#pragma unroll 8
+    for (int i = 0; i < THREADS / 4; i++)
+    {
+        const uint4 v = t[i];
+        above += (v.x > mine) + (v.y > mine) + (v.z > mine) + (v.w > mine);
+    }
+    const unsigned least = __reduce_min_sync(FULL, above < n ? mine : 0xffffffffu);
+    if (lane == 0) atomicMin(&sh.bar, least);
+    groupSync<THREADS>();
+    return sh.bar;
+}
+
+// A group's best, found and written by a block or a warp.  chunkTop(c) is the largest
+// logit of chunk c = (beam * segs + segment) * 32 + lane, topOf(k) that of beam k; base[k]
+// is the score minus the normaliser, -inf where beam k reads no logits or has none; and
+// overOf(k) is the score of a finished beam, -inf of another.
 //
 // The width-th largest of the threads' largest totals is a bar that `width` elements
 // reach; the chunks that reach it (lowered by the margin of the comparison) are read
-// again, and their elements that do are the candidates.  Where there are too many of
-// either (rows of equal logits), every element is one.
-template <class T, int E, class ChunkTop, class TopOf>
-__device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, int segs, ChunkTop chunkTop, TopOf topOf,
-                                            double* base, GroupShared<E>& sh)
+// again, and their elements that do are the candidates, usually little more than
+// `width`.  Each thread then counts the candidates that go before its own, which is that
+// one's place.  Where there are too many for that (rows of equal logits), sorted lists
+// take over, of every element if need be.
+template <class T, int THREADS, int E, class ChunkTop, class TopOf, class OverOf>
+__device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, int tid, ChunkTop chunkTop,
+                                            TopOf topOf, OverOf overOf, double* base, GroupShared<THREADS, E>& sh)
 {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    using Shared = GroupShared<THREADS, E>;
+    constexpr int VE = Row<T>::VE;
+    const int lane = tid & 31, warp = tid >> 5;
     const long long row0 = g * p.beams;
+    const int segs = THREADS == 32 ? 1 : p.segs, segVectors = THREADS == 32 ? 1 << 30 : p.segVectors;  // a warp's rows are whole
     const int K = p.beams, all = K * segs * 32;
+    const auto sync = [] { groupSync<THREADS>(); };
 
     if (tid == 0) sh.chunks = sh.candidates = sh.repair = 0;
-    if (tid < BEAM_MAX_BEAMS / 32) sh.near[tid] = 0;
+    // The totals of the chunks, some at a time so that their loads overlap.
+    constexpr int AT_ONCE = 8;
+    const auto chunkTotals = [&](int c0, float (&top)[AT_ONCE], double (&total)[AT_ONCE]) {
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; j++)
+        {
+            const int c = c0 + j * THREADS;
+            top[j] = c < all ? chunkTop(c) : NEG_INF;
+        }
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; j++)
+        {
+            const int c = c0 + j * THREADS;
+            const double b = c < all ? base[(c >> 5) / segs] : (double)NEG_INF;
+            total[j] = b > NEG_INF && top[j] > NEG_INF ? b + (double)top[j] : (double)NEG_INF;
+        }
+    };
     float best = NEG_INF;
-    for (int c = tid; c < all; c += ROW_THREADS)
+    for (int c0 = tid; c0 < all; c0 += AT_ONCE * THREADS)
     {
-        const double b = base[c / (32 * segs)];
-        if (b > NEG_INF) best = fmaxf(best, (float)(b + (double)chunkTop(c)));
+        float top[AT_ONCE];
+        double total[AT_ONCE];
+        chunkTotals(c0, top, total);
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; j++) best = fmaxf(best, (float)total[j]);
     }
-    nthLargest(best > NEG_INF ? ordered(best) : 0u, p.width, sh);
+    sync();
+    const unsigned nth = nthLargest<THREADS, E>(best > NEG_INF ? ordered(best) : 0u, p.width, tid, sh);
     // Lower by twice NEAR_TOTALS and by eight roundings to float32.
-    float bar = sh.bar && sh.bar != 0xffffffffu ? fromOrdered(sh.bar) : NEG_INF;
+    float bar = nth && nth != 0xffffffffu ? fromOrdered(nth) : NEG_INF;
     bar = fabsf(bar) < FLT_MAX ? bar - (2.f * (float)NEAR_TOTALS + 8.f * 0x1p-24f * fabsf(bar)) : NEG_INF;
-    for (int c = tid; c < all; c += ROW_THREADS)
+
+    const auto offer = [&](double total, unsigned index, int k) {
+        if (!(total > NEG_INF && total >= (double)bar)) return;
+        const int at = atomicAdd(&sh.candidates, 1);
+        if (at < Shared::CANDIDATES) sh.found[at] = Candidate{ total, index, k };
+    };
+    for (int c0 = tid; c0 < all; c0 += AT_ONCE * THREADS)
     {
-        const double b = base[c / (32 * segs)];
-        const float top = b > NEG_INF ? chunkTop(c) : NEG_INF;
-        if (!(top > NEG_INF && b + (double)top >= (double)bar)) continue;
-        const int at = atomicAdd(&sh.chunks, 1);
-        if (at < MAX_CHUNKS) sh.chunk[at] = c;
+        float top[AT_ONCE];
+        double total[AT_ONCE];
+        chunkTotals(c0, top, total);
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; j++)
+        {
+            if (!(total[j] > NEG_INF && total[j] >= (double)bar)) continue;
+            const int at = atomicAdd(&sh.chunks, 1);
+            if (at < Shared::CHUNKS) sh.chunk[at] = c0 + j * THREADS;
+        }
     }
-    __syncthreads();
+    for (int k = tid; p.finished && k < K; k += THREADS) offer((double)overOf(k), (unsigned)k * p.vocab, k);
+    sync();
+    // The vectors of all these chunks, shared out over the threads.
     const int chunks = sh.chunks;
-    for (int i = warp; i < chunks && chunks <= MAX_CHUNKS; i += ROW_WARPS)
+    const int per = (min(segVectors, p.vocab / VE) + 31) / 32 + 1;  // vectors of a chunk, and its edge
+    constexpr int VECTORS = 4;
+    for (int i0 = tid; chunks <= Shared::CHUNKS && i0 < chunks * per; i0 += VECTORS * THREADS)
     {
-        const int c = sh.chunk[i], k = c / (32 * segs), seg = c / 32 - k * segs;
-        const double b = base[k];
-        Row<T> row(p, g, k, c & 31);
-        const int begin = Row<T>::segmentStart(row.vectors, seg, segs) + row.lane;
-        const int end = min(row.vectors, Row<T>::segmentStart(row.vectors, seg + 1, segs));
-        auto offer = [&](float v, int action) {
-            if (!(v > NEG_INF && b + (double)v >= (double)bar)) return;
-            const int at = atomicAdd(&sh.candidates, 1);
-            if (at < MAX_CANDIDATES) sh.found[at] = (u64)ordered(v) << 32 | ((unsigned)k * p.vocab + action);
-        };
-        for (int e = lane;; e += 32)
+        uint4 r[VECTORS];
+        unsigned legal[VECTORS];
+        int action[VECTORS], beam[VECTORS];
+        double b[VECTORS];
+#pragma unroll
+        for (int u = 0; u < VECTORS; u++)
         {
-            const int v = begin + e / Row<T>::VE * 32;
-            if (v >= end) break;
-            const int action = row.head + v * Row<T>::VE + e % Row<T>::VE;
-            if (!row.allowed || row.allowed[action]) offer(toFloat(row.x[action]), action);
+            const int i = i0 + u * THREADS;
+            legal[u] = 0;
+            if (i >= chunks * per) continue;
+            const int j = i / per, v = i - j * per, c = sh.chunk[j], k = (c >> 5) / segs, seg = (c >> 5) - k * segs;
+            const Row<T> row(p, g, k, c & 31);
+            const int begin = THREADS == 32 ? 0 : seg * segVectors, at = begin + row.lane + 32 * v;
+            beam[u] = k;
+            b[u] = base[k];
+            if (v == per - 1)
+            {
+                float x;
+                action[u] = begin == 0 ? row.edge(x) : -1;
+                if (action[u] >= 0) offer(b[u] + (double)x, (unsigned)k * p.vocab + action[u], k);
+            }
+            else if (at < row.vectors && at - begin < segVectors)
+            {
+                r[u] = *(reinterpret_cast<const uint4*>(row.x + row.head) + at);
+                action[u] = row.head + at * VE;
+                legal[u] = (1u << VE) - 1;
+                if (row.allowed)
+                {
+                    legal[u] = 0;
+#pragma unroll
+                    for (int q = 0; q < VE; q++) legal[u] |= row.allowed[action[u] + q] ? 1u << q : 0u;
+                }
+            }
         }
-        if (seg == 0 && lane == 0)
+#pragma unroll
+        for (int u = 0; u < VECTORS; u++)
         {
-            float v;
-            const int action = row.edge(v);
-            if (action >= 0) offer(v, action);
+            const unsigned words[4] = { r[u].x, r[u].y, r[u].z, r[u].w };
+#pragma unroll
+            for (int q = 0; q < VE; q++)
+            {
+                if (!(legal[u] >> q & 1)) continue;
+                const double total = b[u] + (double)Words<T>::at(words[q / Words<T>::PER], q % Words<T>::PER);
+                if (total >= (double)bar) offer(total, (unsigned)beam[u] * p.vocab + action[u] + q, beam[u]);
+            }
         }
     }
-    __syncthreads();
-    const bool every = chunks > MAX_CHUNKS || sh.candidates > MAX_CANDIDATES;
+    sync();
+    const bool every = chunks > Shared::CHUNKS || sh.candidates > Shared::CANDIDATES;
     const int n = every ? K * p.vocab : sh.candidates;
+
+    // Marks beams whose totals are too near one another's, and computes the marked beams'
+    // normalisers in 64 bits, in an order that depends on nothing but the actions.
+    const auto clear = [&] {
+        for (int i = tid; i < BEAM_MAX_BEAMS / 32; i += THREADS) sh.near[i] = 0;
+        sync();
+    };
+    const auto mark = [&](int beam) {
+        atomicOr(&sh.near[beam >> 5], 1u << (beam & 31));
+        sh.repair = 1;
+    };
+    const auto marked = [&](int k) { return (sh.near[k >> 5] >> (k & 31) & 1) && readsLogits(p, row0 + k); };
+    const auto repair = [&] {
+        for (int k = 0; k < K; k++)
+        {
+            if (!marked(k)) continue;  // the same for all threads
+            const T* x = rowLogits<T>(p, g, k);
+            const uint8_t* allowed = rowMask(p, g, k);
+            const double t = (double)topOf(k);
+            double sum = 0.0;
+            for (int a = tid; a < p.vocab; a += THREADS)
+                if (!allowed || allowed[a]) sum += exp((double)toFloat(x[a]) - t);
+#pragma unroll
+            for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
+            if (lane == 0) sh.red[warp] = sum;
+            sync();
+            if (tid == 0)
+            {
+                sum = 0.0;
+                for (int w = 0; w < Shared::WARPS; w++) sum += sh.red[w];
+                base[k] = (double)p.scores[row0 + k] - (t + log(sum));
+            }
+            sync();
+        }
+    };
+    const auto write = [&](int place, double total, unsigned index) {
+        const long long o = g * p.width + place;
+        const int beam = index / p.vocab;
+        p.outScores[o] = (float)total;
+        p.outParents[o] = beam;
+        p.outActions[o] = index - (unsigned)beam * p.vocab;
+    };
+    const auto writeNone = [&](int place) {
+        const long long o = g * p.width + place;
+        p.outScores[o] = NEG_INF;
+        p.outParents[o] = place % K;
+        p.outActions[o] = 0;
+    };
+
+    if (n <= THREADS)
+    {
+        Candidate mine{ NEG_INF, 0, -1 };
+        if (tid < n) mine = sh.found[tid];
+        int place = 0;
+        bool near = false;
+#pragma unroll 4
+        for (int i = 0; i < n; i++)
+        {
+            const Candidate c = sh.found[i];
+            place += c.total > mine.total || (c.total == mine.total && c.index < mine.index);
+            near |= c.beam != mine.beam && fabs(c.total - mine.total) <= NEAR_TOTALS;
+        }
+        if (tid < n && near && place < p.width + 1) sh.repair = 1;
+        sync();
+        if (sh.repair)
+        {
+            clear();
+            for (int i = 0; tid < n && i < n; i++)
+            {
+                const Candidate c = sh.found[i];
+                if (c.beam != mine.beam && fabs(c.total - mine.total) <= NEAR_TOTALS) mark(mine.beam);
+            }
+            sync();
+            repair();
+            if (tid < n && marked(mine.beam))
+            {
+                const int action = mine.index - (unsigned)mine.beam * p.vocab;
+                mine.total = base[mine.beam] + (double)toFloat(rowLogits<T>(p, g, mine.beam)[action]);
+                sh.found[tid].total = mine.total;
+            }
+            sync();
+            place = 0;
+            for (int i = 0; i < n; i++)
+            {
+                const Candidate c = sh.found[i];
+                place += c.total > mine.total || (c.total == mine.total && c.index < mine.index);
+            }
+        }
+        if (tid < n && place < p.width) write(place, mine.total, mine.index);
+        for (int i = n + tid; i < p.width; i += THREADS) writeNone(i);
+        return;
+    }
 
     // Candidate c: its total, beam and index; -inf for none.
     auto totalOf = [&](int c, int& beam, unsigned& index) {
-        if (every)
+        if (!every)
         {
-            index = c;
-            beam = c / p.vocab;
-            if (!(base[beam] > NEG_INF)) return (double)NEG_INF;
-            const int action = c - beam * p.vocab;
-            const uint8_t* allowed = rowMask(p, g, beam);
-            const float x = !allowed || allowed[action] ? toFloat(rowLogits<T>(p, g, beam)[action]) : NEG_INF;
-            return x > NEG_INF ? base[beam] + (double)x : (double)NEG_INF;
+            index = sh.found[c].index;
+            beam = sh.found[c].beam;
+            return sh.found[c].total;
         }
-        const u64 key = sh.found[c];
-        index = (unsigned)key;
-        beam = index / p.vocab;
-        return base[beam] + (double)fromOrdered((unsigned)(key >> 32));
-    };
-    // Few candidates are one warp's work, and the others are done; more are shared out
-    // and merged pairwise.
-    const int warps = n <= 128 * E ? 1 : ROW_WARPS, threads = warps * 32;
-    if (warp >= warps) return;
-    auto sync = [&]() {
-        if (warps == 1)
-            __syncwarp();
-        else
-            __syncthreads();
+        index = c;
+        beam = c / p.vocab;
+        const int action = c - beam * p.vocab;
+        if (p.finished && p.finished[row0 + beam])
+            return action == 0 ? (double)p.scores[row0 + beam] : (double)NEG_INF;
+        if (!(base[beam] > NEG_INF)) return (double)NEG_INF;
+        const uint8_t* allowed = rowMask(p, g, beam);
+        const float x = !allowed || allowed[action] ? toFloat(rowLogits<T>(p, g, beam)[action]) : NEG_INF;
+        return x > NEG_INF ? base[beam] + (double)x : (double)NEG_INF;
     };
     auto choose = [&]() {
         BestList<GroupKey, E> list;
         list.init(sh.wait[warp], p.width, lane);
-        for (int c0 = warp * 32; c0 < n; c0 += threads)
+        for (int c0 = warp * 32; c0 < n; c0 += THREADS)
         {
             int beam = 0;
             unsigned index = 0;
@@ -670,19 +837,12 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
             const GroupKey key{ ordered64(total), ~index };
             list.push(total > NEG_INF && better(key, list.bar), key);
         }
-        for (int k0 = warp * 32; p.finished && k0 < K; k0 += threads)
-        {
-            const int k = k0 + lane;
-            const double total = k < K && p.finished[row0 + k] ? (double)p.scores[row0 + k] : NEG_INF;
-            const GroupKey key{ ordered64(total), ~((unsigned)k * p.vocab) };
-            list.push(total > NEG_INF && better(key, list.bar), key);
-        }
         list.finish();
         __syncwarp();  // the buffer of waiting keys becomes the list
 #pragma unroll
         for (int e = 0; e < E; e++) sh.wait[warp][e * 32 + lane] = list.list[e];
         sync();
-        for (int m = warps / 2; m > 0; m /= 2)
+        for (int m = Shared::WARPS / 2; m > 0; m /= 2)
         {
             if (warp < m)
             {
@@ -696,17 +856,11 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
             sync();
         }
     };
+    clear();
     choose();
-
-    // Beams whose totals are too near one another's: neighbours in the list, and what
-    // lies around its last place.
     const GroupKey* list = sh.wait[0];
     const GroupKey last = list[p.width - 1];
-    auto mark = [&](int beam) {
-        atomicOr(&sh.near[beam >> 5], 1u << (beam & 31));
-        sh.repair = 1;
-    };
-    for (int i = tid; i + 1 < p.width; i += threads)
+    for (int i = tid; i + 1 < p.width; i += THREADS)
     {
         const GroupKey a = list[i], b = list[i + 1];
         if (!b.t || fromOrdered64(a.t) - fromOrdered64(b.t) > NEAR_TOTALS) continue;
@@ -715,60 +869,38 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
         mark(ka);
         mark(kb);
     }
-    if (last.t)
+    const double edge = last.t ? fromOrdered64(last.t) : (double)INFINITY;
+    const int kl = ~last.i / p.vocab;
+    for (int c = tid; c < n; c += THREADS)
     {
-        const double edge = fromOrdered64(last.t);
-        const int kl = ~last.i / p.vocab;
-        for (int c = tid; c < n; c += threads)
-        {
-            int beam = 0;
-            unsigned index = 0;
-            const double total = totalOf(c, beam, index);
-            if (beam == kl || !(fabs(total - edge) <= NEAR_TOTALS)) continue;
-            mark(beam);
-            mark(kl);
-        }
-        for (int k = tid; p.finished && k < K; k += threads)
-        {
-            if (!p.finished[row0 + k] || k == kl || !(fabs((double)p.scores[row0 + k] - edge) <= NEAR_TOTALS)) continue;
-            mark(kl);
-        }
+        int beam = 0;
+        unsigned index = 0;
+        const double total = totalOf(c, beam, index);
+        if (beam == kl || !(fabs(total - edge) <= NEAR_TOTALS)) continue;
+        mark(beam);
+        mark(kl);
     }
     sync();
     if (sh.repair)
     {
-        for (int k = 0; k < K; k++)
+        repair();
+        for (int c = tid; c < n && !every; c += THREADS)
         {
-            if (!(sh.near[k >> 5] >> (k & 31) & 1) || !readsLogits(p, row0 + k)) continue;  // the same for all threads
-            const T* x = rowLogits<T>(p, g, k);
-            const uint8_t* allowed = rowMask(p, g, k);
-            const double t = (double)topOf(k);
-            double sum = 0.0;
-            for (int a = tid; a < p.vocab; a += threads)
-                if (!allowed || allowed[a]) sum += exp((double)toFloat(x[a]) - t);
-#pragma unroll
-            for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
-            if (lane == 0) sh.red[warp] = sum;
-            sync();
-            if (tid == 0)
-            {
-                sum = 0.0;
-                for (int w = 0; w < warps; w++) sum += sh.red[w];
-                base[k] = (double)p.scores[row0 + k] - (t + log(sum));
-            }
-            sync();
+            const Candidate f = sh.found[c];
+            if (!marked(f.beam)) continue;
+            const int action = f.index - (unsigned)f.beam * p.vocab;
+            sh.found[c].total = base[f.beam] + (double)toFloat(rowLogits<T>(p, g, f.beam)[action]);
         }
+        sync();
         choose();
     }
-
-    for (int i = tid; i < p.width; i += threads)
+    for (int i = tid; i < p.width; i += THREADS)
     {
         const GroupKey key = list[i];
-        const unsigned index = ~key.i;
-        const long long o = g * p.width + i;
-        p.outScores[o] = key.t ? (float)fromOrdered64(key.t) : NEG_INF;
-        p.outParents[o] = key.t ? index / p.vocab : i % K;
-        p.outActions[o] = key.t ? index % p.vocab : 0;
+        if (key.t)
+            write(i, fromOrdered64(key.t), ~key.i);
+        else
+            writeNone(i);
     }
 }
 
@@ -777,7 +909,7 @@ template <class T, int E>
 __global__ void __launch_bounds__(ROW_THREADS) selectMergeKernel(BeamParams p)
 {
     __shared__ double baseS[BEAM_MAX_BEAMS];
-    __shared__ GroupShared<E> sh;
+    __shared__ GroupShared<ROW_THREADS, E> sh;
     const long long g = blockIdx.x, row0 = g * p.beams;
     const int segs = p.segs;
     const float* tops = p.top + row0 * segs;
@@ -792,54 +924,108 @@ __global__ void __launch_bounds__(ROW_THREADS) selectMergeKernel(BeamParams p)
     for (int k = threadIdx.x >> 5; k < p.beams; k += ROW_WARPS)
     {
         const int lane = threadIdx.x & 31;
-        double b = NEG_INF;
-        if (readsLogits(p, row0 + k))
+        const float score = p.scores[row0 + k];
+        const bool over = p.finished && p.finished[row0 + k];
+        float t = NEG_INF;
+        for (int s = lane; s < segs; s += 32) t = fmaxf(t, tops[k * segs + s]);
+        t = fromOrdered(__reduce_max_sync(FULL, ordered(t)));
+        double sum = 0.0;
+        for (int s = lane; s < segs; s += 32)
         {
-            float t = NEG_INF;
-            for (int s = lane; s < segs; s += 32) t = fmaxf(t, tops[k * segs + s]);
-            t = fromOrdered(__reduce_max_sync(FULL, ordered(t)));
-            double sum = 0.0;
-            for (int s = lane; s < segs; s += 32)
-            {
-                // A segment without a finite logit has sum 0, or NaN where one was NaN.
-                const float ts = tops[k * segs + s];
-                sum += ts > NEG_INF && ts < t ? sums[k * segs + s] * exp((double)ts - (double)t) : sums[k * segs + s];
-            }
-#pragma unroll
-            for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
-            if (t > NEG_INF) b = (double)p.scores[row0 + k] - ((double)t + log(sum));
+            // A segment without a finite logit has sum 0, or NaN where one was NaN.
+            const float ts = tops[k * segs + s];
+            const double part = sums[k * segs + s];
+            sum += ts > NEG_INF && ts < t ? part * exp((double)ts - (double)t) : part;
         }
-        if (lane == 0) baseS[k] = b;
+#pragma unroll
+        for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
+        // What was not read is not there.
+        if (lane == 0) baseS[k] = score > NEG_INF && !over && t > NEG_INF ? (double)score - ((double)t + log(sum)) : (double)NEG_INF;
     }
     __syncthreads();
-    finishGroup<T, E>(p, g, segs, [&](int c) { return chunks[c]; }, topOf, baseS, sh);
+    finishGroup<T, ROW_THREADS, E>(
+        p, g, threadIdx.x, [&](int c) { return chunks[c]; }, topOf,
+        [&](int k) { return p.finished[row0 + k] ? p.scores[row0 + k] : NEG_INF; }, baseS, sh);
 }
 
-// Short rows: a block per group for both.
-constexpr int GROUP_MAX_BEAMS = 64;
+// Short rows: groups in turn, some at a time.  The warps of a block read the rows of
+// its next groups while the last ones, a warp per group, finish the groups before.
+constexpr int GROUP_MAX_BEAMS = 32;
+constexpr int GROUP_MAX_WIDTH = 16;
+constexpr int GROUP_SCANNERS = 8;
+constexpr int GROUP_FINISHERS = 4;
+constexpr int GROUP_BLOCKS = 2;  // of an SM
+
+// What the scan of a group's rows leaves, in shared memory.
+struct GroupRows
+{
+    double *base, *sum;                 // [beams]
+    float *top, *score, *over, *chunk;  // [beams] (over: a finished beam's score), [beams, 32]
+
+    __host__ __device__ static int bytes(int beams) { return (beams * 156 + 15) / 16 * 16; }
+    __device__ GroupRows(char* m, int beams)
+        : base(reinterpret_cast<double*>(m)), sum(base + beams), top(reinterpret_cast<float*>(sum + beams)),
+          score(top + beams), over(score + beams), chunk(over + beams)
+    {
+    }
+};
 
 template <class T, bool MASKED>
-__global__ void __launch_bounds__(ROW_THREADS, 4) selectGroupKernel(BeamParams p)
+__global__ void __launch_bounds__((GROUP_SCANNERS + GROUP_FINISHERS) * 32, GROUP_BLOCKS)
+    selectGroupKernel(BeamParams p, int scanners, int together)
 {
-    __shared__ float chunkS[GROUP_MAX_BEAMS * 32], topS[GROUP_MAX_BEAMS];
-    __shared__ double baseS[GROUP_MAX_BEAMS];
-    __shared__ GroupShared<1> sh;
-    const int lane = threadIdx.x & 31;
-    const long long g = blockIdx.x;
-    for (int k = threadIdx.x >> 5; k < p.beams; k += ROW_WARPS)
+    extern __shared__ __align__(16) char groupMem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = p.beams, size = GroupRows::bytes(K);
+    // [2][together] rows' results, then the finishers' own.
+    GroupShared<32, 1>* shared = reinterpret_cast<GroupShared<32, 1>*>(groupMem + 2 * together * size);
+    const long long step = (long long)gridDim.x * together;
+    long long g0 = (long long)blockIdx.x * together;
+    for (int turn = 0; g0 - step < p.groups; g0 += step, turn ^= 1)
     {
-        double b = NEG_INF;
-        if (readsLogits(p, g * p.beams + k))
+        if (warp < scanners)
         {
-            const Scan scan = scanRow<T, MASKED>(Row<T>(p, g, k, lane), 0, 1);
-            if (scan.top > NEG_INF) b = (double)p.scores[g * p.beams + k] - ((double)scan.top + log(scan.sum));
-            chunkS[k * 32 + lane] = scan.laneTop;
-            topS[k] = scan.top;
+            for (int i = warp; i < together * K && g0 < p.groups; i += scanners)
+            {
+                const int q = i / K, k = i - q * K;
+                const long long g = g0 + q;
+                if (g >= p.groups) break;
+                GroupRows r(groupMem + (turn * together + q) * size, K);
+                const float score = p.scores[g * K + k];
+                const bool over = p.finished && p.finished[g * K + k];
+                Scan scan;
+                if (score > NEG_INF && !over)
+                {
+                    const Row<T> row(p, g, k, lane);
+                    scan = scanRow<T, MASKED, 8, false>(row, 0, row.vectors);
+                }
+                r.chunk[k * 32 + lane] = scan.laneTop;
+                if (lane == 0)
+                {
+                    r.top[k] = scan.top;
+                    r.sum[k] = scan.sum;
+                    r.score[k] = score;
+                    r.over[k] = over ? score : NEG_INF;
+                }
+            }
         }
-        baseS[k] = b;
+        else
+        {
+            const int q = warp - scanners;
+            const long long g = g0 - step + q;
+            if (g >= 0 && g < p.groups && g0 >= step)
+            {
+                GroupRows r(groupMem + ((turn ^ 1) * together + q) * size, K);
+                if (lane < K)
+                    r.base[lane] = r.top[lane] > NEG_INF ? (double)r.score[lane] - ((double)r.top[lane] + log(r.sum[lane]))
+                                                         : (double)NEG_INF;
+                __syncwarp();
+                finishGroup<T, 32, 1>(
+                    p, g, lane, [&](int c) { return r.chunk[c]; }, [&](int k) { return r.top[k]; },
+                    [&](int k) { return r.over[k]; }, r.base, shared[q]);
+            }
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    finishGroup<T, 1>(p, g, 1, [&](int c) { return chunkS[c]; }, [&](int k) { return topS[k]; }, baseS, sh);
 }
 
 // ---- selection over the action heads ---------------------------------------------------
@@ -1135,10 +1321,20 @@ void launchSelect(const BeamParams& p, cudaStream_t s)
 {
     if (p.segs == 0)
     {
+        // As many groups at a time as keep the finishers' latency behind the reading, fewer
+        // where blocks would stay without any.
+        const long long share = (p.groups + 148 * GROUP_BLOCKS - 1) / (148 * GROUP_BLOCKS);
+        const int size = 2 * GroupRows::bytes(p.beams) + (int)sizeof(GroupShared<32, 1>);
+        const int most = std::min(GROUP_FINISHERS, 48 * 1024 / size);
+        const int together = (int)std::max<long long>(1, std::min<long long>(most, share));
+        const int scanners = std::min(GROUP_SCANNERS, together * p.beams), threads = (scanners + together) * 32;
+        const size_t shared = (size_t)together * size;
+        const unsigned blocks = (unsigned)std::min<long long>((p.groups + together - 1) / together, 148 * GROUP_BLOCKS);
+        static_assert(2 * (GROUP_MAX_BEAMS * 156 + 16) + sizeof(GroupShared<32, 1>) < 48 * 1024, "one group fits");
         if (p.mask)
-            selectGroupKernel<T, true><<<p.groups, ROW_THREADS, 0, s>>>(p);
+            selectGroupKernel<T, true><<<blocks, threads, shared, s>>>(p, scanners, together);
         else
-            selectGroupKernel<T, false><<<p.groups, ROW_THREADS, 0, s>>>(p);
+            selectGroupKernel<T, false><<<blocks, threads, shared, s>>>(p, scanners, together);
         return;
     }
     const long long items = (long long)p.groups * p.beams * p.segs;
@@ -1185,7 +1381,7 @@ long long planBeamSelect(BeamParams& p, LogitType type, void* base)
     const int tiles = (int)(((long long)p.vocab * (type == LOGITS_F32 ? 4 : 2) + 2047) / 2048);  // of a warp's pass
     // Short rows are one block's work per group.
     const int turns = tiles * ((p.beams + ROW_WARPS - 1) / ROW_WARPS);
-    if (p.width <= 32 && p.beams <= GROUP_MAX_BEAMS && (turns <= 4 || (tiles <= 16 && p.groups >= 4 * 148)))
+    if (p.width <= GROUP_MAX_WIDTH && p.beams <= GROUP_MAX_BEAMS && (turns <= 4 || (tiles <= 16 && p.groups >= 4 * 148)))
     {
         p.segs = 0;
         return 0;
@@ -1193,6 +1389,8 @@ long long planBeamSelect(BeamParams& p, LogitType type, void* base)
     // Warps the card holds at a time, at the pass's register use.
     constexpr long long WARPS = 148 * 32;
     p.segs = (int)std::max<long long>(1, std::min<long long>(tiles, WARPS / std::max<long long>(1, rows)));
+    const int perVector = type == LOGITS_F32 ? 4 : 8, blocks = (p.vocab / perVector + 31) / 32;
+    p.segVectors = std::max(1, (blocks + p.segs - 1) / p.segs) * 32;
     const long long items = rows * p.segs;
     char* c = static_cast<char*>(base);
     p.sum = reinterpret_cast<double*>(c);

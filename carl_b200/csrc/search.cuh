@@ -30,6 +30,7 @@ struct BeamParams
     float* top;                         // [rows, segs] largest logit
     float* chunks;                      // [rows, segs, 32] largest logit of each lane's part
     int groups, beams, vocab, width;
+    int segVectors;                     // 16-byte vectors of a segment
     int segs;                           // warps to a row; 0: a block to a group
 };
 
