@@ -313,41 +313,49 @@ struct Row
         tail = p.vocab - head - vectors * VE;
         wideMask = (reinterpret_cast<uintptr_t>(allowed + head) & 3) == 0;
     }
-    // Vectors v0 + lane + 32 j below `end`; beyond it they are -inf.  A j with nothing below
-    // `end` for the whole warp is left out, here and by what follows.
+    // Vectors v0 + lane + 32 j below `end`; lanes beyond it read the last one, which
+    // `hideBeyond` takes out again.  A j with nothing below `end` for the whole warp is left
+    // out, here and by what follows.
     template <bool MASKED, int NV>
     __device__ __forceinline__ void load(int v0, int end, uint4 (&w)[NV], unsigned (&m)[NV * VE / 4]) const
     {
-        const uint4* v = reinterpret_cast<const uint4*>(x + head) + lane;
-        const uint8_t* a = allowed + head + lane * VE;
+        const uint4* v = reinterpret_cast<const uint4*>(x + head);
 #pragma unroll
         for (int j = 0; j < NV; j++)
         {
-            const int i = v0 + 32 * j;
-            if (i >= end) break;
-            if (i + lane < end)
-            {
-                w[j] = __ldcs(v + i);
-                if (MASKED)
-                {
+            if (v0 + 32 * j >= end) break;
+            w[j] = __ldcs(v + min(v0 + 32 * j + lane, end - 1));
+        }
+        if (!MASKED) return;
+        const uint8_t* a = allowed + head;
+        if (wideMask)
+        {
 #pragma unroll
-                    for (int q = 0; q < VE / 4; q++)
-                    {
-                        const uint8_t* b = a + (long long)i * VE + 4 * q;
-                        if (wideMask)
-                            m[j * VE / 4 + q] = __ldcs(reinterpret_cast<const unsigned*>(b));
-                        else
-                            m[j * VE / 4 + q] = b[0] | b[1] << 8 | b[2] << 16 | (unsigned)b[3] << 24;
-                    }
-                }
-            }
-            else
+            for (int j = 0; j < NV; j++)
             {
-                w[j] = make_uint4(Words<T>::NONE, Words<T>::NONE, Words<T>::NONE, Words<T>::NONE);
+                if (v0 + 32 * j >= end) break;
+                const unsigned* b = reinterpret_cast<const unsigned*>(a + (long long)min(v0 + 32 * j + lane, end - 1) * VE);
 #pragma unroll
-                for (int q = 0; MASKED && q < VE / 4; q++) m[j * VE / 4 + q] = 0;
+                for (int q = 0; q < VE / 4; q++) m[j * VE / 4 + q] = __ldcs(b + q);
             }
         }
+        else
+        {
+#pragma unroll
+            for (int j = 0; j < NV; j++)
+            {
+                if (v0 + 32 * j >= end) break;
+                const uint8_t* b = a + (long long)min(v0 + 32 * j + lane, end - 1) * VE;
+#pragma unroll
+                for (int q = 0; q < VE / 4; q++)
+                    m[j * VE / 4 + q] = b[4 * q] | b[4 * q + 1] << 8 | b[4 * q + 2] << 16 | (unsigned)b[4 * q + 3] << 24;
+            }
+        }
+    }
+    __device__ __forceinline__ void hideBeyond(int v0, int end, uint4& w) const
+    {
+        if (v0 + 32 > end && v0 + lane >= end)
+            w = make_uint4(Words<T>::NONE, Words<T>::NONE, Words<T>::NONE, Words<T>::NONE);
     }
     // What is not allowed becomes -inf.
     __device__ __forceinline__ static void hide(uint4& w, const unsigned* m)
@@ -442,6 +450,7 @@ __device__ __forceinline__ Scan scanRow(const Row<T>& row, int begin, int end)
         {
             if (v0 + 32 * j >= end) break;  // the same for the whole warp
             if (MASKED) Row<T>::hide(w[j], m + j * VE / 4);
+            row.hideBeyond(v0 + 32 * j, end, w[j]);
             most = Words<T>::larger(most, Words<T>::larger(Words<T>::larger(w[j].x, w[j].y), Words<T>::larger(w[j].z, w[j].w)));
         }
         scan.raise(largestOf<T>(most));
@@ -545,16 +554,24 @@ __device__ __forceinline__ void groupSync()
         __syncthreads();
 }
 
-// A value that at least n of the threads' `mine` reach, the n-th largest where it can be
-// told quickly (0: there are none).
+// A value that at least n of the threads' `mine` reach (0: there are none), nearly the
+// n-th largest.
 template <int THREADS, int E>
 __device__ __forceinline__ unsigned nthLargest(unsigned mine, int n, int tid, GroupShared<THREADS, E>& sh)
 {
     const int lane = tid & 31;
-    unsigned top = 0;
-    if (THREADS == 32 && n <= 12)
+    if (THREADS > 32 || n > 12)
     {
-        // The maximum is taken out n times.
+        sh.tops[tid] = mine;
+        if (tid == 0) sh.bar = 0xffffffffu;
+        groupSync<THREADS>();
+    }
+    if (n <= 12)
+    {
+        // Each warp, from the largest of 32 columns: the maximum is taken out n times.
+#pragma unroll
+        for (int w = 0; THREADS > 32 && w < THREADS / 32; w++) mine = max(mine, sh.tops[w * 32 + lane]);
+        unsigned top = 0;
         for (int left = n; left > 0;)
         {
             top = __reduce_max_sync(FULL, mine);
@@ -566,12 +583,9 @@ __device__ __forceinline__ unsigned nthLargest(unsigned mine, int n, int tid, Gr
         return top;
     }
     // The smallest of the values with fewer than n above them.
-    sh.tops[tid] = mine;
-    if (tid == 0) sh.bar = 0xffffffffu;
-    groupSync<THREADS>();
     int above = 0;
     const uint4* t = reinterpret_cast<const uint4*>(sh.tops);
-#pragma unroll 8
+#pragma unroll 4
     for (int i = 0; i < THREADS / 4; i++)
     {
         const uint4 v = t[i];
@@ -603,38 +617,59 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
     const int lane = tid & 31, warp = tid >> 5;
     const long long row0 = g * p.beams;
     const int segs = THREADS == 32 ? 1 : p.segs, segVectors = THREADS == 32 ? 1 << 30 : p.segVectors;  // a warp's rows are whole
-    const int K = p.beams, all = K * segs * 32;
+    const int K = p.beams, items = K * segs;
     const auto sync = [] { groupSync<THREADS>(); };
 
     if (tid == 0) sh.chunks = sh.candidates = sh.repair = 0;
-    // The totals of the chunks, some at a time so that their loads overlap.
-    constexpr int AT_ONCE = 8;
-    const auto chunkTotals = [&](int c0, float (&top)[AT_ONCE], double (&total)[AT_ONCE]) {
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; j++)
+    // The totals of a thread's chunks (beam k, segment s, its lane), some at a time so that
+    // their loads overlap: the best, its place, and the second best.
+    constexpr int AT_ONCE = 4;
+    const int stepBeams = Shared::WARPS / segs, stepSegs = Shared::WARPS - stepBeams * segs;
+    double best = NEG_INF, second = NEG_INF;
+    int bestAt = 0;
+    const auto eachChunk = [&](auto use) {
+        int k = warp / segs, seg = warp - k * segs;
+        for (int i0 = warp; i0 < items; i0 += AT_ONCE * Shared::WARPS)
         {
-            const int c = c0 + j * THREADS;
-            top[j] = c < all ? chunkTop(c) : NEG_INF;
-        }
+            float top[AT_ONCE];
+            int beam[AT_ONCE];
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; j++)
-        {
-            const int c = c0 + j * THREADS;
-            const double b = c < all ? base[(c >> 5) / segs] : (double)NEG_INF;
-            total[j] = b > NEG_INF && top[j] > NEG_INF ? b + (double)top[j] : (double)NEG_INF;
+            for (int j = 0; j < AT_ONCE; j++)
+            {
+                const int i = i0 + j * Shared::WARPS;
+                top[j] = i < items ? chunkTop(i * 32 + lane) : NEG_INF;
+                beam[j] = k;
+                k += stepBeams;
+                seg += stepSegs;
+                if (seg >= segs)
+                {
+                    seg -= segs;
+                    k++;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; j++)
+            {
+                const int i = i0 + j * Shared::WARPS;
+                if (i >= items) break;
+                const double b = base[beam[j]];
+                // A beam that was not read has left nothing here.
+                use(b > NEG_INF ? b + (double)top[j] : (double)NEG_INF, i * 32 + lane);
+            }
         }
     };
-    float best = NEG_INF;
-    for (int c0 = tid; c0 < all; c0 += AT_ONCE * THREADS)
-    {
-        float top[AT_ONCE];
-        double total[AT_ONCE];
-        chunkTotals(c0, top, total);
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; j++) best = fmaxf(best, (float)total[j]);
-    }
-    sync();
-    const unsigned nth = nthLargest<THREADS, E>(best > NEG_INF ? ordered(best) : 0u, p.width, tid, sh);
+    eachChunk([&](double total, int c) {
+        const bool lead = total > best;
+        const double less = lead ? best : total;
+        if (less > second) second = less;
+        if (lead)
+        {
+            best = total;
+            bestAt = c;
+        }
+    });
+    if (THREADS > 32) sync();
+    const unsigned nth = nthLargest<THREADS, E>(best > NEG_INF ? ordered((float)best) : 0u, p.width, tid, sh);
     // Lower by twice NEAR_TOTALS and by eight roundings to float32.
     float bar = nth && nth != 0xffffffffu ? fromOrdered(nth) : NEG_INF;
     bar = fabsf(bar) < FLT_MAX ? bar - (2.f * (float)NEAR_TOTALS + 8.f * 0x1p-24f * fabsf(bar)) : NEG_INF;
@@ -644,31 +679,26 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
         const int at = atomicAdd(&sh.candidates, 1);
         if (at < Shared::CANDIDATES) sh.found[at] = Candidate{ total, index, k };
     };
-    for (int c0 = tid; c0 < all; c0 += AT_ONCE * THREADS)
-    {
-        float top[AT_ONCE];
-        double total[AT_ONCE];
-        chunkTotals(c0, top, total);
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; j++)
-        {
-            if (!(total[j] > NEG_INF && total[j] >= (double)bar)) continue;
-            const int at = atomicAdd(&sh.chunks, 1);
-            if (at < Shared::CHUNKS) sh.chunk[at] = c0 + j * THREADS;
-        }
-    }
+    const auto readAgain = [&](double total, int c) {
+        if (!(total > NEG_INF && total >= (double)bar)) return;
+        const int at = atomicAdd(&sh.chunks, 1);
+        if (at < Shared::CHUNKS) sh.chunk[at] = c;
+    };
+    if (second > NEG_INF && second >= (double)bar)
+        eachChunk(readAgain);
+    else
+        readAgain(best, bestAt);
     for (int k = tid; p.finished && k < K; k += THREADS) offer((double)overOf(k), (unsigned)k * p.vocab, k);
     sync();
     // The vectors of all these chunks, shared out over the threads.
     const int chunks = sh.chunks;
     const int per = (min(segVectors, p.vocab / VE) + 31) / 32 + 1;  // vectors of a chunk, and its edge
-    constexpr int VECTORS = 4;
+    constexpr int VECTORS = THREADS == 32 ? 3 : 2;
     for (int i0 = tid; chunks <= Shared::CHUNKS && i0 < chunks * per; i0 += VECTORS * THREADS)
     {
         uint4 r[VECTORS];
         unsigned legal[VECTORS];
         int action[VECTORS], beam[VECTORS];
-        double b[VECTORS];
 #pragma unroll
         for (int u = 0; u < VECTORS; u++)
         {
@@ -679,12 +709,11 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
             const Row<T> row(p, g, k, c & 31);
             const int begin = THREADS == 32 ? 0 : seg * segVectors, at = begin + row.lane + 32 * v;
             beam[u] = k;
-            b[u] = base[k];
             if (v == per - 1)
             {
                 float x;
                 action[u] = begin == 0 ? row.edge(x) : -1;
-                if (action[u] >= 0) offer(b[u] + (double)x, (unsigned)k * p.vocab + action[u], k);
+                if (action[u] >= 0) offer(base[k] + (double)x, (unsigned)k * p.vocab + action[u], k);
             }
             else if (at < row.vectors && at - begin < segVectors)
             {
@@ -702,13 +731,22 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
 #pragma unroll
         for (int u = 0; u < VECTORS; u++)
         {
+            if (!legal[u]) continue;
+            const double b = base[beam[u]];
+            // Logits that can reach the bar, then those that do.
+            float need = (float)((double)bar - b);
+            need = need > -FLT_MAX ? need - 2.f * 0x1p-24f * fabsf(need) : -FLT_MAX;
             const unsigned words[4] = { r[u].x, r[u].y, r[u].z, r[u].w };
+            unsigned hits = 0;
 #pragma unroll
             for (int q = 0; q < VE; q++)
+                if (Words<T>::at(words[q / Words<T>::PER], q % Words<T>::PER) >= need) hits |= 1u << q;
+            for (hits &= legal[u]; hits; hits &= hits - 1)
             {
-                if (!(legal[u] >> q & 1)) continue;
-                const double total = b[u] + (double)Words<T>::at(words[q / Words<T>::PER], q % Words<T>::PER);
-                if (total >= (double)bar) offer(total, (unsigned)beam[u] * p.vocab + action[u] + q, beam[u]);
+                const int q = __ffs(hits) - 1, w = q / Words<T>::PER;
+                const unsigned word = w == 0 ? words[0] : w == 1 ? words[1] : w == 2 ? words[2] : words[3];
+                const float x = q % Words<T>::PER ? Words<T>::at(word, 1) : Words<T>::at(word, 0);
+                offer(b + (double)x, (unsigned)beam[u] * p.vocab + action[u] + q, beam[u]);
             }
         }
     }
@@ -735,8 +773,21 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
             const uint8_t* allowed = rowMask(p, g, k);
             const double t = (double)topOf(k);
             double sum = 0.0;
-            for (int a = tid; a < p.vocab; a += THREADS)
-                if (!allowed || allowed[a]) sum += exp((double)toFloat(x[a]) - t);
+            constexpr int AHEAD = 8;  // independent exponentials hide each other's latency
+            for (int a0 = tid; a0 < p.vocab; a0 += AHEAD * THREADS)
+            {
+                double v[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++)
+                {
+                    const int a = a0 + u * THREADS;
+                    v[u] = a < p.vocab && (!allowed || allowed[a]) ? (double)toFloat(x[a]) : (double)NEG_INF;
+                }
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++) v[u] = exp(v[u] - t);
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++) sum += v[u];
+            }
 #pragma unroll
             for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
             if (lane == 0) sh.red[warp] = sum;
@@ -750,9 +801,8 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
             sync();
         }
     };
-    const auto write = [&](int place, double total, unsigned index) {
+    const auto write = [&](int place, double total, unsigned index, int beam) {
         const long long o = g * p.width + place;
-        const int beam = index / p.vocab;
         p.outScores[o] = (float)total;
         p.outParents[o] = beam;
         p.outActions[o] = index - (unsigned)beam * p.vocab;
@@ -803,7 +853,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
                 place += c.total > mine.total || (c.total == mine.total && c.index < mine.index);
             }
         }
-        if (tid < n && place < p.width) write(place, mine.total, mine.index);
+        if (tid < n && place < p.width) write(place, mine.total, mine.index, mine.beam);
         for (int i = n + tid; i < p.width; i += THREADS) writeNone(i);
         return;
     }
@@ -898,7 +948,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
     {
         const GroupKey key = list[i];
         if (key.t)
-            write(i, fromOrdered64(key.t), ~key.i);
+            write(i, fromOrdered64(key.t), ~key.i, ~key.i / p.vocab);
         else
             writeNone(i);
     }
@@ -948,13 +998,11 @@ __global__ void __launch_bounds__(ROW_THREADS) selectMergeKernel(BeamParams p)
         [&](int k) { return p.finished[row0 + k] ? p.scores[row0 + k] : NEG_INF; }, baseS, sh);
 }
 
-// Short rows: groups in turn, some at a time.  The warps of a block read the rows of
-// its next groups while the last ones, a warp per group, finish the groups before.
+// Short rows need no workspace: what the scan of a group's rows leaves stays in shared
+// memory.
 constexpr int GROUP_MAX_BEAMS = 32;
 constexpr int GROUP_MAX_WIDTH = 16;
-constexpr int GROUP_SCANNERS = 8;
-constexpr int GROUP_FINISHERS = 4;
-constexpr int GROUP_BLOCKS = 2;  // of an SM
+constexpr int GROUP_WARPS = 8;   // warps of a group's block
 
 // What the scan of a group's rows leaves, in shared memory.
 struct GroupRows
@@ -970,62 +1018,54 @@ struct GroupRows
     }
 };
 
+// The rows of a group from beam k0 on, every `step`-th.
 template <class T, bool MASKED>
-__global__ void __launch_bounds__((GROUP_SCANNERS + GROUP_FINISHERS) * 32, GROUP_BLOCKS)
-    selectGroupKernel(BeamParams p, int scanners, int together)
+__device__ __forceinline__ void scanGroup(const BeamParams& p, long long g, int k0, int step, int lane, GroupRows& r)
+{
+    for (int k = k0; k < p.beams; k += step)
+    {
+        const float score = p.scores[g * p.beams + k];
+        const bool over = p.finished && p.finished[g * p.beams + k];
+        Scan scan;
+        if (score > NEG_INF && !over)
+        {
+            const Row<T> row(p, g, k, lane);
+            scan = scanRow<T, MASKED, 8, false>(row, 0, row.vectors);
+        }
+        r.chunk[k * 32 + lane] = scan.laneTop;
+        if (lane == 0)
+        {
+            r.top[k] = scan.top;
+            r.sum[k] = scan.sum;
+            r.score[k] = score;
+            r.over[k] = over ? score : NEG_INF;
+        }
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void finishRows(const BeamParams& p, long long g, int lane, GroupRows& r, GroupShared<32, 1>& sh)
+{
+    if (lane < p.beams)
+        r.base[lane] = r.top[lane] > NEG_INF ? (double)r.score[lane] - ((double)r.top[lane] + log(r.sum[lane]))
+                                             : (double)NEG_INF;
+    __syncwarp();
+    finishGroup<T, 32, 1>(
+        p, g, lane, [&](int c) { return r.chunk[c]; }, [&](int k) { return r.top[k]; }, [&](int k) { return r.over[k]; },
+        r.base, sh);
+}
+
+// A block reads a group's rows, its first warp finishes.
+template <class T, bool MASKED>
+__global__ void __launch_bounds__(GROUP_WARPS * 32, 3) selectGroupKernel(BeamParams p)
 {
     extern __shared__ __align__(16) char groupMem[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = p.beams, size = GroupRows::bytes(K);
-    // [2][together] rows' results, then the finishers' own.
-    GroupShared<32, 1>* shared = reinterpret_cast<GroupShared<32, 1>*>(groupMem + 2 * together * size);
-    const long long step = (long long)gridDim.x * together;
-    long long g0 = (long long)blockIdx.x * together;
-    for (int turn = 0; g0 - step < p.groups; g0 += step, turn ^= 1)
-    {
-        if (warp < scanners)
-        {
-            for (int i = warp; i < together * K && g0 < p.groups; i += scanners)
-            {
-                const int q = i / K, k = i - q * K;
-                const long long g = g0 + q;
-                if (g >= p.groups) break;
-                GroupRows r(groupMem + (turn * together + q) * size, K);
-                const float score = p.scores[g * K + k];
-                const bool over = p.finished && p.finished[g * K + k];
-                Scan scan;
-                if (score > NEG_INF && !over)
-                {
-                    const Row<T> row(p, g, k, lane);
-                    scan = scanRow<T, MASKED, 8, false>(row, 0, row.vectors);
-                }
-                r.chunk[k * 32 + lane] = scan.laneTop;
-                if (lane == 0)
-                {
-                    r.top[k] = scan.top;
-                    r.sum[k] = scan.sum;
-                    r.score[k] = score;
-                    r.over[k] = over ? score : NEG_INF;
-                }
-            }
-        }
-        else
-        {
-            const int q = warp - scanners;
-            const long long g = g0 - step + q;
-            if (g >= 0 && g < p.groups && g0 >= step)
-            {
-                GroupRows r(groupMem + ((turn ^ 1) * together + q) * size, K);
-                if (lane < K)
-                    r.base[lane] = r.top[lane] > NEG_INF ? (double)r.score[lane] - ((double)r.top[lane] + log(r.sum[lane]))
-                                                         : (double)NEG_INF;
-                __syncwarp();
-                finishGroup<T, 32, 1>(
-                    p, g, lane, [&](int c) { return r.chunk[c]; }, [&](int k) { return r.top[k]; },
-                    [&](int k) { return r.over[k]; }, r.base, shared[q]);
-            }
-        }
-        __syncthreads();
-    }
+    __shared__ GroupShared<32, 1> sh;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    GroupRows r(groupMem, p.beams);
+    scanGroup<T, MASKED>(p, blockIdx.x, warp, blockDim.x >> 5, lane, r);
+    __syncthreads();
+    if (warp == 0) finishRows<T>(p, blockIdx.x, lane, r, sh);
 }
 
 // ---- selection over the action heads ---------------------------------------------------
@@ -1321,20 +1361,17 @@ void launchSelect(const BeamParams& p, cudaStream_t s)
 {
     if (p.segs == 0)
     {
-        // As many groups at a time as keep the finishers' latency behind the reading, fewer
-        // where blocks would stay without any.
-        const long long share = (p.groups + 148 * GROUP_BLOCKS - 1) / (148 * GROUP_BLOCKS);
-        const int size = 2 * GroupRows::bytes(p.beams) + (int)sizeof(GroupShared<32, 1>);
-        const int most = std::min(GROUP_FINISHERS, 48 * 1024 / size);
-        const int together = (int)std::max<long long>(1, std::min<long long>(most, share));
-        const int scanners = std::min(GROUP_SCANNERS, together * p.beams), threads = (scanners + together) * 32;
-        const size_t shared = (size_t)together * size;
-        const unsigned blocks = (unsigned)std::min<long long>((p.groups + together - 1) / together, 148 * GROUP_BLOCKS);
-        static_assert(2 * (GROUP_MAX_BEAMS * 156 + 16) + sizeof(GroupShared<32, 1>) < 48 * 1024, "one group fits");
+        const int bytes = GroupRows::bytes(p.beams);
+        // About 16 warps to an SM: fewer warps to a group waste less in its serial part, more
+        // shorten a lone group (8 beams over 648 with a mask, us with 1 / 2 / 4 / 8 warps: 148
+        // groups 16 / 11 / 8.6 / 7.5; 1184: 20 / 15 / 19 / 21; 16384: 123 / 144 / 145 / 207).
+        int warps = GROUP_WARPS;
+        while (warps > 1 && (long long)p.groups * warps > 148 * 24) warps /= 2;
+        const int threads = std::min(warps, p.beams) * 32;
         if (p.mask)
-            selectGroupKernel<T, true><<<blocks, threads, shared, s>>>(p, scanners, together);
+            selectGroupKernel<T, true><<<p.groups, threads, bytes, s>>>(p);
         else
-            selectGroupKernel<T, false><<<blocks, threads, shared, s>>>(p, scanners, together);
+            selectGroupKernel<T, false><<<p.groups, threads, bytes, s>>>(p);
         return;
     }
     const long long items = (long long)p.groups * p.beams * p.segs;
@@ -1388,7 +1425,7 @@ long long planBeamSelect(BeamParams& p, LogitType type, void* base)
     }
     // Warps the card holds at a time, at the pass's register use.
     constexpr long long WARPS = 148 * 32;
-    p.segs = (int)std::max<long long>(1, std::min<long long>(tiles, WARPS / std::max<long long>(1, rows)));
+    p.segs = (int)std::max<long long>(1, std::min<long long>((tiles + 3) / 4, WARPS / std::max<long long>(1, rows)));
     const int perVector = type == LOGITS_F32 ? 4 : 8, blocks = (p.vocab / perVector + 31) / 32;
     p.segVectors = std::max(1, (blocks + p.segs - 1) / p.segs) * 32;
     const long long items = rows * p.segs;
