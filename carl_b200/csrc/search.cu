@@ -1080,7 +1080,15 @@ struct JointKey
     int i;     // action, then beam * JOINT_ACTIONS + action
 };
 
-__device__ __forceinline__ bool ahead(const JointKey& a, const JointKey& b) { return a.v > b.v || (a.v == b.v && a.i < b.i); }
+// Without branches, as the exchanges below.
+__device__ __forceinline__ bool ahead(const JointKey& a, const JointKey& b)
+{
+    return (bool)((a.v > b.v) | ((a.v == b.v) & (a.i < b.i)));
+}
+__device__ __forceinline__ JointKey pick(bool first, const JointKey& a, const JointKey& b)
+{
+    return JointKey{ first ? a.v : b.v, first ? a.i : b.i };
+}
 
 // Sorts a bitonic list, best first.
 template <int N>
@@ -1094,8 +1102,8 @@ __device__ __forceinline__ void settle(JointKey (&l)[N])
             if (i & s) continue;
             const JointKey a = l[i], b = l[i | s];
             const bool swap = ahead(b, a);
-            l[i] = swap ? b : a;
-            l[i | s] = swap ? a : b;
+            l[i] = pick(swap, b, a);
+            l[i | s] = pick(swap, a, b);
         }
 }
 
@@ -1172,8 +1180,8 @@ __global__ void __launch_bounds__(JOINT_THREADS) jointSelectKernel(BeamParams p,
             auto order = [&](int a, int b) {
                 const JointKey l = option[a], r = option[b];
                 const bool swap = ahead(r, l);
-                option[a] = swap ? r : l;
-                option[b] = swap ? l : r;
+                option[a] = pick(swap, r, l);
+                option[b] = pick(swap, l, r);
             };
             order(0, 1);
             order(1, 2);
@@ -1193,7 +1201,7 @@ __global__ void __launch_bounds__(JOINT_THREADS) jointSelectKernel(BeamParams p,
                 for (int i = 0; i < N / (r + 1); i++)
                 {
                     const JointKey c{ before[i].v + option[r].v, before[i].i * size + option[r].i };
-                    if (ahead(c, best[N - 1 - i])) best[N - 1 - i] = c;
+                    best[N - 1 - i] = pick(ahead(c, best[N - 1 - i]), c, best[N - 1 - i]);
                 }
                 settle(best);
             }
@@ -1223,14 +1231,14 @@ __global__ void __launch_bounds__(JOINT_THREADS) jointSelectKernel(BeamParams p,
             for (int i = 0; i < N; i++)
             {
                 const bool take = ahead(other[i], best[i]);
-                const JointKey drop = take ? best[i] : other[i];
-                if (take) best[i] = other[i];
-                if (drop.v > lost.v) lost = drop;
+                const JointKey drop = pick(take, best[i], other[i]);
+                best[i] = pick(take, other[i], best[i]);
+                lost = pick(drop.v > lost.v, drop, lost);
             }
             settle(best);
             const JointKey theirs{ __shfl_xor_sync(FULL, out.v, m), __shfl_xor_sync(FULL, out.i, m) };
-            if (theirs.v > out.v) out = theirs;
-            if (lost.v > out.v) out = lost;
+            out = pick(theirs.v > out.v, theirs, out);
+            out = pick(lost.v > out.v, lost, out);
         }
         if (pass == 1) break;
         bool near = false;
