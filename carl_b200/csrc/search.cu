@@ -1274,6 +1274,12 @@ __global__ void __launch_bounds__(JOINT_THREADS) jointSelectKernel(BeamParams p,
 }
 
 // ---- state reordering --------------------------------------------------------------------
+//
+// Every byte of a moved row is read and written once; the kernels differ in how a block
+// finds them.  Rows of whole 16-byte columns go through registers (reorderRowsKernel);
+// short rows, as the simulator's words of a few cars, through shared memory as one dense
+// run of whole groups (reorderRunsKernel); anything else, and what is too small for more
+// than one launch to pay, in the row's largest unit (reorderTilesKernel).
 
 constexpr int REORDER_ARRAYS = 24;        // arrays of one launch
 constexpr int REORDER_TILE = 32 * 1024;   // bytes of shared memory of a tile
@@ -1282,10 +1288,10 @@ constexpr int REORDER_THREADS = 256;
 struct ReorderArray
 {
     char* data;
-    long long outerStride, inner;    // bytes
+    long long outer, outerStride, inner;  // slabs; bytes
     long long firstBlock;
-    int groupsPerTile, groupTiles;   // whole groups of a tile, tiles along the groups
-    int units, unitTiles;            // units (of `unit` bytes) of a tile's rows, tiles along a row
+    int groupsPerTile, groupTiles;        // whole groups of a tile, tiles along the groups
+    int units, unitTiles;                 // units (of `unit` bytes) of a tile's rows, tiles along a row
     int unit;
 };
 
@@ -1295,6 +1301,20 @@ struct ReorderParams
     const long long* parents;
     int count, groups, beams;
 };
+
+// The slot's parent; an index outside the group leaves the slot.
+__device__ __forceinline__ int parentOf(const ReorderParams& p, long long row, int slot)
+{
+    const long long q = p.parents[row];
+    return q >= 0 && q < p.beams ? (int)q : slot;
+}
+
+__device__ __forceinline__ const ReorderArray& arrayOf(const ReorderParams& p)
+{
+    int k = 0;
+    while (k + 1 < p.count && (long long)blockIdx.x >= p.a[k + 1].firstBlock) k++;
+    return p.a[k];
+}
 
 // A tile is whole groups by a range of columns: the rows that some slot takes are
 // read into shared memory, then the slots that change are written.
@@ -1313,9 +1333,7 @@ __device__ void reorderTile(const ReorderParams& p, const ReorderArray& a, char*
     __syncthreads();
     for (int r = tid; r < rows; r += REORDER_THREADS)
     {
-        const int j = r % K;
-        const long long q = p.parents[(long long)g0 * K + r];
-        const int parent = q >= 0 && q < K ? (int)q : j;  // an index outside the group leaves the slot
+        const int j = r % K, parent = parentOf(p, (long long)g0 * K + r, j);
         parentS[r] = (short)(r - j + parent);
         if (parent != j) takenS[r - j + parent] = 1;
     }
@@ -1335,14 +1353,12 @@ __device__ void reorderTile(const ReorderParams& p, const ReorderArray& a, char*
     }
 }
 
-__global__ void __launch_bounds__(REORDER_THREADS) reorderKernel(ReorderParams p)
+__global__ void __launch_bounds__(REORDER_THREADS) reorderTilesKernel(ReorderParams p)
 {
     __shared__ __align__(16) char tile[REORDER_TILE];
     __shared__ short parentS[BEAM_MAX_BEAMS];
     __shared__ uint8_t takenS[BEAM_MAX_BEAMS];
-    int k = 0;
-    while (k + 1 < p.count && (long long)blockIdx.x >= p.a[k + 1].firstBlock) k++;
-    const ReorderArray a = p.a[k];
+    const ReorderArray a = arrayOf(p);
     switch (a.unit)
     {
     case 16: reorderTile<uint4>(p, a, tile, parentS, takenS); break;
@@ -1350,6 +1366,119 @@ __global__ void __launch_bounds__(REORDER_THREADS) reorderKernel(ReorderParams p
     case 4: reorderTile<unsigned>(p, a, tile, parentS, takenS); break;
     case 2: reorderTile<unsigned short>(p, a, tile, parentS, takenS); break;
     default: reorderTile<uint8_t>(p, a, tile, parentS, takenS); break;
+    }
+}
+
+// Short rows of whole words: a tile is a dense run of whole groups, read and written in
+// 16-byte vectors, permuted by words in shared memory.  The words' places are worked out
+// once and used for several slabs; the next slab is loaded while this one is permuted.
+constexpr int RUN_VECTORS = 2;                                         // of a thread
+constexpr int RUN_WORDS = REORDER_THREADS * RUN_VECTORS * 4;           // of a tile
+constexpr int RUN_SLABS = 8;                                           // of a block
+
+__global__ void __launch_bounds__(REORDER_THREADS) reorderRunsKernel(ReorderParams p)
+{
+    __shared__ __align__(16) unsigned tile[2][RUN_WORDS];
+    short* parentS = reinterpret_cast<short*>(tile[1]);  // until the first slab is permuted
+    const ReorderArray a = arrayOf(p);
+    const int tid = threadIdx.x, K = p.beams, W = (int)(a.inner / 4);
+    const long long b = blockIdx.x - a.firstBlock;
+    const int gt = (int)(b % a.groupTiles);
+    const long long s0 = b / a.groupTiles * RUN_SLABS, s1 = min(a.outer, s0 + RUN_SLABS);
+    const int g0 = gt * a.groupsPerTile, ng = min(a.groupsPerTile, p.groups - g0), rows = ng * K, words = rows * W;
+    char* data = a.data + (long long)g0 * K * a.inner;
+
+    uint4 next[RUN_VECTORS];
+    const auto load = [&](long long s) {
+        const uint4* from = reinterpret_cast<const uint4*>(data + s * a.outerStride);
+#pragma unroll
+        for (int u = 0; u < RUN_VECTORS; u++)
+            if ((tid + u * REORDER_THREADS) * 4 + 3 < words) next[u] = from[tid + u * REORDER_THREADS];
+    };
+    load(s0);
+    for (int r = tid; r < rows; r += REORDER_THREADS)
+    {
+        const int j = r % K;
+        parentS[r] = (short)(r - j + parentOf(p, (long long)g0 * K + r, j));
+    }
+    __syncthreads();
+    short source[RUN_VECTORS][4];
+    bool moves[RUN_VECTORS];
+#pragma unroll
+    for (int u = 0; u < RUN_VECTORS; u++)
+    {
+        moves[u] = false;
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+        {
+            const int w = (tid + u * REORDER_THREADS) * 4 + q, r = w / W;
+            source[u][q] = (short)(w < words ? parentS[r] * W + (w - r * W) : 0);
+            moves[u] |= w < words && source[u][q] != w;
+        }
+    }
+    // The words behind the last whole vector, fewer than four.
+    const int tail = words & ~3, tw = tail + tid;
+    const bool hasTail = tw < words;
+    const int tailSource = hasTail ? parentS[tw / W] * W + tw % W : 0;
+    for (long long s = s0, turn = 0; s < s1; s++, turn ^= 1)
+    {
+        unsigned* t = tile[turn];
+        unsigned* slab = reinterpret_cast<unsigned*>(data + s * a.outerStride);
+#pragma unroll
+        for (int u = 0; u < RUN_VECTORS; u++)
+            if ((tid + u * REORDER_THREADS) * 4 + 3 < words) reinterpret_cast<uint4*>(t)[tid + u * REORDER_THREADS] = next[u];
+        if (hasTail) t[tw] = slab[tw];
+        __syncthreads();
+        if (s + 1 < s1) load(s + 1);
+#pragma unroll
+        for (int u = 0; u < RUN_VECTORS; u++)
+        {
+            const int v = tid + u * REORDER_THREADS;
+            if (!moves[u] || v * 4 + 3 >= words) continue;
+            reinterpret_cast<uint4*>(slab)[v] = make_uint4(t[source[u][0]], t[source[u][1]], t[source[u][2]], t[source[u][3]]);
+        }
+        if (hasTail) slab[tw] = t[tailSource];
+    }
+}
+
+// Rows of whole 16-byte columns: a thread holds its column of a group's rows.
+constexpr int COLUMN_BEAMS = 16;
+constexpr int COLUMN_THREADS = 128;
+
+template <int BEAMS>
+__global__ void __launch_bounds__(COLUMN_THREADS) reorderRowsKernel(ReorderParams p)
+{
+    __shared__ int parentS[BEAMS];
+    __shared__ unsigned takenS;
+    const ReorderArray a = arrayOf(p);
+    const int tid = threadIdx.x, K = p.beams;
+    const long long b = blockIdx.x - a.firstBlock, og = b / a.unitTiles, outer = og / p.groups, g = og - outer * p.groups;
+    const int ut = (int)(b - og * a.unitTiles), columns = (int)(a.inner / 16);
+    if (tid == 0) takenS = 0;
+    __syncthreads();
+    if (tid < K)
+    {
+        const int parent = parentOf(p, g * K + tid, tid);
+        parentS[tid] = parent;
+        if (parent != tid) atomicOr(&takenS, 1u << parent);
+    }
+    __syncthreads();
+    const unsigned taken = takenS;
+    if (!taken) return;
+    uint4* data = reinterpret_cast<uint4*>(a.data + outer * a.outerStride + g * K * a.inner);
+    for (int c = ut * a.units + tid; c < min(columns, (ut + 1) * a.units); c += COLUMN_THREADS)
+    {
+        uint4 held[BEAMS];
+#pragma unroll
+        for (int k = 0; k < BEAMS; k++)
+            if (taken >> k & 1) held[k] = data[(long long)k * columns + c];
+#pragma unroll
+        for (int k = 0; k < BEAMS; k++)
+        {
+            if (!(taken >> k & 1)) continue;
+            for (int j = 0; j < K; j++)  // the same for the whole block
+                if (parentS[j] == k && j != k) data[(long long)j * columns + c] = held[k];
+        }
     }
 }
 
@@ -1466,23 +1595,60 @@ void launchJointSelect(const BeamParams& p, LogitType type, cudaStream_t s)
 
 void launchReorder(const StateArray* arrays, int count, const long long* parents, int groups, int beams, cudaStream_t s)
 {
-    for (int first = 0; first < count; first += REORDER_ARRAYS)
-    {
-        ReorderParams p{};
-        p.parents = parents;
-        p.groups = groups;
-        p.beams = beams;
-        long long blocks = 0;
-        for (int k = first; k < count && k < first + REORDER_ARRAYS; k++)
+    enum Form { TILES, RUNS, ROWS, FORMS };
+    ReorderParams p[FORMS] = {};
+    long long blocks[FORMS] = {};
+    const auto flush = [&](int f) {
+        if (blocks[f] > 0)
         {
-            const StateArray& in = arrays[k];
-            if (in.inner == 0 || in.outer == 0) continue;
-            ReorderArray& a = p.a[p.count++];
-            a.data = static_cast<char*>(in.data);
-            a.outerStride = in.outerStride;
-            a.inner = in.inner;
-            const unsigned long long bits = reinterpret_cast<uintptr_t>(in.data) | (unsigned long long)in.inner
-                                            | (in.outer > 1 ? (unsigned long long)in.outerStride : 0);
+            const unsigned n = (unsigned)blocks[f];
+            if (f == TILES)
+                reorderTilesKernel<<<n, REORDER_THREADS, 0, s>>>(p[f]);
+            else if (f == RUNS)
+                reorderRunsKernel<<<n, REORDER_THREADS, 0, s>>>(p[f]);
+            else if (beams <= 8)
+                reorderRowsKernel<8><<<n, COLUMN_THREADS, 0, s>>>(p[f]);
+            else
+                reorderRowsKernel<COLUMN_BEAMS><<<n, COLUMN_THREADS, 0, s>>>(p[f]);
+        }
+        p[f].count = 0;
+        blocks[f] = 0;
+    };
+    const long long rows = (long long)groups * beams;
+    long long bytes = 0;
+    for (int k = 0; k < count; k++) bytes += rows * arrays[k].outer * arrays[k].inner;
+    // Below this a second launch costs more than the better form saves.
+    const bool small = bytes < (1 << 20);
+    for (int k = 0; k < count; k++)
+    {
+        const StateArray& in = arrays[k];
+        if (in.inner == 0 || in.outer == 0) continue;
+        ReorderArray a{};
+        a.data = static_cast<char*>(in.data);
+        a.outer = in.outer;
+        a.outerStride = in.outerStride;
+        a.inner = in.inner;
+        const unsigned long long base = reinterpret_cast<uintptr_t>(in.data) | (in.outer > 1 ? (unsigned long long)in.outerStride : 0);
+        const unsigned long long bits = base | (unsigned long long)in.inner;
+        int form = TILES;
+        long long n = 0;
+        if (!small && bits % 16 == 0 && in.inner >= 256 && beams <= COLUMN_BEAMS)
+        {
+            form = ROWS;
+            a.units = 4 * COLUMN_THREADS;
+            a.unitTiles = (int)((in.inner / 16 + a.units - 1) / a.units);
+            n = in.outer * groups * a.unitTiles;
+        }
+        else if (!small && base % 16 == 0 && in.inner % 4 == 0 && in.inner / 4 * beams <= RUN_WORDS / 4)
+        {
+            form = RUNS;
+            const int words = (int)(in.inner / 4) * beams;
+            a.groupsPerTile = RUN_WORDS / words / 4 * 4;  // tiles start at whole vectors
+            a.groupTiles = (groups + a.groupsPerTile - 1) / a.groupsPerTile;
+            n = (in.outer + RUN_SLABS - 1) / RUN_SLABS * a.groupTiles;
+        }
+        else
+        {
             a.unit = 16;
             while (bits % a.unit) a.unit /= 2;
             const long long rowUnits = in.inner / a.unit;
@@ -1490,13 +1656,21 @@ void launchReorder(const StateArray* arrays, int count, const long long* parents
             a.unitTiles = (int)((rowUnits + a.units - 1) / a.units);
             a.groupsPerTile = 1;
             if (a.unitTiles == 1)
-                a.groupsPerTile = (int)std::max<long long>(1, std::min<long long>(REORDER_TILE / (beams * in.inner), BEAM_MAX_BEAMS / beams));
+                a.groupsPerTile = (int)std::max<long long>(
+                    1, std::min<long long>(REORDER_TILE / (beams * in.inner), BEAM_MAX_BEAMS / beams));
             a.groupTiles = (groups + a.groupsPerTile - 1) / a.groupsPerTile;
-            a.firstBlock = blocks;
-            blocks += in.outer * a.groupTiles * a.unitTiles;
+            n = in.outer * a.groupTiles * a.unitTiles;
         }
-        if (blocks > 0) reorderKernel<<<(unsigned)blocks, REORDER_THREADS, 0, s>>>(p);
+        ReorderParams& q = p[form];
+        if (q.count == REORDER_ARRAYS || blocks[form] + n > 0x7fffffff) flush(form);
+        q.parents = parents;
+        q.groups = groups;
+        q.beams = beams;
+        a.firstBlock = blocks[form];
+        q.a[q.count++] = a;
+        blocks[form] += n;
     }
+    for (int f = 0; f < FORMS; f++) flush(f);
 }
 
 void launchMoveContacts(int* contact, const long long* parents, int nSim, int beams, int nCars, cudaStream_t s)

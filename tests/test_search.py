@@ -358,6 +358,31 @@ def test_reorder_rows_and_words(G, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("G, K", [(4001, 3), (1500, 8), (700, 16), (301, 17), (97, 64), (5001, 2), (11, 1000)])
+def test_reorder_large_arrays(G, K):
+    """Sizes at which rows go through registers and short rows as dense runs, with odd ends and slabs."""
+    import torch
+    from carl_b200.search import reorder_states
+
+    g = torch.Generator("cuda").manual_seed(G + K)
+    n = G * K
+    parents = torch.randint(-1, K + 1, (G, K), device="cuda", generator=g)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    # Runs: slabs of 1, 2, 3, 6 and 7 words a row (odd slab strides too), one slab, 128 words a row.
+    words = [rand(29, n, w) for w in (1, 2, 3, 6, 7)] + [rand(1, n, 5), rand(13, n, 2).bfloat16(), rand(2, n, 128)]
+    want = [_reordered(t, parents, 1) for t in words]
+    reorder_states(words, parents, dim=1)
+    assert all(torch.equal(a, b) for a, b in zip(words, want))
+    # Rows: 256 bytes to 12 KB, whole columns or not, at an offset.
+    store = rand(n + 1, 64)
+    rows = [rand(n, 6, 252), rand(n, 64), rand(n, 516).bfloat16(), rand(n, 1030).half(), rand(n, 2500), store[1:], rand(n) > 0]
+    want = [_reordered(t, parents, 0) for t in rows]
+    first = store[0].clone()
+    reorder_states(rows, parents)
+    assert all(torch.equal(a, b) for a, b in zip(rows, want)) and torch.equal(store[0], first)
+
+
+@pytest.mark.gpu
 def test_reorder_many_arrays_and_neighbours():
     """More arrays than one launch takes; nothing around an array is touched."""
     import torch
