@@ -1536,7 +1536,8 @@ static const char* historyError(const carlb_history* h)
     if (h->row_pages < 1 || h->page_len < 1 || h->record_bytes < 1)
         return "row_pages, page_len and record_bytes must be positive";
     if ((int64_t)h->row_pages * h->page_len > INT32_MAX) return "rows are too long";
-    if (h->record_bytes > (1ll << 40) / h->page_len) return "pages are too large";
+    if (h->record_bytes > (1ll << 30)) return "records are too long";
+    if ((int64_t)h->n_rows * h->page_len > (1ll << 33)) return "too many rows or records of a page";
     if (h->n_pages > 0 && (!h->pages || !h->refs || misaligned(h->refs, 4))) return "pages or refs is null or misaligned";
     if (h->n_rows > 0 && (!h->table || !h->lengths || misaligned(h->table, 4) || misaligned(h->lengths, 4)))
         return "table or lengths is null or misaligned";

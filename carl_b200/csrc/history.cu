@@ -16,9 +16,66 @@ using u64 = unsigned long long;
 
 constexpr unsigned FULL = 0xffffffffu;
 constexpr int THREADS = 256;
-constexpr int CHUNK = 1024;  // rows or pages whose counts one block takes together
+constexpr int CHUNK = THREADS;          // rows or pages that one block counts
+constexpr int ITEM_BYTES = 4096;        // what a warp copies, where records are smaller
 
 inline unsigned blocks(long long n, int t) { return (unsigned)((n + t - 1) / t); }
+
+// ---- copies of whole records -------------------------------------------------------------
+
+// Copies `bytes` with the threads of a warp or block (tid of `threads`); four loads of a
+// thread are under way before the first store.
+template <class U>
+__device__ __forceinline__ void copyUnits(char* to, const char* from, long long bytes, int tid, int threads)
+{
+    U* t = reinterpret_cast<U*>(to);
+    const U* f = reinterpret_cast<const U*>(from);
+    const long long n = bytes / (long long)sizeof(U);
+    long long i = tid;
+    for (; i + 3ll * threads < n; i += 4ll * threads)
+    {
+        U v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = f[i + (long long)k * threads];
+#pragma unroll
+        for (int k = 0; k < 4; k++) t[i + (long long)k * threads] = v[k];
+    }
+    U v[3];
+#pragma unroll
+    for (int k = 0; k < 3; k++)
+        if (i + (long long)k * threads < n) v[k] = f[i + (long long)k * threads];
+#pragma unroll
+    for (int k = 0; k < 3; k++)
+        if (i + (long long)k * threads < n) t[i + (long long)k * threads] = v[k];
+}
+
+__device__ __forceinline__ void copyBytes(char* to, const char* from, long long bytes, int unit, int tid, int threads)
+{
+    switch (unit)
+    {
+    case 16: copyUnits<uint4>(to, from, bytes, tid, threads); break;
+    case 8: copyUnits<uint2>(to, from, bytes, tid, threads); break;
+    case 4: copyUnits<unsigned>(to, from, bytes, tid, threads); break;
+    case 2: copyUnits<unsigned short>(to, from, bytes, tid, threads); break;
+    default: copyUnits<uint8_t>(to, from, bytes, tid, threads); break;
+    }
+}
+
+// Largest unit that divides addresses and sizes (their bits or-ed together).
+int unitOf(unsigned long long bits)
+{
+    int unit = 16;
+    while (bits % unit) unit /= 2;
+    return unit;
+}
+
+// Records of an item of work.
+int itemRecords(long long recordBytes, int most)
+{
+    return (int)std::max<long long>(1, std::min<long long>(most, ITEM_BYTES / recordBytes));
+}
+
+// ---- counts ------------------------------------------------------------------------------
 
 // The page of a table entry, or -1 where the table names none.
 __device__ __forceinline__ int pageAt(const HistoryView& h, long long row, int col)
@@ -50,18 +107,26 @@ __global__ void __launch_bounds__(THREADS) forkKernel(HistoryView from, HistoryV
 
 // ---- append ---------------------------------------------------------------------------
 
-enum RowKind : uint8_t { ROW_IDLE = 0, ROW_IN_PLACE, ROW_NEW_PAGE, ROW_COPY, ROW_FULL };
+// What a row needs, from the counts before anything changes.
+enum RowKind { ROW_IDLE = 0, ROW_IN_PLACE, ROW_NEW_PAGE, ROW_COPY, ROW_FULL };
+
+struct Job
+{
+    int kind;
+    int length;  // before the record
+    int held;    // page with the records before it, -1 at a page's start
+    int rank;    // rows in need before it in its chunk
+};
 
 struct AppendWork
 {
     u64* leader;      // [nPages] longest, then first, of the rows that share the page and append
     int* sharers;     // [nPages] how many those are
+    unsigned* done;   // blocks that have counted
     int* rowNeeds;    // [row chunks + 1] pages needed, then their prefix sums
     int* pageFree;    // [page chunks + 1] free pages, then their prefix sums
-    int* freeList;    // [nRows] the lowest free pages
-    int* target;      // [nRows] page a record goes to, -1 for none
-    int* source;      // [nRows] page whose records come with it, -1 for none
-    uint8_t* kind;    // [nRows]
+    unsigned* bits;   // [page chunks, CHUNK / 32] free pages
+    Job* job;         // [nRows]
     int rowChunks, pageChunks;
 };
 
@@ -75,15 +140,14 @@ AppendWork planAppend(const HistoryView& h, void* base, long long* bytes, long l
     char* c = static_cast<char*>(base);
     long long at = 0;
     auto take = [&](long long n) { const long long o = at; at += alignUp(n); return c + o; };
+    w.done = reinterpret_cast<unsigned*>(take(4));
     w.leader = reinterpret_cast<u64*>(take(8ll * h.nPages));
     w.sharers = reinterpret_cast<int*>(take(4ll * h.nPages));
     if (zeroBytes) *zeroBytes = at;
     w.rowNeeds = reinterpret_cast<int*>(take(4ll * (w.rowChunks + 1)));
     w.pageFree = reinterpret_cast<int*>(take(4ll * (w.pageChunks + 1)));
-    w.freeList = reinterpret_cast<int*>(take(4ll * h.nRows));
-    w.target = reinterpret_cast<int*>(take(4ll * h.nRows));
-    w.source = reinterpret_cast<int*>(take(4ll * h.nRows));
-    w.kind = reinterpret_cast<uint8_t*>(take(h.nRows));
+    w.bits = reinterpret_cast<unsigned*>(take(4ll * w.pageChunks * (CHUNK / 32)));
+    w.job = reinterpret_cast<Job*>(take((long long)sizeof(Job) * h.nRows));
     if (bytes) *bytes = at;
     return w;
 }
@@ -95,7 +159,7 @@ __device__ __forceinline__ u64 leaderKey(int slot, int row) { return (u64)(unsig
 struct Append
 {
     bool on, room;
-    int col, slot, held;
+    int length, col, slot, held;
 };
 
 __device__ __forceinline__ Append appendOf(const HistoryView& h, const uint8_t* mask, int r)
@@ -103,10 +167,10 @@ __device__ __forceinline__ Append appendOf(const HistoryView& h, const uint8_t* 
     Append a{};
     a.held = -1;
     a.on = !mask || mask[r];
-    const int length = h.lengths[r];
-    a.col = length / h.pageLen;
-    a.slot = length - a.col * h.pageLen;
-    a.room = length >= 0 && a.col < h.rowPages;
+    a.length = h.lengths[r];
+    a.col = a.length / h.pageLen;
+    a.slot = a.length - a.col * h.pageLen;
+    a.room = a.length >= 0 && a.col < h.rowPages;
     if (a.on && a.room && a.slot > 0)
     {
         a.held = pageAt(h, r, a.col);
@@ -125,18 +189,6 @@ __global__ void __launch_bounds__(THREADS) appendShareKernel(HistoryView h, cons
     atomicMax(&w.leader[a.held], leaderKey(a.slot, r));
 }
 
-__device__ __forceinline__ int blockSum(int v)
-{
-    __shared__ int part[THREADS / 32];
-    v = __reduce_add_sync(FULL, v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    int s = 0;
-    for (int k = 0; k < THREADS / 32; k++) s += part[k];
-    return s;
-}
-
 // Exclusive prefix sum of a flag over the block's threads; total over the block.
 __device__ __forceinline__ int blockRank(bool flag, int& total)
 {
@@ -147,6 +199,7 @@ __device__ __forceinline__ int blockRank(bool flag, int& total)
     __syncthreads();
     int before = 0;
     total = 0;
+#pragma unroll
     for (int k = 0; k < THREADS / 32; k++)
     {
         if (k < (int)(threadIdx.x >> 5)) before += part[k];
@@ -155,174 +208,168 @@ __device__ __forceinline__ int blockRank(bool flag, int& total)
     return before + __popc(votes & ((1u << (threadIdx.x & 31)) - 1));
 }
 
-// What each row needs, counted per chunk of rows; free pages per chunk of pages.
+// Exclusive prefix sums of n counts in place, the total behind them; one block.
+__device__ void scanCounts(int* counts, int n)
+{
+    __shared__ int part[THREADS / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int carry = 0;
+    for (int i0 = 0; i0 < n; i0 += THREADS)
+    {
+        const int i = i0 + threadIdx.x, mine = i < n ? __ldcg(counts + i) : 0;
+        int sum = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2)
+        {
+            const int o = __shfl_up_sync(FULL, sum, d);
+            if (lane >= d) sum += o;
+        }
+        __syncthreads();
+        if (lane == 31) part[warp] = sum;
+        __syncthreads();
+        int total = 0;
+#pragma unroll
+        for (int k = 0; k < THREADS / 32; k++)
+        {
+            if (k < warp) sum += part[k];
+            total += part[k];
+        }
+        if (i < n) counts[i] = carry + sum - mine;
+        carry += total;
+    }
+    if (threadIdx.x == 0) counts[n] = carry;
+}
+
+// Whether this block is the last to come here; what the others wrote before is visible.
+__device__ __forceinline__ bool lastBlock(unsigned* done)
+{
+    __shared__ bool last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(done, 1) + 1 == gridDim.x;
+    __syncthreads();
+    if (last) __threadfence();
+    return last;
+}
+
+// What each row needs, counted per chunk of rows; the free pages, counted per chunk of
+// pages.  The last block adds the counts up.
 __global__ void __launch_bounds__(THREADS) appendCountKernel(HistoryView h, const uint8_t* mask, AppendWork w)
 {
     const int b = blockIdx.x;
-    int count = 0;
+    int total;
     if (b < w.rowChunks)
     {
-        for (int i = threadIdx.x; i < CHUNK; i += THREADS)
+        const long long r = (long long)b * CHUNK + threadIdx.x;
+        Job job{ ROW_IDLE, 0, -1, 0 };
+        if (r < h.nRows)
         {
-            const long long r = (long long)b * CHUNK + i;
-            if (r >= h.nRows) break;
             const Append a = appendOf(h, mask, (int)r);
-            RowKind kind = ROW_IDLE;
+            job.length = a.length;
+            job.held = a.held;
             if (a.on && !a.room)
-                kind = ROW_FULL;
+                job.kind = ROW_FULL;
             else if (a.on && a.slot == 0)
-                kind = ROW_NEW_PAGE;
+                job.kind = ROW_NEW_PAGE;
             else if (a.on)
             {
                 const int refs = h.refs[a.held];
                 const bool stays = refs <= 1 || (w.sharers[a.held] == refs && w.leader[a.held] == leaderKey(a.slot, (int)r));
-                kind = stays ? ROW_IN_PLACE : ROW_COPY;
+                job.kind = stays ? ROW_IN_PLACE : ROW_COPY;
             }
-            w.kind[r] = kind;
-            count += kind == ROW_NEW_PAGE || kind == ROW_COPY;
         }
-        count = blockSum(count);
-        if (threadIdx.x == 0) w.rowNeeds[b] = count;
+        job.rank = blockRank(job.kind == ROW_NEW_PAGE || job.kind == ROW_COPY, total);
+        if (r < h.nRows) w.job[r] = job;
+        if (threadIdx.x == 0) w.rowNeeds[b] = total;
     }
     else
     {
         const int c = b - w.rowChunks;
-        for (int i = threadIdx.x; i < CHUNK; i += THREADS)
-        {
-            const long long p = (long long)c * CHUNK + i;
-            if (p < h.nPages) count += h.refs[p] <= 0;
-        }
-        count = blockSum(count);
-        if (threadIdx.x == 0) w.pageFree[c] = count;
-    }
-}
-
-// Exclusive prefix sums of n counts in place, the total behind them; one block.
-__device__ void scanCounts(int* counts, int n)
-{
-    __shared__ int part[THREADS];
-    const int each = (n + THREADS - 1) / THREADS, i0 = threadIdx.x * each, i1 = min(n, i0 + each);
-    int s = 0;
-    for (int i = i0; i < i1; i++) s += counts[i];
-    __syncthreads();
-    part[threadIdx.x] = s;
-    __syncthreads();
-    int before = 0, total = 0;
-    for (int k = 0; k < THREADS; k++)
-    {
-        if (k < (int)threadIdx.x) before += part[k];
-        total += part[k];
-    }
-    for (int i = i0; i < i1; i++)
-    {
-        const int c = counts[i];
-        counts[i] = before;
-        before += c;
-    }
-    if (threadIdx.x == 0) counts[n] = total;
-}
-
-__global__ void __launch_bounds__(THREADS) scanKernel(int* a, int na, int* b, int nb)
-{
-    if (blockIdx.x == 0)
-        scanCounts(a, na);
-    else
-        scanCounts(b, nb);
-}
-
-// The k-th free page for every k that a row needs.
-__global__ void __launch_bounds__(THREADS) freeListKernel(HistoryView h, AppendWork w)
-{
-    const int needs = w.rowNeeds[w.rowChunks];
-    int rank = w.pageFree[blockIdx.x];
-    if (rank >= needs) return;
-    for (int i0 = 0; i0 < CHUNK; i0 += THREADS)
-    {
-        const long long p = (long long)blockIdx.x * CHUNK + i0 + threadIdx.x;
+        const long long p = (long long)c * CHUNK + threadIdx.x;
         const bool isFree = p < h.nPages && h.refs[p] <= 0;
-        int total;
-        const int k = rank + blockRank(isFree, total);
-        if (isFree && k < needs) w.freeList[k] = (int)p;
-        rank += total;
+        const unsigned votes = __ballot_sync(FULL, isFree);
+        if ((threadIdx.x & 31) == 0) w.bits[c * (CHUNK / 32) + (threadIdx.x >> 5)] = votes;
+        blockRank(isFree, total);
+        if (threadIdx.x == 0) w.pageFree[c] = total;
     }
+    if (!lastBlock(w.done)) return;
+    scanCounts(w.rowNeeds, w.rowChunks);
+    __syncthreads();
+    scanCounts(w.pageFree, w.pageChunks);
 }
 
-// Every row's page: table, counts and lengths; rows that find none are dropped.
-__global__ void __launch_bounds__(THREADS) appendAssignKernel(HistoryView h, AppendWork w, int* dropped)
+// The k-th free page: its chunk by bisection of the prefix sums, then its bit.
+__device__ __forceinline__ int freePage(const AppendWork& w, int k)
 {
-    const int nFree = w.pageFree[w.pageChunks];
-    int rank = w.rowNeeds[blockIdx.x];
-    for (int i0 = 0; i0 < CHUNK; i0 += THREADS)
+    int lo = 0, hi = w.pageChunks - 1;
+    while (lo < hi)
     {
-        const long long r = (long long)blockIdx.x * CHUNK + i0 + threadIdx.x;
-        const RowKind kind = r < h.nRows ? (RowKind)w.kind[r] : ROW_IDLE;
-        const bool needs = kind == ROW_NEW_PAGE || kind == ROW_COPY;
-        int total;
-        const int k = rank + blockRank(needs, total);
-        rank += total;
-        if (r >= h.nRows) continue;
-        int target = -1, source = -1;
-        const int length = h.lengths[r];
-        const int col = length / h.pageLen;
-        if (kind == ROW_IN_PLACE) target = h.table[r * h.rowPages + col];
-        if (needs && k < nFree)
-        {
-            target = w.freeList[k];
-            if (kind == ROW_COPY)
-            {
-                source = h.table[r * h.rowPages + col];
-                atomicSub(&h.refs[source], 1);
-            }
-            h.refs[target] = 1;
-            h.table[r * h.rowPages + col] = target;
-        }
-        if (target >= 0)
-            h.lengths[r] = length + 1;
-        else if (kind != ROW_IDLE)
-            atomicAdd(dropped, 1);
-        w.target[r] = target;
-        w.source[r] = source;
+        const int mid = (lo + hi + 1) / 2;
+        if (w.pageFree[mid] <= k)
+            lo = mid;
+        else
+            hi = mid - 1;
     }
-}
-
-template <class U>
-__device__ __forceinline__ void copyUnits(char* to, const char* from, long long bytes, int lane, int lanes)
-{
-    U* t = reinterpret_cast<U*>(to);
-    const U* f = reinterpret_cast<const U*>(from);
-    for (long long i = lane; i < bytes / (long long)sizeof(U); i += lanes) t[i] = f[i];
-}
-
-__device__ __forceinline__ void copyRecord(char* to, const char* from, long long bytes, int unit, int lane, int lanes)
-{
-    switch (unit)
+    k -= w.pageFree[lo];
+    const uint4* bits = reinterpret_cast<const uint4*>(w.bits + lo * (CHUNK / 32));
+    const uint4 a = bits[0], b = bits[1];
+    const unsigned word[CHUNK / 32] = { a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w };
+    int page = lo * CHUNK;
+#pragma unroll
+    for (int i = 0; i < CHUNK / 32; i++)
     {
-    case 16: copyUnits<uint4>(to, from, bytes, lane, lanes); break;
-    case 8: copyUnits<uint2>(to, from, bytes, lane, lanes); break;
-    case 4: copyUnits<unsigned>(to, from, bytes, lane, lanes); break;
-    case 2: copyUnits<unsigned short>(to, from, bytes, lane, lanes); break;
-    default: copyUnits<uint8_t>(to, from, bytes, lane, lanes); break;
+        const int n = __popc(word[i]);
+        if (k >= 0 && k < n) return page + 32 * i + __fns(word[i], 0, k + 1);
+        k -= n;
     }
+    return -1;
 }
 
-// A warp per (row, slot): the row's record, or one record of the page it copies.
-__global__ void __launch_bounds__(THREADS) appendDataKernel(HistoryView h, AppendWork w, const char* records,
-                                                            long long recordStride, int unit)
+// A warp per row and item of its page: the records that come along with a copied page,
+// and the row's own.  The first item's warp enters the row's page and length.
+__global__ void __launch_bounds__(THREADS) appendWriteKernel(HistoryView h, AppendWork w, const char* records,
+                                                             long long recordStride, int unit, int perItem, int items,
+                                                             int* dropped)
 {
     const long long item = (blockIdx.x * (long long)THREADS + threadIdx.x) >> 5;
     const int lane = threadIdx.x & 31;
-    const long long r = item / h.pageLen;
-    const int s = (int)(item - r * h.pageLen);
+    const long long r = item / items;
     if (r >= h.nRows) return;
-    const int target = w.target[r];
+    const int part = (int)(item - r * items);
+    const int4 j = *reinterpret_cast<const int4*>(w.job + r);
+    const Job job{ j.x, j.y, j.z, j.w };
+    if (job.kind == ROW_IDLE) return;
+    const int col = job.length / h.pageLen, slot = job.length - col * h.pageLen;
+    const int s0 = part * perItem, s1 = min(s0 + perItem, slot);
+    const bool own = s0 <= slot && slot < s0 + perItem, copies = job.kind == ROW_COPY && s0 < s1;
+    if (!own && !copies && part != 0) return;
+    int target = job.kind == ROW_IN_PLACE ? job.held : -1;
+    if (job.kind == ROW_NEW_PAGE || job.kind == ROW_COPY)
+    {
+        const int k = w.rowNeeds[r / CHUNK] + job.rank;
+        if (k < w.pageFree[w.pageChunks]) target = freePage(w, k);
+    }
+    if (part == 0 && lane == 0)
+    {
+        if (target < 0)
+            atomicAdd(dropped, 1);
+        else
+        {
+            h.lengths[r] = job.length + 1;
+            if (job.kind != ROW_IN_PLACE)
+            {
+                h.table[r * h.rowPages + col] = target;
+                h.refs[target] = 1;
+                if (job.kind == ROW_COPY) atomicSub(&h.refs[job.held], 1);
+            }
+        }
+    }
     if (target < 0) return;
-    const int slot = (h.lengths[r] - 1) % h.pageLen;
-    const int source = w.source[r];
-    char* to = h.pages + ((long long)target * h.pageLen + s) * h.recordBytes;
-    if (s == slot)
-        copyRecord(to, records + r * recordStride, h.recordBytes, unit, lane, 32);
-    else if (s < slot && source >= 0)
-        copyRecord(to, h.pages + ((long long)source * h.pageLen + s) * h.recordBytes, h.recordBytes, unit, lane, 32);
+    char* to = h.pages + (long long)target * h.pageLen * h.recordBytes;
+    if (copies)
+        copyBytes(to + s0 * h.recordBytes, h.pages + ((long long)job.held * h.pageLen + s0) * h.recordBytes,
+                  (s1 - s0) * h.recordBytes, unit, lane, 32);
+    if (own) copyBytes(to + slot * h.recordBytes, records + r * recordStride, h.recordBytes, unit, lane, 32);
 }
 
 // ---- free -----------------------------------------------------------------------------
@@ -344,10 +391,12 @@ __global__ void __launch_bounds__(THREADS) freeKernel(HistoryView h, const uint8
 
 struct CompactWork
 {
+    unsigned* done;   // blocks that have counted
+    int* moves;       // pages that move
     int* liveCount;   // [page chunks + 1]
     int* hole;        // [nPages] hole of rank k
     int* moved;       // [nPages] page that goes to hole k
-    int* rankOf;      // [nPages] k of a page that moves
+    int* rankOf;      // [nPages] k of a page that moves, -1 of another
     int pageChunks;
 };
 
@@ -358,6 +407,8 @@ CompactWork planCompact(const HistoryView& h, void* base, long long* bytes)
     char* c = static_cast<char*>(base);
     long long at = 0;
     auto take = [&](long long n) { const long long o = at; at += alignUp(n); return reinterpret_cast<int*>(c + o); };
+    w.done = reinterpret_cast<unsigned*>(take(4));
+    w.moves = take(4);
     w.liveCount = take(4ll * (w.pageChunks + 1));
     w.hole = take(4ll * h.nPages);
     w.moved = take(4ll * h.nPages);
@@ -366,61 +417,60 @@ CompactWork planCompact(const HistoryView& h, void* base, long long* bytes)
     return w;
 }
 
-__global__ void __launch_bounds__(THREADS) liveCountKernel(HistoryView h, CompactWork w)
+__global__ void __launch_bounds__(THREADS) liveCountKernel(HistoryView h, CompactWork w, int* live)
 {
-    int count = 0;
-    for (int i = threadIdx.x; i < CHUNK; i += THREADS)
+    const long long p = (long long)blockIdx.x * CHUNK + threadIdx.x;
+    int total;
+    blockRank(p < h.nPages && h.refs[p] > 0, total);
+    if (threadIdx.x == 0) w.liveCount[blockIdx.x] = total;
+    if (!lastBlock(w.done)) return;
+    scanCounts(w.liveCount, w.pageChunks);
+    if (threadIdx.x == 0)
     {
-        const long long p = (long long)blockIdx.x * CHUNK + i;
-        if (p < h.nPages) count += h.refs[p] > 0;
+        *live = w.liveCount[w.pageChunks];
+        if (*live == h.nPages) *w.moves = 0;  // otherwise page L tells
     }
-    count = blockSum(count);
-    if (threadIdx.x == 0) w.liveCount[blockIdx.x] = count;
 }
 
 // With L live pages, the k-th hole below L takes the k-th highest live page: both
 // ranks come from the number of live pages before a page.
-__global__ void __launch_bounds__(THREADS) compactPlanKernel(HistoryView h, CompactWork w, int* live)
+__global__ void __launch_bounds__(THREADS) compactPlanKernel(HistoryView h, CompactWork w)
 {
     const int L = w.liveCount[w.pageChunks];
-    if (blockIdx.x == 0 && threadIdx.x == 0) *live = L;
-    int before = w.liveCount[blockIdx.x];
-    for (int i0 = 0; i0 < CHUNK; i0 += THREADS)
+    const long long p = (long long)blockIdx.x * CHUNK + threadIdx.x;
+    const bool isLive = p < h.nPages && h.refs[p] > 0;
+    int total;
+    const int q = w.liveCount[blockIdx.x] + blockRank(isLive, total);
+    if (p >= h.nPages) return;
+    if (p == L) *w.moves = L - q;
+    if (p < L)
     {
-        const long long p = (long long)blockIdx.x * CHUNK + i0 + threadIdx.x;
-        const bool isLive = p < h.nPages && h.refs[p] > 0;
-        int total;
-        const int q = before + blockRank(isLive, total);
-        before += total;
-        if (p >= h.nPages) continue;
-        if (!isLive && p < L) w.hole[p - q] = (int)p;
-        if (isLive && p >= L)
-        {
-            w.moved[L - 1 - q] = (int)p;
-            w.rankOf[p] = L - 1 - q;
-        }
+        if (!isLive) w.hole[p - q] = (int)p;
+        return;
     }
+    w.rankOf[p] = isLive ? L - 1 - q : -1;
+    if (isLive) w.moved[L - 1 - q] = (int)p;
 }
 
-__global__ void __launch_bounds__(THREADS) compactTableKernel(HistoryView h, CompactWork w)
-{
-    const long long i = blockIdx.x * (long long)THREADS + threadIdx.x;
-    if (i >= (long long)h.nRows * h.rowPages) return;
-    const int page = h.table[i], L = w.liveCount[w.pageChunks];
-    if (page >= L && page < h.nPages && h.refs[page] > 0) h.table[i] = w.hole[w.rankOf[page]];
-}
-
-// Blocks take the moves in turn; their number is known on the device only.
-__global__ void __launch_bounds__(THREADS) compactMoveKernel(HistoryView h, CompactWork w, int unit)
+// The first blocks take the moves in turn (their number is known on the device only),
+// the others follow them in the table.
+__global__ void __launch_bounds__(THREADS) compactMoveKernel(HistoryView h, CompactWork w, int movers, int unit)
 {
     const int L = w.liveCount[w.pageChunks];
-    // Live pages at or beyond L, as many as there are holes below it.
+    if ((int)blockIdx.x >= movers)
+    {
+        const long long i = (blockIdx.x - movers) * (long long)THREADS + threadIdx.x;
+        if (i >= (long long)h.nRows * h.rowPages) return;
+        const int page = h.table[i];
+        if (page >= L && page < h.nPages && w.rankOf[page] >= 0) h.table[i] = w.hole[w.rankOf[page]];
+        return;
+    }
     const long long bytes = (long long)h.pageLen * h.recordBytes;
-    for (int k = blockIdx.x; k < h.nPages - L && k < L; k += gridDim.x)
+    const int moves = *w.moves;
+    for (int k = blockIdx.x; k < moves; k += movers)
     {
         const int to = w.hole[k], from = w.moved[k];
-        if (from < 0) break;
-        copyRecord(h.pages + to * bytes, h.pages + from * bytes, bytes, unit, threadIdx.x, THREADS);
+        copyBytes(h.pages + to * bytes, h.pages + from * bytes, bytes, unit, threadIdx.x, THREADS);
         if (threadIdx.x == 0)
         {
             h.refs[to] = h.refs[from];
@@ -431,41 +481,47 @@ __global__ void __launch_bounds__(THREADS) compactMoveKernel(HistoryView h, Comp
 
 // ---- read -----------------------------------------------------------------------------
 
-// A warp per (row, step): the last min(length, steps) records of a row, zeros behind.
-__global__ void __launch_bounds__(THREADS) readKernel(HistoryView h, const long long* rows, int n, int steps, char* out,
-                                                      int* counts, int unit)
+// A warp per item of `perItem` steps of a row: the last min(length, steps) records of the
+// row, zeros behind them.  Lane l finds record l of the item.
+template <class U>
+__global__ void __launch_bounds__(THREADS) readKernel(HistoryView h, const long long* rows, int n, int steps, int perItem,
+                                                      int items, char* out, int* counts)
 {
     const long long item = (blockIdx.x * (long long)THREADS + threadIdx.x) >> 5;
     const int lane = threadIdx.x & 31;
-    const long long i = item / steps;
-    const int t = (int)(item - i * steps);
+    const long long i = item / items;
     if (i >= n) return;
+    const int part = (int)(item - i * items), t0 = part * perItem, here = min(perItem, steps - t0);
     const long long r = rows ? rows[i] : i;
     int length = r >= 0 && r < h.nRows ? h.lengths[r] : 0;
-    length = max(0, min(length, (int)min((long long)h.rowPages * h.pageLen, 0x7fffffffll)));
+    length = (int)max(0ll, min((long long)length, (long long)h.rowPages * h.pageLen));
     const int count = min(length, steps);
-    if (t == 0 && lane == 0) counts[i] = count;
-    char* to = out + item * h.recordBytes;
-    int page = -1, at = 0;
-    if (t < count)
+    if (part == 0 && lane == 0) counts[i] = count;
+    long long source = -1;  // record of the pages
+    if (lane < here && t0 + lane < count)
     {
-        at = length - count + t;
-        page = pageAt(h, r, at / h.pageLen);
+        const int at = length - count + t0 + lane, col = at / h.pageLen, page = pageAt(h, r, col);
+        if (page >= 0) source = (long long)page * h.pageLen + at - col * h.pageLen;
     }
-    if (page >= 0)
+    const int units = (int)(h.recordBytes / sizeof(U)), all = here * units;
+    U* to = reinterpret_cast<U*>(out + (i * steps + t0) * h.recordBytes);
+    const U* pages = reinterpret_cast<const U*>(h.pages);
+    constexpr int AHEAD = 4;
+    for (int u0 = 0; u0 < all; u0 += 32 * AHEAD)
     {
-        copyRecord(to, h.pages + ((long long)page * h.pageLen + at % h.pageLen) * h.recordBytes, h.recordBytes, unit,
-                   lane, 32);
-        return;
+        U v[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++)
+        {
+            const int u = u0 + 32 * a + lane, record = u / units;
+            const long long from = __shfl_sync(FULL, source, record & 31);
+            v[a] = U{};
+            if (u < all && from >= 0) v[a] = pages[from * units + (u - record * units)];
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++)
+            if (u0 + 32 * a + lane < all) to[u0 + 32 * a + lane] = v[a];
     }
-    for (long long b = lane; b < h.recordBytes; b += 32) to[b] = 0;
-}
-
-int unitOf(unsigned long long bits)
-{
-    int unit = 16;
-    while (bits % unit) unit /= 2;
-    return unit;
 }
 
 }  // namespace
@@ -502,13 +558,11 @@ cudaError_t launchHistoryAppend(const HistoryView& h, const char* records, long 
     }
     appendShareKernel<<<blocks(h.nRows, THREADS), THREADS, 0, s>>>(h, mask, w);
     appendCountKernel<<<w.rowChunks + w.pageChunks, THREADS, 0, s>>>(h, mask, w);
-    scanKernel<<<2, THREADS, 0, s>>>(w.rowNeeds, w.rowChunks, w.pageFree, w.pageChunks);
-    if (w.pageChunks > 0) freeListKernel<<<w.pageChunks, THREADS, 0, s>>>(h, w);
-    appendAssignKernel<<<w.rowChunks, THREADS, 0, s>>>(h, w, dropped);
     const int unit = unitOf(reinterpret_cast<uintptr_t>(h.pages) | reinterpret_cast<uintptr_t>(records)
                             | (unsigned long long)h.recordBytes | (unsigned long long)recordStride);
-    appendDataKernel<<<blocks((long long)h.nRows * h.pageLen * 32, THREADS), THREADS, 0, s>>>(h, w, records, recordStride,
-                                                                                             unit);
+    const int perItem = itemRecords(h.recordBytes, h.pageLen), items = (h.pageLen + perItem - 1) / perItem;
+    appendWriteKernel<<<blocks((long long)h.nRows * items * 32, THREADS), THREADS, 0, s>>>(h, w, records, recordStride, unit,
+                                                                                          perItem, items, dropped);
     return cudaGetLastError();
 }
 
@@ -529,16 +583,13 @@ cudaError_t launchHistoryCompact(const HistoryView& h, int* live, void* workspac
 {
     if (h.nPages == 0) return cudaMemsetAsync(live, 0, sizeof(int), s);
     const CompactWork w = planCompact(h, workspace, nullptr);
-    // -1 marks the end of the moves.
-    const cudaError_t err = cudaMemsetAsync(w.moved, 0xff, 4ll * h.nPages, s);
+    const cudaError_t err = cudaMemsetAsync(w.done, 0, sizeof(unsigned), s);
     if (err != cudaSuccess) return err;
-    liveCountKernel<<<w.pageChunks, THREADS, 0, s>>>(h, w);
-    scanKernel<<<1, THREADS, 0, s>>>(w.liveCount, w.pageChunks, nullptr, 0);
-    compactPlanKernel<<<w.pageChunks, THREADS, 0, s>>>(h, w, live);
-    const long long n = (long long)h.nRows * h.rowPages;
-    if (n > 0) compactTableKernel<<<blocks(n, THREADS), THREADS, 0, s>>>(h, w);
+    liveCountKernel<<<w.pageChunks, THREADS, 0, s>>>(h, w, live);
+    compactPlanKernel<<<w.pageChunks, THREADS, 0, s>>>(h, w);
     const int unit = unitOf(reinterpret_cast<uintptr_t>(h.pages) | (unsigned long long)h.recordBytes * h.pageLen);
-    compactMoveKernel<<<(unsigned)std::min(h.nPages, 148 * 8), THREADS, 0, s>>>(h, w, unit);
+    const int movers = std::min(h.nPages, 148 * 8);
+    compactMoveKernel<<<movers + blocks((long long)h.nRows * h.rowPages, THREADS), THREADS, 0, s>>>(h, w, movers, unit);
     return cudaGetLastError();
 }
 
@@ -548,7 +599,16 @@ void launchHistoryRead(const HistoryView& h, const long long* rows, int n, int s
     if (n <= 0 || steps <= 0) return;
     const int unit = unitOf(reinterpret_cast<uintptr_t>(h.pages) | reinterpret_cast<uintptr_t>(out)
                             | (unsigned long long)h.recordBytes);
-    readKernel<<<blocks((long long)n * steps * 32, THREADS), THREADS, 0, s>>>(h, rows, n, steps, out, counts, unit);
+    const int perItem = itemRecords(h.recordBytes, std::min(32, steps)), items = (steps + perItem - 1) / perItem;
+    const unsigned n32 = blocks((long long)n * items * 32, THREADS);
+    switch (unit)
+    {
+    case 16: readKernel<uint4><<<n32, THREADS, 0, s>>>(h, rows, n, steps, perItem, items, out, counts); break;
+    case 8: readKernel<uint2><<<n32, THREADS, 0, s>>>(h, rows, n, steps, perItem, items, out, counts); break;
+    case 4: readKernel<unsigned><<<n32, THREADS, 0, s>>>(h, rows, n, steps, perItem, items, out, counts); break;
+    case 2: readKernel<unsigned short><<<n32, THREADS, 0, s>>>(h, rows, n, steps, perItem, items, out, counts); break;
+    default: readKernel<uint8_t><<<n32, THREADS, 0, s>>>(h, rows, n, steps, perItem, items, out, counts); break;
+    }
 }
 
 }  // namespace cb
