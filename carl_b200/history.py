@@ -22,10 +22,21 @@ streams.  Errors are as in ``carl_b200.carl``.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import capi
+
+
+@functools.lru_cache
+def _workspaces(n_rows: int, row_pages: int, n_pages: int, page_len: int) -> tuple[int, int]:
+    """Workspace bytes of an append and a compaction."""
+    sizes = ctypes.c_int64(), ctypes.c_int64()
+    # The addresses are not looked at beyond being there.
+    capi.check(capi.load().carlb_history_workspace(capi.History(16, 16, 16, 16, 1, n_rows, row_pages, n_pages, page_len, 0),
+                                                   *sizes))
+    return max(16, sizes[0].value), max(16, sizes[1].value)
 
 
 class PagedHistory:
@@ -63,14 +74,17 @@ class PagedHistory:
             raise ValueError("table must be [n_rows, row_pages], lengths [n_rows] and refs [n_pages]")
         if table.shape[1] * pages.shape[1] > 0x7fffffff or max(pages.shape[0], table.shape[0]) > 0x7fffffff:
             raise ValueError("too many rows, pages or records of a row")
-        self.pages, self.table, self.lengths, self.refs = pages, table, lengths, refs
-        self.record_shape = tuple(pages.shape[2:])
-        self._dropped = dropped
         record_bytes = pages.element_size()
-        for n in self.record_shape:
+        for n in pages.shape[2:]:
             record_bytes *= n
+        self._hold(pages, table, lengths, refs, dropped, record_bytes, pages.device, table.shape[0])
+
+    def _hold(self, pages, table, lengths, refs, dropped, record_bytes: int, device, n_rows: int) -> None:
+        self.pages, self.table, self.lengths, self.refs, self._dropped = pages, table, lengths, refs, dropped
+        self._device, self._record_bytes = device, record_bytes
+        shape = pages.shape
         self._view = capi.History(pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), record_bytes,
-                                  table.shape[0], table.shape[1], pages.shape[0], pages.shape[1], pages.device.index)
+                                  n_rows, table.shape[1], shape[0], shape[1], device.index)
 
     @classmethod
     def empty(cls, n_rows: int, row_pages: int, n_pages: int, page_len: int, record_shape: tuple = (),
@@ -84,6 +98,10 @@ class PagedHistory:
                    torch.full((n_rows, row_pages), -1, dtype=torch.int32, device=device),
                    torch.zeros(n_rows, dtype=torch.int32, device=device),
                    torch.zeros(n_pages, dtype=torch.int32, device=device))
+
+    @property
+    def record_shape(self) -> tuple[int, ...]:
+        return tuple(self.pages.shape[2:])
 
     @property
     def n_rows(self) -> int:
@@ -100,27 +118,27 @@ class PagedHistory:
     @property
     def dropped(self) -> torch.Tensor:
         if self._dropped is None:
-            self._dropped = torch.zeros(1, dtype=torch.int32, device=self.pages.device)
+            self._dropped = torch.zeros(1, dtype=torch.int32, device=self._device)
         return self._dropped
 
     def _stream(self) -> int:
-        return torch.cuda.current_stream(self.pages.device).cuda_stream
+        return capi.current_stream(self._device.index)
 
     def _mask(self, mask, name: str) -> torch.Tensor:
         if not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool:
             raise TypeError(f"{name} must be a bool tensor")
-        if mask.device != self.pages.device:
-            raise ValueError(f"{name} must be on {self.pages.device}")
+        if mask.device != self._device:
+            raise ValueError(f"{name} must be on {self._device}")
         if mask.shape != self.lengths.shape:
             raise ValueError(f"{name} must have shape [n_rows]")
-        return mask.contiguous()
+        return mask if mask.is_contiguous() else mask.contiguous()
 
     def _indices(self, indices, name: str) -> torch.Tensor:
         if not isinstance(indices, torch.Tensor) or indices.dtype != torch.int64:
             raise TypeError(f"{name} must be an int64 tensor")
-        if indices.device != self.pages.device:
-            raise ValueError(f"{name} must be on {self.pages.device}")
-        return indices.contiguous()
+        if indices.device != self._device:
+            raise ValueError(f"{name} must be on {self._device}")
+        return indices if indices.is_contiguous() else indices.contiguous()
 
     def fork(self, parents: torch.Tensor, out: PagedHistory | None = None) -> PagedHistory:
         """The history whose row r continues row parents[r] of this one.
@@ -133,12 +151,15 @@ class PagedHistory:
         appended to or compacted.  `out` takes the result instead of a new history: one
         over the same pages with a table, lengths and refs of its own (two histories
         used in turn, for instance by captured graphs)."""
-        p = self._indices(parents, "parents").view(-1)
-        n, row_pages, n_pages = p.numel(), self.table.shape[1], self.n_pages
+        p = self._indices(parents, "parents")
+        n, row_pages, n_pages = p.numel(), self.table.shape[1], self.pages.shape[0]
         if out is None:
-            book = torch.empty(n * row_pages + n + n_pages, dtype=torch.int32, device=self.pages.device)
-            out = PagedHistory(self.pages, book[:n * row_pages].view(n, row_pages),
-                               book[n * row_pages:n * row_pages + n], book[n * row_pages + n:], self._dropped)
+            if n > 0x7fffffff:
+                raise ValueError("too many rows, pages or records of a row")
+            table, lengths, refs = torch.empty(n * row_pages + n + n_pages, dtype=torch.int32, device=self._device).split(
+                (n * row_pages, n, n_pages))
+            out = PagedHistory.__new__(PagedHistory)
+            out._hold(self.pages, table.view(n, row_pages), lengths, refs, self._dropped, self._record_bytes, self._device, n)
         elif (out.pages.data_ptr() != self.pages.data_ptr() or out.pages.shape != self.pages.shape
               or out.pages.dtype != self.pages.dtype or out.table.shape != (n, row_pages)):
             raise ValueError("out must be over the same pages, with a row for every parent")
@@ -155,23 +176,23 @@ class PagedHistory:
         or has no table entry left, stays as it was and is counted in `dropped`."""
         if not isinstance(records, torch.Tensor) or records.dtype != self.pages.dtype:
             raise TypeError("records must be a tensor of the pages' dtype")
-        if records.device != self.pages.device:
-            raise ValueError(f"records must be on {self.pages.device}")
-        if records.shape != (self.n_rows, *self.record_shape):
+        if records.device != self._device:
+            raise ValueError(f"records must be on {self._device}")
+        shape = records.shape
+        n = self.lengths.shape[0]
+        if len(shape) == 0 or shape[0] != n or shape[1:] != self.pages.shape[2:]:
             raise ValueError("records must have shape [n_rows, *record]")
         m = None if mask is None else self._mask(mask, "mask")
-        if self.n_rows == 0:
+        if n == 0:
             return
-        rec = records.detach()
-        if not rec[0].is_contiguous() or rec.stride(0) < 0:
-            rec = rec.contiguous()
-        size = ctypes.c_int64()
+        if not records.is_contiguous() and not records[0].is_contiguous():
+            records = records.detach().contiguous()
         lib = capi.load()
-        capi.check(lib.carlb_history_workspace(self._view, size, None))
-        work = torch.empty(size.value, dtype=torch.uint8, device=self.pages.device)
-        capi.check(lib.carlb_history_append(self._view, rec.data_ptr(), rec.stride(0) * rec.element_size(),
+        size = _workspaces(n, self._view.row_pages, self._view.n_pages, self._view.page_len)[0]
+        work = torch.empty(size, dtype=torch.uint8, device=self._device)
+        capi.check(lib.carlb_history_append(self._view, records.data_ptr(), records.stride(0) * records.element_size(),
                                             None if m is None else m.data_ptr(), self.dropped.data_ptr(),
-                                            work.data_ptr(), size.value, self._stream()))
+                                            work.data_ptr(), size, self._stream()))
 
     def free(self, mask: torch.Tensor) -> None:
         """Empties the rows with mask[r]; a page is free when no row names it any more."""
@@ -183,12 +204,11 @@ class PagedHistory:
         """Moves the live pages to the front and returns their number, int32 [1] on the
         device: of L live pages, the k-th highest goes to the k-th free page below L.
         pages[:L] is then all that the history holds."""
-        size = ctypes.c_int64()
-        lib = capi.load()
-        capi.check(lib.carlb_history_workspace(self._view, None, size))
-        work = torch.empty(max(16, size.value), dtype=torch.uint8, device=self.pages.device)
-        live = torch.empty(1, dtype=torch.int32, device=self.pages.device)
-        capi.check(lib.carlb_history_compact(self._view, live.data_ptr(), work.data_ptr(), size.value, self._stream()))
+        v = self._view
+        size = _workspaces(v.n_rows, v.row_pages, v.n_pages, v.page_len)[1]
+        work = torch.empty(size, dtype=torch.uint8, device=self._device)
+        live = torch.empty(1, dtype=torch.int32, device=self._device)
+        capi.check(capi.load().carlb_history_compact(v, live.data_ptr(), work.data_ptr(), size, self._stream()))
         return live
 
     def read(self, steps: int, rows: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -199,12 +219,12 @@ class PagedHistory:
         if steps < 1:
             raise ValueError("steps must be positive")
         r = None if rows is None else self._indices(rows, "rows")
-        shape = (self.n_rows,) if r is None else tuple(r.shape)
-        counts = torch.empty(shape, dtype=torch.int32, device=self.pages.device)
+        shape = self.lengths.shape if r is None else r.shape
+        counts = torch.empty(shape, dtype=torch.int32, device=self._device)
         n = counts.numel()
         if n * steps > 1 << 33:
             raise ValueError("too many records")
-        out = torch.empty((*shape, steps, *self.record_shape), dtype=self.pages.dtype, device=self.pages.device)
+        out = torch.empty((*shape, steps, *self.pages.shape[2:]), dtype=self.pages.dtype, device=self._device)
         if n:
             capi.check(capi.load().carlb_history_read(self._view, None if r is None else r.data_ptr(), n, steps,
                                                       out.data_ptr(), counts.data_ptr(), self._stream()))

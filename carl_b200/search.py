@@ -61,26 +61,31 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, mask: torch.Tensor |
     return select(logits, scores, mask, width, finished, joint=False)
 
 
+def _check_device(name: str, t, device) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a CUDA device")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+
+
 def select(logits, scores, mask, width, finished, *, joint: bool) -> BeamStep:
     """Both selections: checks the arguments, allocates the outputs and launches."""
-    for name, t in (("logits", logits), ("scores", scores), ("mask", mask), ("finished", finished)):
-        if t is None and name in ("mask", "finished"):
-            continue
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a tensor")
-        if t.device.type != "cuda":
-            raise ValueError(f"{name} must be on a CUDA device")
-        if t.device != logits.device:
-            raise ValueError(f"{name} must be on {logits.device}")
+    if not isinstance(logits, torch.Tensor):
+        raise TypeError("logits must be a tensor")
+    device = logits.device
+    _check_device("logits", logits, device)
+    _check_device("scores", scores, device)
     kind = _LOGIT_TYPES.get(logits.dtype)
     if kind is None:
         raise TypeError("logits must have dtype float32, bfloat16 or float16")
-    if scores.dtype != torch.float32:
+    if scores.dtype is not torch.float32:
         raise TypeError("scores must have dtype float32")
-    if logits.dim() < 2 or logits.shape[-1] < 1 or logits.shape[-2] < 1:
-        raise ValueError("logits must have shape [..., beams, vocab] with at least one beam and action")
     shape = logits.shape
-    beams, vocab = shape[-2], shape[-1]
+    if len(shape) < 2 or shape[-1] < 1 or shape[-2] < 1:
+        raise ValueError("logits must have shape [..., beams, vocab] with at least one beam and action")
+    lead, beams, vocab = shape[:-2], shape[-2], shape[-1]
     if scores.shape != shape[:-1]:
         raise ValueError("scores must have the shape of logits without its last dimension")
     width = beams if width is None else int(width)
@@ -90,59 +95,67 @@ def select(logits, scores, mask, width, finished, *, joint: bool) -> BeamStep:
         raise ValueError(f"at most {most_beams} beams and {capi.BEAM_MAX_CANDIDATES} continuations of a group")
     if not 1 <= width <= most_width:
         raise ValueError(f"width must be 1 to {most_width}")
-    args = capi.BeamArgs()
-    x = logits.detach()
-    if x.stride(-1) != 1:
-        x = x.contiguous()
-    x = x.reshape(-1, beams, vocab) if x.dim() != 3 else x
-    groups = x.shape[0]
+    x, x_group, x_beam = _rows(logits, beams, vocab)
+    groups = lead[0] if len(lead) == 1 else logits.numel() // (beams * vocab)
     if groups > 0x7fffffff // beams:
         raise ValueError("too many groups")
-    s = scores.detach().contiguous()
-    args.logits, args.scores = x.data_ptr(), s.data_ptr()
-    args.logits_group_stride, args.logits_beam_stride = x.stride(0), x.stride(1)
-    m = f = None
+    s = scores if scores.is_contiguous() else scores.detach().contiguous()
+    m = f = m_ptr = f_ptr = None
+    m_group = m_beam = 0
     if mask is not None:
-        if mask.dtype != torch.bool:
+        _check_device("mask", mask, device)
+        if mask.dtype is not torch.bool:
             raise TypeError("mask must have dtype bool")
-        try:
-            m = mask.expand(shape)
-        except RuntimeError:
-            raise ValueError("mask must be broadcastable to logits") from None
-        if m.stride(-1) != 1:
-            m = m.contiguous()
-        m = m.reshape(-1, beams, vocab) if m.dim() != 3 else m
-        args.mask = m.data_ptr()
-        args.mask_group_stride, args.mask_beam_stride = m.stride(0), m.stride(1)
+        if mask.shape != shape:
+            try:
+                mask = mask.expand(shape)
+            except RuntimeError:
+                raise ValueError("mask must be broadcastable to logits") from None
+        m, m_group, m_beam = _rows(mask, beams, vocab)
+        m_ptr = m.data_ptr()
     if finished is not None:
-        if finished.dtype != torch.bool:
+        _check_device("finished", finished, device)
+        if finished.dtype is not torch.bool:
             raise TypeError("finished must have dtype bool")
         if finished.shape != shape[:-1]:
             raise ValueError("finished must have the shape of scores")
-        f = finished.contiguous()
-        args.finished = f.data_ptr()
-    out_shape = (*shape[:-2], width)
-    device = x.device
+        f = finished if finished.is_contiguous() else finished.contiguous()
+        f_ptr = f.data_ptr()
+    out_shape = (*lead, width)
     best = BeamStep(torch.empty(out_shape, dtype=torch.float32, device=device),
                     torch.empty(out_shape, dtype=torch.int64, device=device),
                     torch.empty((*out_shape, _HEADS) if joint else out_shape, dtype=torch.int32, device=device))
-    args.out_scores, args.out_parents, args.out_actions = (t.data_ptr() for t in best)
-    args.groups, args.beams, args.vocab, args.width = groups, beams, vocab, width
-    args.logit_type, args.device = kind, device.index
     if groups == 0:
         return best
+    args = capi.BeamArgs(x.data_ptr(), s.data_ptr(), m_ptr, f_ptr, best[0].data_ptr(), best[1].data_ptr(),
+                         best[2].data_ptr(), None, 0, x_group, x_beam, m_group, m_beam, groups, beams, vocab, width, kind,
+                         device.index)
     lib = capi.load()
-    stream = torch.cuda.current_stream(device).cuda_stream
     if joint:
-        capi.check(lib.carlb_joint_select(args, stream))
+        capi.check(lib.carlb_joint_select(args, capi.current_stream(device.index)))
         return best
     size = ctypes.c_int64()
     capi.check(lib.carlb_beam_workspace(args, size))
     if size.value:
         work = torch.empty(size.value, dtype=torch.uint8, device=device)
         args.workspace, args.workspace_bytes = work.data_ptr(), size.value
-    capi.check(lib.carlb_beam_select(args, stream))
+    capi.check(lib.carlb_beam_select(args, capi.current_stream(device.index)))
     return best
+
+
+def _rows(t: torch.Tensor, beams: int, vocab: int) -> tuple[torch.Tensor, int, int]:
+    """`t` [..., beams, vocab] with a dense last dimension and one stride between
+    groups, and its strides of a group and a beam; a copy where it has no such view."""
+    stride = t.stride()
+    if stride[-1] != 1:
+        t = t.detach().contiguous()
+        stride = t.stride()
+    if len(stride) == 3:
+        return t, stride[0], stride[1]
+    if len(stride) == 2:
+        return t, 0, stride[0]
+    t = t.detach().reshape(-1, beams, vocab)
+    return t, t.stride(0), t.stride(1)
 
 
 def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, dim: int = 0) -> None:
@@ -160,37 +173,39 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, dim: i
     """
     if isinstance(states, torch.Tensor):
         raise TypeError("states must be a sequence of tensors")
-    if not isinstance(parents, torch.Tensor) or parents.dtype != torch.int64:
+    if not isinstance(parents, torch.Tensor) or parents.dtype is not torch.int64:
         raise TypeError("parents must be an int64 tensor")
-    if parents.device.type != "cuda":
+    if not parents.is_cuda:
         raise ValueError("parents must be on a CUDA device")
     if parents.dim() < 1 or not 1 <= parents.shape[-1] <= capi.BEAM_MAX_BEAMS:
         raise ValueError(f"parents must have shape [..., beams] with 1 to {capi.BEAM_MAX_BEAMS} beams")
-    rows, beams = parents.numel(), parents.shape[-1]
-    arrays = (capi.StateArray * max(1, len(states)))()
-    for a, t in zip(arrays, states):
+    device, rows, beams, count = parents.device, parents.numel(), parents.shape[-1], len(states)
+    grad = torch.is_grad_enabled()
+    arrays = (capi.StateArray * max(1, count))()
+    for i, t in enumerate(states):
         if not isinstance(t, torch.Tensor):
             raise TypeError("states must be tensors")
-        if t.device != parents.device:
-            raise ValueError(f"states must be on {parents.device}")
-        if not -t.dim() <= dim < t.dim():
+        if t.device != device:
+            raise ValueError(f"states must be on {device}")
+        shape = t.shape
+        d = dim + len(shape) if dim < 0 else dim
+        if not 0 <= d < len(shape):
             raise ValueError("dim is out of range")
-        d = dim % t.dim()
-        if t.shape[d] != rows:
+        if shape[d] != rows:
             raise ValueError(f"dimension {dim} of every state must count the {rows} rows of parents")
         if not t.is_contiguous():
             raise ValueError("states must be contiguous")
-        if t.requires_grad and torch.is_grad_enabled():
+        if grad and t.requires_grad:
             raise ValueError("states that require a gradient cannot be moved in place")
-        if t.numel() == 0:
+        total = t.numel() * t.element_size()
+        if total == 0:
             continue
         outer = 1
-        for n in t.shape[:d]:
+        for n in shape[:d]:
             outer *= n
-        slab = t.numel() // outer * t.element_size()
-        a.data, a.outer, a.outer_stride, a.inner_bytes = t.data_ptr(), outer, slab, slab // rows
-    if rows == 0 or not len(states):
+        arrays[i] = (t.data_ptr(), outer, total // outer, total // outer // rows)
+    if rows == 0 or not count:
         return
-    p = parents.contiguous()
-    capi.check(capi.load().carlb_reorder_states(arrays, len(states), p.data_ptr(), rows // beams, beams, p.device.index,
-                                                torch.cuda.current_stream(p.device).cuda_stream))
+    p = parents if parents.is_contiguous() else parents.contiguous()
+    capi.check(capi.load().carlb_reorder_states(arrays, count, p.data_ptr(), rows // beams, beams, device.index,
+                                                capi.current_stream(device.index)))
