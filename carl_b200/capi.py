@@ -157,7 +157,7 @@ def load() -> ctypes.CDLL:
     lib.carlb_joint_select.argtypes = [beam, vp]
     lib.carlb_reorder_states.argtypes = [ctypes.POINTER(StateArray), i32, vp, i32, i32, i32, vp]
     lib.carlb_reorder.argtypes = [vp, vp, i32]
-    lib.carlb_history_fork.argtypes = [hist, hist, vp, vp]
+    lib.carlb_history_fork.argtypes = [hist, hist, vp, vp, vp]
     lib.carlb_history_workspace.argtypes = [hist, i64p, i64p]
     lib.carlb_history_append.argtypes = [hist, vp, i64, vp, vp, vp, i64, vp]
     lib.carlb_history_free.argtypes = [hist, vp, vp]

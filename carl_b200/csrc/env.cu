@@ -1550,7 +1550,8 @@ static HistoryView historyView(const carlb_history* h)
                         h->n_rows, h->row_pages, h->n_pages, h->page_len };
 }
 
-carlb_status carlb_history_fork(const carlb_history* from, const carlb_history* to, const int64_t* parents, void* stream)
+carlb_status carlb_history_fork(const carlb_history* from, const carlb_history* to, const int64_t* parents,
+                                int32_t* dropped, void* stream)
 {
     const char* bad = historyError(from);
     if (!bad) bad = historyError(to);
@@ -1561,11 +1562,12 @@ carlb_status carlb_history_fork(const carlb_history* from, const carlb_history* 
     if (!bad && ((to->n_pages > 0 && from->refs == to->refs)
                  || (to->n_rows > 0 && (from->table == to->table || from->lengths == to->lengths))))
         bad = "the forked history must not overlap its source";
+    if (!bad && misaligned(dropped, 4)) bad = "dropped is misaligned";
     if (bad) return fail(nullptr, CARLB_ERR_VALUE, bad);
     DeviceScope scope(to->device);
     if (scope.err != cudaSuccess) return cudaFail(nullptr, scope.err, "history fork");
     const cudaError_t err = launchHistoryFork(historyView(from), historyView(to),
-                                              reinterpret_cast<const long long*>(parents), (cudaStream_t)stream);
+                                              reinterpret_cast<const long long*>(parents), dropped, (cudaStream_t)stream);
     if (err != cudaSuccess) return cudaFail(nullptr, err, "history fork");
     return CARLB_OK;
 }

@@ -20,7 +20,9 @@ struct HistoryView
     int nRows, rowPages, nPages, pageLen;
 };
 
-cudaError_t launchHistoryFork(const HistoryView& from, const HistoryView& to, const long long* parents, cudaStream_t s);
+// counter: set to 0, or null.
+cudaError_t launchHistoryFork(const HistoryView& from, const HistoryView& to, const long long* parents, int* counter,
+                              cudaStream_t s);
 
 long long historyAppendWorkspace(const HistoryView& h);
 // records: nRows rows of recordBytes, recordStride bytes apart; mask: u8 [nRows] or

@@ -152,18 +152,21 @@ class PagedHistory:
         over the same pages with a table, lengths and refs of its own (two histories
         used in turn, for instance by captured graphs)."""
         p = self._indices(parents, "parents")
+        counter = None
         n, row_pages, n_pages = p.numel(), self.table.shape[1], self.pages.shape[0]
         if out is None:
             if n > 0x7fffffff:
                 raise ValueError("too many rows, pages or records of a row")
-            table, lengths, refs = torch.empty(n * row_pages + n + n_pages, dtype=torch.int32, device=self._device).split(
-                (n * row_pages, n, n_pages))
+            table, lengths, refs, fresh = torch.empty(
+                n * row_pages + n + n_pages + 1, dtype=torch.int32, device=self._device).split((n * row_pages, n, n_pages, 1))
             out = PagedHistory.__new__(PagedHistory)
             out._hold(self.pages, table.view(n, row_pages), lengths, refs, self._dropped, self._record_bytes, self._device, n)
+            if out._dropped is None:
+                out._dropped, counter = fresh, fresh.data_ptr()
         elif (out.pages.data_ptr() != self.pages.data_ptr() or out.pages.shape != self.pages.shape
               or out.pages.dtype != self.pages.dtype or out.table.shape != (n, row_pages)):
             raise ValueError("out must be over the same pages, with a row for every parent")
-        capi.check(capi.load().carlb_history_fork(self._view, out._view, p.data_ptr(), self._stream()))
+        capi.check(capi.load().carlb_history_fork(self._view, out._view, p.data_ptr(), counter, self._stream()))
         return out
 
     def append(self, records: torch.Tensor, mask: torch.Tensor | None = None) -> None:

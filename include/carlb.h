@@ -440,9 +440,10 @@ typedef struct carlb_history {
  * outside [0, from->n_rows) gives an empty row); the pages are shared, not copied,
  * and to->refs counts what to->table names.  Both name the same pages; table,
  * lengths and refs of `to` must not overlap those of `from`, which is void once
- * `to` is appended to. */
+ * `to` is appended to.  *dropped is set to 0 unless NULL (the counter of a history
+ * that has none yet). */
 carlb_status carlb_history_fork(const carlb_history* from, const carlb_history* to, const int64_t* parents,
-                                void* stream);
+                                int32_t* dropped, void* stream);
 
 /* Workspace bytes of carlb_history_append and carlb_history_compact. */
 carlb_status carlb_history_workspace(const carlb_history* h, int64_t* append_bytes, int64_t* compact_bytes);

@@ -34,8 +34,8 @@ def test_history_refuses_before_launch(lib, bad, needle):
     h = _view(**bad)
     calls = [lambda: lib.carlb_history_append(h, 64, 8, None, 64, 64, 1 << 40, None),
              lambda: lib.carlb_history_free(h, 64, None), lambda: lib.carlb_history_compact(h, 64, 64, 1 << 40, None),
-             lambda: lib.carlb_history_read(h, None, 4, 3, 64, 64, None), lambda: lib.carlb_history_fork(h, _view(), 64, None),
-             lambda: lib.carlb_history_fork(_view(), h, 64, None)]
+             lambda: lib.carlb_history_read(h, None, 4, 3, 64, 64, None), lambda: lib.carlb_history_fork(h, _view(), 64, None, None),
+             lambda: lib.carlb_history_fork(_view(), h, 64, None, None)]
     for call in calls:
         assert call() == capi.ERR_VALUE
         assert needle in lib.carlb_last_error(None).decode()
@@ -43,10 +43,10 @@ def test_history_refuses_before_launch(lib, bad, needle):
 
 def test_history_refuses_arguments(lib):
     h = _view()
-    assert lib.carlb_history_fork(h, _view(), 64, None) == capi.ERR_VALUE
+    assert lib.carlb_history_fork(h, _view(), 64, None, None) == capi.ERR_VALUE
     assert "overlap" in lib.carlb_last_error(None).decode()
-    assert lib.carlb_history_fork(h, _view(table=128, lengths=128, refs=128, page_len=2), 64, None) == capi.ERR_VALUE
-    assert lib.carlb_history_fork(h, _view(table=128, lengths=128, refs=128), None, None) == capi.ERR_VALUE
+    assert lib.carlb_history_fork(h, _view(table=128, lengths=128, refs=128, page_len=2), 64, None, None) == capi.ERR_VALUE
+    assert lib.carlb_history_fork(h, _view(table=128, lengths=128, refs=128), None, None, None) == capi.ERR_VALUE
     assert lib.carlb_history_append(h, None, 8, None, 64, 64, 1 << 40, None) == capi.ERR_VALUE
     assert lib.carlb_history_append(h, 64, -8, None, 64, 64, 1 << 40, None) == capi.ERR_VALUE
     assert lib.carlb_history_append(h, 64, 8, None, 64, 64, 1, None) == capi.ERR_VALUE
@@ -95,7 +95,8 @@ def _mirror(h):
 GEOMETRIES = [  # rows, row_pages, pages, page_len, record shape, dtype
     (1, 1, 1, 1, (), "float32"), (3, 2, 5, 1, (3,), "int32"), (8, 3, 20, 4, (7,), "float16"), (12, 4, 30, 3, (2, 5), "uint8"),
     (40, 3, 100, 8, (64,), "float32"), (600, 3, 1500, 2, (4,), "int64"), (2500, 2, 3500, 3, (1,), "float16"),
-    (16, 40, 200, 5, (252,), "float32"), (5, 2, 0, 4, (3,), "float32"),
+    (16, 40, 200, 5, (252,), "float32"), (5, 2, 0, 4, (3,), "float32"), (1100, 3, 3300, 9, (300,), "float32"),
+    (30, 2, 80, 7, (1500,), "float32"), (4, 600, 2300, 1, (2,), "float16"),
 ]
 
 
