@@ -57,34 +57,31 @@ class PagedHistory:
         for name, t in (("pages", pages), ("table", table), ("lengths", lengths), ("refs", refs)):
             if not isinstance(t, torch.Tensor):
                 raise TypeError(f"{name} must be a tensor")
-            if name != "pages" and t.dtype != torch.int32:
+        device, shape, rows = pages.device, pages.shape, table.shape
+        for name, t in (("table", table), ("lengths", lengths), ("refs", refs)):
+            if t.dtype is not torch.int32:
                 raise TypeError(f"{name} must have dtype int32")
         for name, t in (("pages", pages), ("table", table), ("lengths", lengths), ("refs", refs)):
-            if t.device.type != "cuda":
+            if not t.is_cuda:
                 raise ValueError(f"{name} must be on a CUDA device")
-            if t.device != pages.device:
-                raise ValueError(f"{name} must be on {pages.device}")
+            if t.device != device:
+                raise ValueError(f"{name} must be on {device}")
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
         if pages.requires_grad:
             raise ValueError("pages must not require a gradient")
-        if pages.dim() < 2 or pages.shape[1] < 1 or 0 in pages.shape[2:]:
+        if len(shape) < 2 or 0 in shape[1:]:
             raise ValueError("pages must have shape [n_pages, page_len, *record] without empty dimensions")
-        if table.dim() != 2 or table.shape[1] < 1 or lengths.shape != table.shape[:1] or refs.shape != pages.shape[:1]:
+        if len(rows) != 2 or rows[1] < 1 or lengths.shape != rows[:1] or refs.shape != shape[:1]:
             raise ValueError("table must be [n_rows, row_pages], lengths [n_rows] and refs [n_pages]")
-        if table.shape[1] * pages.shape[1] > 0x7fffffff or max(pages.shape[0], table.shape[0]) > 0x7fffffff:
+        if rows[1] * shape[1] > 0x7fffffff or max(shape[0], rows[0]) > 0x7fffffff:
             raise ValueError("too many rows, pages or records of a row")
         record_bytes = pages.element_size()
-        for n in pages.shape[2:]:
+        for n in shape[2:]:
             record_bytes *= n
-        self._hold(pages, table, lengths, refs, dropped, record_bytes, pages.device, table.shape[0])
-
-    def _hold(self, pages, table, lengths, refs, dropped, record_bytes: int, device, n_rows: int) -> None:
-        self.pages, self.table, self.lengths, self.refs, self._dropped = pages, table, lengths, refs, dropped
-        self._device, self._record_bytes = device, record_bytes
-        shape = pages.shape
+        self._pages, self._books, self._dropped, self._device = pages, (table, lengths, refs), dropped, device
         self._view = capi.History(pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), record_bytes,
-                                  n_rows, table.shape[1], shape[0], shape[1], device.index)
+                                  rows[0], rows[1], shape[0], shape[1], device.index)
 
     @classmethod
     def empty(cls, n_rows: int, row_pages: int, n_pages: int, page_len: int, record_shape: tuple = (),
@@ -100,20 +97,45 @@ class PagedHistory:
                    torch.zeros(n_pages, dtype=torch.int32, device=device))
 
     @property
+    def pages(self) -> torch.Tensor:
+        return self._pages
+
+    def _book(self, which: int) -> torch.Tensor:
+        # A fork keeps its books in one tensor and parts them when they are looked at.
+        if not isinstance(self._books, tuple):
+            v = self._view
+            entries = v.n_rows * v.row_pages
+            table, lengths, refs, _ = self._books.split((entries, v.n_rows, v.n_pages, 1))
+            self._books = table.view(v.n_rows, v.row_pages), lengths, refs
+        return self._books[which]
+
+    @property
+    def table(self) -> torch.Tensor:
+        return self._book(0)
+
+    @property
+    def lengths(self) -> torch.Tensor:
+        return self._book(1)
+
+    @property
+    def refs(self) -> torch.Tensor:
+        return self._book(2)
+
+    @property
     def record_shape(self) -> tuple[int, ...]:
-        return tuple(self.pages.shape[2:])
+        return tuple(self._pages.shape[2:])
 
     @property
     def n_rows(self) -> int:
-        return self.table.shape[0]
+        return self._view.n_rows
 
     @property
     def n_pages(self) -> int:
-        return self.pages.shape[0]
+        return self._view.n_pages
 
     @property
     def page_len(self) -> int:
-        return self.pages.shape[1]
+        return self._view.page_len
 
     @property
     def dropped(self) -> torch.Tensor:
@@ -129,7 +151,7 @@ class PagedHistory:
             raise TypeError(f"{name} must be a bool tensor")
         if mask.device != self._device:
             raise ValueError(f"{name} must be on {self._device}")
-        if mask.shape != self.lengths.shape:
+        if mask.shape != (self._view.n_rows,):
             raise ValueError(f"{name} must have shape [n_rows]")
         return mask if mask.is_contiguous() else mask.contiguous()
 
@@ -152,21 +174,24 @@ class PagedHistory:
         over the same pages with a table, lengths and refs of its own (two histories
         used in turn, for instance by captured graphs)."""
         p = self._indices(parents, "parents")
-        counter = None
-        n, row_pages, n_pages = p.numel(), self.table.shape[1], self.pages.shape[0]
+        v, n, counter = self._view, p.numel(), None
         if out is None:
             if n > 0x7fffffff:
                 raise ValueError("too many rows, pages or records of a row")
-            table, lengths, refs, fresh = torch.empty(
-                n * row_pages + n + n_pages + 1, dtype=torch.int32, device=self._device).split((n * row_pages, n, n_pages, 1))
+            entries = n * v.row_pages
+            book = torch.empty(entries + n + v.n_pages + 1, dtype=torch.int32, device=self._device)
             out = PagedHistory.__new__(PagedHistory)
-            out._hold(self.pages, table.view(n, row_pages), lengths, refs, self._dropped, self._record_bytes, self._device, n)
+            out._pages, out._books, out._dropped, out._device = self._pages, book, self._dropped, self._device
+            at = book.data_ptr()
+            lengths = at + 4 * entries
+            refs = lengths + 4 * n
+            out._view = capi.History(v.pages, at, lengths, refs, v.record_bytes, n, v.row_pages, v.n_pages, v.page_len, v.device)
             if out._dropped is None:
-                out._dropped, counter = fresh, fresh.data_ptr()
-        elif (out.pages.data_ptr() != self.pages.data_ptr() or out.pages.shape != self.pages.shape
-              or out.pages.dtype != self.pages.dtype or out.table.shape != (n, row_pages)):
+                out._dropped, counter = book[-1:], refs + 4 * v.n_pages
+        elif (out._view.pages != v.pages or out._pages.shape != self._pages.shape or out._pages.dtype != self._pages.dtype
+              or (out._view.n_rows, out._view.row_pages) != (n, v.row_pages)):
             raise ValueError("out must be over the same pages, with a row for every parent")
-        capi.check(capi.load().carlb_history_fork(self._view, out._view, p.data_ptr(), counter, self._stream()))
+        capi.check(capi.load().carlb_history_fork(v, out._view, p.data_ptr(), counter, self._stream()))
         return out
 
     def append(self, records: torch.Tensor, mask: torch.Tensor | None = None) -> None:
@@ -177,13 +202,13 @@ class PagedHistory:
         page append, the longest of them (the first of those) writes on in it instead.
         Free pages go lowest first to the rows in order.  A row that finds no free page,
         or has no table entry left, stays as it was and is counted in `dropped`."""
-        if not isinstance(records, torch.Tensor) or records.dtype != self.pages.dtype:
+        if not isinstance(records, torch.Tensor) or records.dtype != self._pages.dtype:
             raise TypeError("records must be a tensor of the pages' dtype")
         if records.device != self._device:
             raise ValueError(f"records must be on {self._device}")
-        shape = records.shape
-        n = self.lengths.shape[0]
-        if len(shape) == 0 or shape[0] != n or shape[1:] != self.pages.shape[2:]:
+        shape, v = records.shape, self._view
+        n = v.n_rows
+        if len(shape) == 0 or shape[0] != n or shape[1:] != self._pages.shape[2:]:
             raise ValueError("records must have shape [n_rows, *record]")
         m = None if mask is None else self._mask(mask, "mask")
         if n == 0:
@@ -191,16 +216,16 @@ class PagedHistory:
         if not records.is_contiguous() and not records[0].is_contiguous():
             records = records.detach().contiguous()
         lib = capi.load()
-        size = _workspaces(n, self._view.row_pages, self._view.n_pages, self._view.page_len)[0]
+        size = _workspaces(n, v.row_pages, v.n_pages, v.page_len)[0]
         work = torch.empty(size, dtype=torch.uint8, device=self._device)
-        capi.check(lib.carlb_history_append(self._view, records.data_ptr(), records.stride(0) * records.element_size(),
+        capi.check(lib.carlb_history_append(v, records.data_ptr(), records.stride(0) * records.element_size(),
                                             None if m is None else m.data_ptr(), self.dropped.data_ptr(),
                                             work.data_ptr(), size, self._stream()))
 
     def free(self, mask: torch.Tensor) -> None:
         """Empties the rows with mask[r]; a page is free when no row names it any more."""
         m = self._mask(mask, "mask")
-        if self.n_rows:
+        if self._view.n_rows:
             capi.check(capi.load().carlb_history_free(self._view, m.data_ptr(), self._stream()))
 
     def compact(self) -> torch.Tensor:
@@ -222,12 +247,12 @@ class PagedHistory:
         if steps < 1:
             raise ValueError("steps must be positive")
         r = None if rows is None else self._indices(rows, "rows")
-        shape = self.lengths.shape if r is None else r.shape
+        shape = torch.Size((self._view.n_rows,)) if r is None else r.shape
         counts = torch.empty(shape, dtype=torch.int32, device=self._device)
         n = counts.numel()
         if n * steps > 1 << 33:
             raise ValueError("too many records")
-        out = torch.empty((*shape, steps, *self.pages.shape[2:]), dtype=self.pages.dtype, device=self._device)
+        out = torch.empty((*shape, steps, *self._pages.shape[2:]), dtype=self._pages.dtype, device=self._device)
         if n:
             capi.check(capi.load().carlb_history_read(self._view, None if r is None else r.data_ptr(), n, steps,
                                                       out.data_ptr(), counts.data_ptr(), self._stream()))
