@@ -668,7 +668,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
             bestAt = c;
         }
     });
-    if (THREADS > 32) sync();
+    sync();
     const unsigned nth = nthLargest<THREADS, E>(best > NEG_INF ? ordered((float)best) : 0u, p.width, tid, sh);
     // Lower by twice NEAR_TOTALS and by eight roundings to float32.
     float bar = nth && nth != 0xffffffffu ? fromOrdered(nth) : NEG_INF;
@@ -693,8 +693,9 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
     // The vectors of all these chunks, shared out over the threads.
     const int chunks = sh.chunks;
     const int per = (min(segVectors, p.vocab / VE) + 31) / 32 + 1;  // vectors of a chunk, and its edge
+    const bool fits = chunks <= Shared::CHUNKS && (long long)chunks * per <= 1 << 30;
     constexpr int VECTORS = THREADS == 32 ? 3 : 2;
-    for (int i0 = tid; chunks <= Shared::CHUNKS && i0 < chunks * per; i0 += VECTORS * THREADS)
+    for (int i0 = tid; fits && i0 < chunks * per; i0 += VECTORS * THREADS)
     {
         uint4 r[VECTORS];
         unsigned legal[VECTORS];
@@ -751,7 +752,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
         }
     }
     sync();
-    const bool every = chunks > Shared::CHUNKS || sh.candidates > Shared::CANDIDATES;
+    const bool every = !fits || sh.candidates > Shared::CANDIDATES;
     const int n = every ? K * p.vocab : sh.candidates;
 
     // Marks beams whose totals are too near one another's, and computes the marked beams'

@@ -49,7 +49,9 @@ class PagedHistory:
     refs     int32 [n_pages]: how many table entries name the page; 0 = free
 
     The constructor wraps tensors that already hold a history; `empty` makes a new one.
-    `dropped` (int32 [1]) counts the records that `append` found no place for.
+    `dropped` (int32 [1]) counts the records that `append` found no place for; forks go on
+    with it.  A constructor that is given none makes it with the first append, or fork, or
+    look: one of these before a capture keeps it out of the graph.
     """
 
     def __init__(self, pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
@@ -94,7 +96,8 @@ class PagedHistory:
         return cls(torch.zeros((n_pages, page_len, *record_shape), dtype=dtype, device=device),
                    torch.full((n_rows, row_pages), -1, dtype=torch.int32, device=device),
                    torch.zeros(n_rows, dtype=torch.int32, device=device),
-                   torch.zeros(n_pages, dtype=torch.int32, device=device))
+                   torch.zeros(n_pages, dtype=torch.int32, device=device),
+                   torch.zeros(1, dtype=torch.int32, device=device))
 
     @property
     def pages(self) -> torch.Tensor:
@@ -215,6 +218,8 @@ class PagedHistory:
             return
         if not records.is_contiguous() and not records[0].is_contiguous():
             records = records.detach().contiguous()
+        elif v.pages is not None and v.pages <= records.data_ptr() < v.pages + v.record_bytes * v.page_len * v.n_pages:
+            records = records.clone()  # records of this history: their pages are written to
         lib = capi.load()
         size = _workspaces(n, v.row_pages, v.n_pages, v.page_len)[0]
         work = torch.empty(size, dtype=torch.uint8, device=self._device)

@@ -169,7 +169,7 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, dim: i
 
     Row g * beams + j takes the content that row g * beams + parents[g, j] had; a value
     outside [0, beams) leaves its row as it is.  The tensors must not overlap one
-    another.  Up to 1024 beams.
+    another or parents.  Up to 1024 beams.
     """
     if isinstance(states, torch.Tensor):
         raise TypeError("states must be a sequence of tensors")
@@ -182,6 +182,9 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, dim: i
     device, rows, beams, count = parents.device, parents.numel(), parents.shape[-1], len(states)
     grad = torch.is_grad_enabled()
     arrays = (capi.StateArray * max(1, count))()
+    p = parents if parents.is_contiguous() else parents.contiguous()
+    at = p.data_ptr()
+    spans = [(at, at + 8 * rows)]
     for i, t in enumerate(states):
         if not isinstance(t, torch.Tensor):
             raise TypeError("states must be tensors")
@@ -203,9 +206,13 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, dim: i
         outer = 1
         for n in shape[:d]:
             outer *= n
-        arrays[i] = (t.data_ptr(), outer, total // outer, total // outer // rows)
+        at = t.data_ptr()
+        arrays[i] = (at, outer, total // outer, total // outer // rows)
+        spans.append((at, at + total))
     if rows == 0 or not count:
         return
-    p = parents if parents.is_contiguous() else parents.contiguous()
+    spans.sort()
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("states must not overlap one another or parents")
     capi.check(capi.load().carlb_reorder_states(arrays, count, p.data_ptr(), rows // beams, beams, device.index,
                                                 capi.current_stream(device.index)))

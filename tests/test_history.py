@@ -233,6 +233,10 @@ def test_records_by_stride_and_refusals():
         h.append(rec)
         ref.append(rec.detach().cpu().numpy())
         _same(h, ref)
+    rec = h.pages[2:6, 0]                               # records of the history's own pages
+    ref.append(rec.cpu().numpy())
+    h.append(rec)
+    _same(h, ref)
     rec = wide.detach()[:, :6]
     for exc, call in [(TypeError, lambda: h.append(rec.half())), (ValueError, lambda: h.append(rec[:3])),
                       (ValueError, lambda: h.append(rec.cpu())), (TypeError, lambda: h.append(rec, rec[:, 0])),

@@ -398,6 +398,10 @@ def test_reorder_many_arrays_and_neighbours():
         assert torch.equal(t[1:21], _reordered(b[1:21], parents, 0))
     reorder_states([], parents)
     reorder_states([torch.zeros(0, 4, device="cuda")], parents[:0])
+    with pytest.raises(ValueError, match="overlap"):
+        reorder_states([store[0][:20], store[1][1:21], store[0][1:21]], parents)
+    with pytest.raises(ValueError, match="overlap"):
+        reorder_states([parents.view(20)], parents)
     with pytest.raises(ValueError):
         reorder_states([store[0]], parents)                      # 22 rows
     with pytest.raises(ValueError):
