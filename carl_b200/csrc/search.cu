@@ -753,7 +753,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
     }
     sync();
     const bool every = !fits || sh.candidates > Shared::CANDIDATES;
-    const int n = every ? K * p.vocab : sh.candidates;
+    const int n = every ? 0x7fffffff : sh.candidates;
 
     // Marks beams whose totals are too near one another's, and computes the marked beams'
     // normalisers in 64 bits, in an order that depends on nothing but the actions.
@@ -859,34 +859,68 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
         return;
     }
 
-    // Candidate c: its total, beam and index; -inf for none.
-    auto totalOf = [&](int c, int& beam, unsigned& index) {
-        if (!every)
+    // Every element, chunk by chunk: a warp leaves out the chunks whose largest total, at
+    // the lowest index it could have, would come behind its list's last place.  Rows of
+    // equal logits so end after the chunks that hold their first few.
+    const auto pushAll = [&](BestList<GroupKey, E>& list) {
+        int k = warp / segs, seg = warp - k * segs;
+        for (int i = warp; i < items; i += Shared::WARPS)
         {
-            index = sh.found[c].index;
-            beam = sh.found[c].beam;
-            return sh.found[c].total;
+            const double b = base[k];
+            const Row<T> row(p, g, k, lane);
+            const int begin = THREADS == 32 ? 0 : seg * segVectors, end = min(row.vectors, begin + segVectors);
+            const float top = b > NEG_INF ? chunkTop(i * 32 + lane) : NEG_INF;
+            const GroupKey most{ ordered64(b + (double)top),
+                                 ~((unsigned)k * p.vocab + row.head + min(begin + lane, row.vectors) * VE) };
+            const GroupKey edgeMost{ most.t, ~((unsigned)k * p.vocab + lane) };  // a lane in front of the vectors
+            const GroupKey& bound = begin == 0 && lane < row.head ? edgeMost : most;
+            unsigned left = FULL;
+            while ((left &= __ballot_sync(FULL, top > NEG_INF && better(bound, list.bar))) != 0)
+            {
+                const int l = __ffs(left) - 1;
+                left &= left - 1;
+                const int elements = max(0, (end - begin - l + 31) / 32) * VE;
+                for (int e0 = 0; e0 < elements; e0 += 32)
+                {
+                    const int e = e0 + lane, action = row.head + (begin + l + e / VE * 32) * VE + e % VE;
+                    GroupKey key{};
+                    if (e < elements && (!row.allowed || row.allowed[action]))
+                    {
+                        const float x = toFloat(row.x[action]);
+                        if (x > NEG_INF) key = GroupKey{ ordered64(b + (double)x), ~((unsigned)k * p.vocab + action) };
+                    }
+                    list.push(key.t && better(key, list.bar), key);
+                }
+                float x = NEG_INF;
+                const int action = begin == 0 && lane == l ? row.edge(x) : -1;
+                const GroupKey key{ ordered64(b + (double)x), ~((unsigned)k * p.vocab + action) };
+                list.push(x > NEG_INF && better(key, list.bar), key);
+            }
+            k += stepBeams;
+            seg += stepSegs;
+            if (seg >= segs)
+            {
+                seg -= segs;
+                k++;
+            }
         }
-        index = c;
-        beam = c / p.vocab;
-        const int action = c - beam * p.vocab;
-        if (p.finished && p.finished[row0 + beam])
-            return action == 0 ? (double)p.scores[row0 + beam] : (double)NEG_INF;
-        if (!(base[beam] > NEG_INF)) return (double)NEG_INF;
-        const uint8_t* allowed = rowMask(p, g, beam);
-        const float x = !allowed || allowed[action] ? toFloat(rowLogits<T>(p, g, beam)[action]) : NEG_INF;
-        return x > NEG_INF ? base[beam] + (double)x : (double)NEG_INF;
+        for (int k0 = warp * 32; p.finished && k0 < K; k0 += THREADS)
+        {
+            const int f = k0 + lane;
+            const double total = f < K ? (double)overOf(f) : (double)NEG_INF;
+            const GroupKey key{ ordered64(total), ~((unsigned)f * p.vocab) };
+            list.push(total > NEG_INF && better(key, list.bar), key);
+        }
     };
-    auto choose = [&]() {
+    const auto choose = [&]() {
         BestList<GroupKey, E> list;
         list.init(sh.wait[warp], p.width, lane);
-        for (int c0 = warp * 32; c0 < n; c0 += THREADS)
+        if (every) pushAll(list);
+        for (int c0 = warp * 32; !every && c0 < n; c0 += THREADS)
         {
-            int beam = 0;
-            unsigned index = 0;
-            const double total = c0 + lane < n ? totalOf(c0 + lane, beam, index) : NEG_INF;
-            const GroupKey key{ ordered64(total), ~index };
-            list.push(total > NEG_INF && better(key, list.bar), key);
+            GroupKey key{};
+            if (c0 + lane < n) key = GroupKey{ ordered64(sh.found[c0 + lane].total), ~sh.found[c0 + lane].index };
+            list.push(key.t && better(key, list.bar), key);
         }
         list.finish();
         __syncwarp();  // the buffer of waiting keys becomes the list
@@ -914,7 +948,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
     for (int i = tid; i + 1 < p.width; i += THREADS)
     {
         const GroupKey a = list[i], b = list[i + 1];
-        if (!b.t || fromOrdered64(a.t) - fromOrdered64(b.t) > NEAR_TOTALS) continue;
+        if (!a.t || !b.t || fromOrdered64(a.t) - fromOrdered64(b.t) > NEAR_TOTALS) continue;
         const int ka = ~a.i / p.vocab, kb = ~b.i / p.vocab;
         if (ka == kb) continue;
         mark(ka);
@@ -922,20 +956,25 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
     }
     const double edge = last.t ? fromOrdered64(last.t) : (double)INFINITY;
     const int kl = ~last.i / p.vocab;
-    for (int c = tid; c < n; c += THREADS)
-    {
-        int beam = 0;
-        unsigned index = 0;
-        const double total = totalOf(c, beam, index);
-        if (beam == kl || !(fabs(total - edge) <= NEAR_TOTALS)) continue;
+    const auto nearEdge = [&](double total, int beam) {
+        if (beam == kl || !(fabs(total - edge) <= NEAR_TOTALS)) return;
         mark(beam);
         mark(kl);
+    };
+    for (int c = tid; !every && c < n; c += THREADS) nearEdge(sh.found[c].total, sh.found[c].beam);
+    if (every && last.t)
+    {
+        // Any beam with a chunk that comes up to the last place may have an element there.
+        eachChunk([&](double total, int c) {
+            if (total > NEG_INF && total >= edge - NEAR_TOTALS) nearEdge(edge, (c >> 5) / segs);
+        });
+        for (int k = tid; p.finished && k < K; k += THREADS) nearEdge((double)overOf(k), k);
     }
     sync();
     if (sh.repair)
     {
         repair();
-        for (int c = tid; c < n && !every; c += THREADS)
+        for (int c = tid; !every && c < n; c += THREADS)
         {
             const Candidate f = sh.found[c];
             if (!marked(f.beam)) continue;

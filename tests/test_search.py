@@ -205,6 +205,27 @@ def test_flat_selection_edge_values(V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("G, K, V, width", [(3, 8, 648, 8), (1300, 3, 700, 16), (2, 5, 30011, 16), (2, 4, 9001, 128),
+                                            (1, 33, 5000, 40), (2, 2, 100003, 64)])
+def test_equal_logits(dtype, G, K, V, width):
+    """Rows that an untrained policy gives: more elements at the bar than there is room for, and the first of them win."""
+    import torch
+
+    x = torch.zeros(G, K, V, dtype=getattr(torch, dtype))
+    s = -torch.arange(G * K, dtype=torch.float32).view(G, K) % 7
+    _check(x, s, None, None, width)
+    m = torch.ones(G, K, V, dtype=torch.bool)
+    m[:, :, : V // 2] = False                        # the first legal action far into the row
+    m[:, 0, 3::5] = True
+    f = torch.zeros(G, K, dtype=torch.bool)
+    f[:, K - 1] = True
+    x[:, :, 1::2] = -0.0
+    x[:, :, 7::11] = 0.5                             # many at two levels
+    _check(x, torch.full((G, K), -1.0), m, f, width) # equal beams: the lower one
+
+
+@pytest.mark.gpu
 def test_near_totals_are_ranked_in_64_bits():
     """Beams whose normalisers differ by less than float32 sums can tell."""
     import torch
