@@ -623,7 +623,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
     if (tid == 0) sh.chunks = sh.candidates = sh.repair = 0;
     // The totals of a thread's chunks (beam k, segment s, its lane), some at a time so that
     // their loads overlap: the best, its place, and the second best.
-    constexpr int AT_ONCE = 4;
+    constexpr int AT_ONCE = THREADS == 32 ? 4 : 8;
     const int stepBeams = Shared::WARPS / segs, stepSegs = Shared::WARPS - stepBeams * segs;
     double best = NEG_INF, second = NEG_INF;
     int bestAt = 0;
@@ -669,10 +669,14 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
         }
     });
     sync();
-    const unsigned nth = nthLargest<THREADS, E>(best > NEG_INF ? ordered((float)best) : 0u, p.width, tid, sh);
-    // Lower by twice NEAR_TOTALS and by eight roundings to float32.
-    float bar = nth && nth != 0xffffffffu ? fromOrdered(nth) : NEG_INF;
-    bar = fabsf(bar) < FLT_MAX ? bar - (2.f * (float)NEAR_TOTALS + 8.f * 0x1p-24f * fabsf(bar)) : NEG_INF;
+    // A bar that `width` elements reach, from a total of each thread that is an element's: lower
+    // than the width-th largest by twice NEAR_TOTALS and by eight roundings to float32.
+    const auto barOf = [&](double mine) {
+        const unsigned nth = nthLargest<THREADS, E>(mine > NEG_INF ? ordered((float)mine) : 0u, p.width, tid, sh);
+        const float b = nth && nth != 0xffffffffu ? fromOrdered(nth) : NEG_INF;
+        return fabsf(b) < FLT_MAX ? b - (2.f * (float)NEAR_TOTALS + 8.f * 0x1p-24f * fabsf(b)) : NEG_INF;
+    };
+    float bar = barOf(best);
 
     const auto offer = [&](double total, unsigned index, int k) {
         if (!(total > NEG_INF && total >= (double)bar)) return;
@@ -684,77 +688,111 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
         const int at = atomicAdd(&sh.chunks, 1);
         if (at < Shared::CHUNKS) sh.chunk[at] = c;
     };
-    if (second > NEG_INF && second >= (double)bar)
-        eachChunk(readAgain);
-    else
-        readAgain(best, bestAt);
-    for (int k = tid; p.finished && k < K; k += THREADS) offer((double)overOf(k), (unsigned)k * p.vocab, k);
-    sync();
-    // The vectors of all these chunks, shared out over the threads.
-    const int chunks = sh.chunks;
     const int per = (min(segVectors, p.vocab / VE) + 31) / 32 + 1;  // vectors of a chunk, and its edge
-    const bool fits = chunks <= Shared::CHUNKS && (long long)chunks * per <= 1 << 30;
-    constexpr int VECTORS = THREADS == 32 ? 3 : 2;
-    for (int i0 = tid; fits && i0 < chunks * per; i0 += VECTORS * THREADS)
-    {
-        uint4 r[VECTORS];
-        unsigned legal[VECTORS];
-        int action[VECTORS], beam[VECTORS];
-#pragma unroll
-        for (int u = 0; u < VECTORS; u++)
+    // The vectors of the noted chunks, shared out over the threads.
+    const auto readChunks = [&](int chunks) {
+        constexpr int VECTORS = THREADS == 32 ? 3 : 4;
+        for (int i0 = tid; i0 < chunks * per; i0 += VECTORS * THREADS)
         {
-            const int i = i0 + u * THREADS;
-            legal[u] = 0;
-            if (i >= chunks * per) continue;
-            const int j = i / per, v = i - j * per, c = sh.chunk[j], k = (c >> 5) / segs, seg = (c >> 5) - k * segs;
-            const Row<T> row(p, g, k, c & 31);
-            const int begin = THREADS == 32 ? 0 : seg * segVectors, at = begin + row.lane + 32 * v;
-            beam[u] = k;
-            if (v == per - 1)
-            {
-                float x;
-                action[u] = begin == 0 ? row.edge(x) : -1;
-                if (action[u] >= 0) offer(base[k] + (double)x, (unsigned)k * p.vocab + action[u], k);
-            }
-            else if (at < row.vectors && at - begin < segVectors)
-            {
-                r[u] = *(reinterpret_cast<const uint4*>(row.x + row.head) + at);
-                action[u] = row.head + at * VE;
-                legal[u] = (1u << VE) - 1;
-                if (row.allowed)
-                {
-                    legal[u] = 0;
+            uint4 r[VECTORS];
+            unsigned legal[VECTORS];
+            int action[VECTORS], beam[VECTORS];
 #pragma unroll
-                    for (int q = 0; q < VE; q++) legal[u] |= row.allowed[action[u] + q] ? 1u << q : 0u;
+            for (int u = 0; u < VECTORS; u++)
+            {
+                const int i = i0 + u * THREADS;
+                legal[u] = 0;
+                if (i >= chunks * per) continue;
+                const int j = i / per, v = i - j * per, c = sh.chunk[j], k = (c >> 5) / segs, seg = (c >> 5) - k * segs;
+                const Row<T> row(p, g, k, c & 31);
+                const int begin = THREADS == 32 ? 0 : seg * segVectors, at = begin + row.lane + 32 * v;
+                beam[u] = k;
+                if (v == per - 1)
+                {
+                    float x;
+                    action[u] = begin == 0 ? row.edge(x) : -1;
+                    if (action[u] >= 0) offer(base[k] + (double)x, (unsigned)k * p.vocab + action[u], k);
+                }
+                else if (at < row.vectors && at - begin < segVectors)
+                {
+                    r[u] = *(reinterpret_cast<const uint4*>(row.x + row.head) + at);
+                    action[u] = row.head + at * VE;
+                    legal[u] = (1u << VE) - 1;
+                    if (row.allowed)
+                    {
+                        legal[u] = 0;
+#pragma unroll
+                        for (int q = 0; q < VE; q++) legal[u] |= row.allowed[action[u] + q] ? 1u << q : 0u;
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < VECTORS; u++)
+            {
+                if (!legal[u]) continue;
+                const double b = base[beam[u]];
+                // Logits that can reach the bar, then those that do.
+                float need = (float)((double)bar - b);
+                need = need > -FLT_MAX ? need - 2.f * 0x1p-24f * fabsf(need) : -FLT_MAX;
+                const unsigned words[4] = { r[u].x, r[u].y, r[u].z, r[u].w };
+                unsigned hits = 0;
+#pragma unroll
+                for (int q = 0; q < VE; q++)
+                    if (Words<T>::at(words[q / Words<T>::PER], q % Words<T>::PER) >= need) hits |= 1u << q;
+                for (hits &= legal[u]; hits; hits &= hits - 1)
+                {
+                    const int q = __ffs(hits) - 1, w = q / Words<T>::PER;
+                    const unsigned word = w == 0 ? words[0] : w == 1 ? words[1] : w == 2 ? words[2] : words[3];
+                    const float x = q % Words<T>::PER ? Words<T>::at(word, 1) : Words<T>::at(word, 0);
+                    offer(b + (double)x, (unsigned)beam[u] * p.vocab + action[u] + q, beam[u]);
                 }
             }
         }
-#pragma unroll
-        for (int u = 0; u < VECTORS; u++)
+    };
+    // Where one beam has most of the best, its few threads' totals make a low bar and too much
+    // reaches it.  What was found then, as far as there was room, gives a higher one (64 groups
+    // of 64 beams over 20000, the 64 best of which are one beam's: 713 us without, 120 with).
+    constexpr int ROUNDS = 6;
+    bool every = false;
+    int n = 0;
+    for (int round = 1;; round++)
+    {
+        if (second > NEG_INF && second >= (double)bar)
+            eachChunk(readAgain);
+        else
+            readAgain(best, bestAt);
+        for (int k = tid; p.finished && k < K; k += THREADS) offer((double)overOf(k), (unsigned)k * p.vocab, k);
+        sync();
+        const int chunks = sh.chunks;
+        const bool fits = chunks <= Shared::CHUNKS && (long long)chunks * per <= 1 << 30;
+        if (fits) readChunks(chunks);
+        sync();
+        n = sh.candidates;
+        if (fits && n <= THREADS) break;
+        double most = NEG_INF;
+        if (fits)
         {
-            if (!legal[u]) continue;
-            const double b = base[beam[u]];
-            // Logits that can reach the bar, then those that do.
-            float need = (float)((double)bar - b);
-            need = need > -FLT_MAX ? need - 2.f * 0x1p-24f * fabsf(need) : -FLT_MAX;
-            const unsigned words[4] = { r[u].x, r[u].y, r[u].z, r[u].w };
-            unsigned hits = 0;
-#pragma unroll
-            for (int q = 0; q < VE; q++)
-                if (Words<T>::at(words[q / Words<T>::PER], q % Words<T>::PER) >= need) hits |= 1u << q;
-            for (hits &= legal[u]; hits; hits &= hits - 1)
+            for (int i = tid; i < min(n, Shared::CANDIDATES); i += THREADS) most = fmax(most, sh.found[i].total);
+        }
+        else
+        {
+            for (int i = tid; i < min(chunks, Shared::CHUNKS); i += THREADS)
             {
-                const int q = __ffs(hits) - 1, w = q / Words<T>::PER;
-                const unsigned word = w == 0 ? words[0] : w == 1 ? words[1] : w == 2 ? words[2] : words[3];
-                const float x = q % Words<T>::PER ? Words<T>::at(word, 1) : Words<T>::at(word, 0);
-                offer(b + (double)x, (unsigned)beam[u] * p.vocab + action[u] + q, beam[u]);
+                const int c = sh.chunk[i];
+                most = fmax(most, base[(c >> 5) / segs] + (double)chunkTop(c));
             }
         }
+        const float higher = barOf(most);
+        if (!(higher > bar) || round == ROUNDS)
+        {
+            every = !fits || n > Shared::CANDIDATES;
+            break;
+        }
+        bar = higher;
+        sync();
+        if (tid == 0) sh.chunks = sh.candidates = 0;
+        sync();
     }
-    sync();
-    const bool every = !fits || sh.candidates > Shared::CANDIDATES;
-    const int n = every ? 0x7fffffff : sh.candidates;
-
     // Marks beams whose totals are too near one another's, and computes the marked beams'
     // normalisers in 64 bits, in an order that depends on nothing but the actions.
     const auto clear = [&] {
@@ -815,7 +853,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
         p.outActions[o] = 0;
     };
 
-    if (n <= THREADS)
+    if (!every && n <= THREADS)
     {
         Candidate mine{ NEG_INF, 0, -1 };
         if (tid < n) mine = sh.found[tid];
@@ -1010,27 +1048,36 @@ __global__ void __launch_bounds__(ROW_THREADS) selectMergeKernel(BeamParams p)
         for (int s = 0; s < segs; s++) t = fmaxf(t, tops[k * segs + s]);
         return t;
     };
-    // A warp per beam, its lanes over the segments.
-    for (int k = threadIdx.x >> 5; k < p.beams; k += ROW_WARPS)
+    // A beam's maximum and sum over its segments, by a thread where they are few, else by a
+    // warp.  What a dead or finished beam left there is not looked at in the end.
+    const bool alone = segs <= 4 || (segs <= 16 && p.beams > 2 * ROW_WARPS);
+    const int lane = threadIdx.x & 31, lanes = alone ? 1 : 32, part = alone ? 0 : lane;
+    for (int k0 = 0; k0 < p.beams; k0 += ROW_THREADS / lanes)
     {
-        const int lane = threadIdx.x & 31;
-        const float score = p.scores[row0 + k];
-        const bool over = p.finished && p.finished[row0 + k];
+        const int k = k0 + threadIdx.x / lanes;
+        const bool on = k < p.beams;
+        const float score = on ? p.scores[row0 + k] : NEG_INF;
+        const bool over = on && p.finished && p.finished[row0 + k];
         float t = NEG_INF;
-        for (int s = lane; s < segs; s += 32) t = fmaxf(t, tops[k * segs + s]);
-        t = fromOrdered(__reduce_max_sync(FULL, ordered(t)));
+#pragma unroll 4
+        for (int s = part; on && s < segs; s += lanes) t = fmaxf(t, tops[k * segs + s]);
+        if (!alone) t = fromOrdered(__reduce_max_sync(FULL, ordered(t)));
         double sum = 0.0;
-        for (int s = lane; s < segs; s += 32)
+#pragma unroll 4
+        for (int s = part; on && s < segs; s += lanes)
         {
             // A segment without a finite logit has sum 0, or NaN where one was NaN.
             const float ts = tops[k * segs + s];
-            const double part = sums[k * segs + s];
-            sum += ts > NEG_INF && ts < t ? part * exp((double)ts - (double)t) : part;
+            const double mine = sums[k * segs + s];
+            sum += ts > NEG_INF && ts < t ? mine * exp((double)ts - (double)t) : mine;
         }
+        if (!alone)
+        {
 #pragma unroll
-        for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
-        // What was not read is not there.
-        if (lane == 0) baseS[k] = score > NEG_INF && !over && t > NEG_INF ? (double)score - ((double)t + log(sum)) : (double)NEG_INF;
+            for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(FULL, sum, m);
+        }
+        if (on && part == 0)
+            baseS[k] = score > NEG_INF && !over && t > NEG_INF ? (double)score - ((double)t + log(sum)) : (double)NEG_INF;
     }
     __syncthreads();
     finishGroup<T, ROW_THREADS, E>(
@@ -1602,7 +1649,11 @@ long long planBeamSelect(BeamParams& p, LogitType type, void* base)
     }
     // Warps the card holds at a time, at the pass's register use.
     constexpr long long WARPS = 148 * 32;
-    p.segs = (int)std::max<long long>(1, std::min<long long>((tiles + 3) / 4, WARPS / std::max<long long>(1, rows)));
+    // At least four tiles to a segment, and at most 256 segments to a group: more of them cost
+    // the block that finishes it more than they save the readers (4 groups of 32 beams over
+    // 131072 in bf16: 42 us without this bound, 33 with 512, 27 with 256, 37 with 128).
+    const long long most = std::min<long long>((tiles + 3) / 4, std::max(1, 256 / p.beams));
+    p.segs = (int)std::max<long long>(1, std::min<long long>(most, WARPS / std::max<long long>(1, rows)));
     const int perVector = type == LOGITS_F32 ? 4 : 8, blocks = (p.vocab / perVector + 31) / 32;
     p.segVectors = std::max(1, (blocks + p.segs - 1) / p.segs) * 32;
     const long long items = rows * p.segs;

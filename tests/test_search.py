@@ -226,6 +226,22 @@ def test_equal_logits(dtype, G, K, V, width):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("G, K, V, width", [(3, 8, 30011, 64), (2, 64, 5000, 128), (5, 16, 648, 16), (2, 2, 9000, 100),
+                                            (1, 12, 70000, 40)])
+def test_one_beam_has_all_the_best(G, K, V, width):
+    """The bar that the threads' maxima make is far too low, and is raised; rows ascend, so that what is found first
+    is the worst."""
+    import torch
+
+    rng = np.random.default_rng(V)
+    x = rng.normal(0, 2, (G, K, V)).astype(np.float32)
+    x[0] = np.sort(x[0], -1)
+    x[0, :, : V // 3] = np.linspace(3, 3.001, V // 3, dtype=np.float32)   # a dense third above most of the rest
+    s = np.tile(-4.0 * np.arange(K, dtype=np.float32), (G, 1))
+    _check(torch.from_numpy(x), torch.from_numpy(s), None, None, width)
+
+
+@pytest.mark.gpu
 def test_near_totals_are_ranked_in_64_bits():
     """Beams whose normalisers differ by less than float32 sums can tell."""
     import torch
