@@ -812,18 +812,25 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
             const uint8_t* allowed = rowMask(p, g, k);
             const double t = (double)topOf(k);
             double sum = 0.0;
-            constexpr int AHEAD = 8;  // independent exponentials hide each other's latency
-            for (int a0 = tid; a0 < p.vocab; a0 += AHEAD * THREADS)
-            {
-                double v[AHEAD];
+            constexpr int AHEAD = 8;  // independent exponentials, the loads of the next ones under way
+            float next[AHEAD];
+            const auto load = [&](int a0) {
 #pragma unroll
                 for (int u = 0; u < AHEAD; u++)
                 {
                     const int a = a0 + u * THREADS;
-                    v[u] = a < p.vocab && (!allowed || allowed[a]) ? (double)toFloat(x[a]) : (double)NEG_INF;
+                    next[u] = a < p.vocab && (!allowed || allowed[a]) ? toFloat(x[a]) : NEG_INF;
                 }
+            };
+            load(tid);
+            for (int a0 = tid; a0 < p.vocab; a0 += AHEAD * THREADS)
+            {
+                double v[AHEAD];
 #pragma unroll
-                for (int u = 0; u < AHEAD; u++) v[u] = exp(v[u] - t);
+                for (int u = 0; u < AHEAD; u++) v[u] = (double)next[u] - t;
+                load(a0 + AHEAD * THREADS);
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++) v[u] = exp(v[u]);
 #pragma unroll
                 for (int u = 0; u < AHEAD; u++) sum += v[u];
             }
