@@ -156,6 +156,7 @@ def _check(x, s, m, f, width, heads=None, fn=None, sum_error=SUM_ERROR):
 @pytest.mark.parametrize("G, K, V, width", [
     (1, 1, 1, 1), (1, 1, 7, 3), (3, 2, 18, 5), (5, 8, 90, 8), (7, 5, 648, 4), (2, 33, 1023, 33), (3, 8, 1025, 64),
     (2, 3, 4099, 128), (1, 8, 50257, 8), (2, 64, 2048, 17), (1, 1024, 33, 128), (300, 4, 31, 4), (2, 2, 131072, 1),
+    (4001, 3, 41, 4), (2000, 2, 130, 16), (650, 2, 8003, 8), (600, 9, 1500, 12),
 ])
 @pytest.mark.parametrize("masked, finished", [(False, False), (True, True)])
 def test_flat_selection(dtype, G, K, V, width, masked, finished):
@@ -260,6 +261,19 @@ def test_near_totals_are_ranked_in_64_bits():
         s2 = s.copy()
         s2[:, 3] = es[:, 0].astype(np.float32)
         _check(torch.from_numpy(x), torch.from_numpy(s2), None, torch.from_numpy(fin), 24)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K, width", [(8, 8), (8, 5), (3, 16), (32, 32), (2, 4)])
+def test_joint_near_totals_are_ranked_in_64_bits(K, width):
+    """Beams whose normalisers differ by 1e-3 to 1e-7: in one choice that hardly counts."""
+    import torch
+
+    rng = np.random.default_rng(17)
+    x = np.tile(rng.normal(0, 2, (40, 1, 18)).astype(np.float32), (1, K, 1))
+    x[:, :, 8] = x[:, :, 6:8].max(-1) - 7 - 8 * rng.random((40, K)).astype(np.float32)
+    x[20:, :, 8] = x[20:, :1, 8]                     # equal beams: ties by index
+    _check(torch.from_numpy(x), torch.full((40, K), -2.0), None, None, width, HEADS, sum_error=JOINT_SUM_ERROR)
 
 
 @pytest.mark.gpu
