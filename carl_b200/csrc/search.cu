@@ -1212,6 +1212,10 @@ __device__ __forceinline__ void settle(JointKey (&l)[N])
 constexpr double NEAR_JOINT = 1e-5;
 
 constexpr int JOINT_THREADS = 128;
+// Blocks of an SM (0: no limit): without these limits the lists of 8 take 72 registers and 49 us where 64
+// take 47 (24576 groups of 8 beams), those of 16 118 and 111 us where 96 take 94 (12288 of 16);
+// lists of 4 and 32 are the faster without one.
+constexpr int jointBlocks(int n) { return n == 8 ? 7 : n == 16 ? 5 : 0; }
 
 // Bound by issue (196608 rows of 18 logits in 24576 groups: 43 us, of which 7 for the few
 // warps that take the 64-bit pass; the bytes alone would take 3.7).  Blocks of 64 threads
@@ -1224,7 +1228,7 @@ constexpr int JOINT_THREADS = 128;
 // Sums of logits are in 64 bits, so they are exact for logits within 29 binades;
 // normalisers are in 32 bits first, and in 64 where two beams' totals are near.
 template <class T, int N>
-__global__ void __launch_bounds__(JOINT_THREADS) jointSelectKernel(BeamParams p, int lanes)
+__global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKernel(BeamParams p, int lanes)
 {
     const int lane = threadIdx.x & 31, K = p.beams;
     const long long warp = (blockIdx.x * (long long)JOINT_THREADS + threadIdx.x) >> 5;
@@ -1236,13 +1240,16 @@ __global__ void __launch_bounds__(JOINT_THREADS) jointSelectKernel(BeamParams p,
     const bool over = on && p.finished && p.finished[row];
     const bool reads = on && !over && score > NEG_INF;
     __shared__ float xS[ACTION_LOGITS][JOINT_THREADS];
+    __shared__ double ownS[N][JOINT_THREADS];
     const auto x = [&](int q) -> float& { return xS[q][threadIdx.x]; };  // a column of the thread's own
+    const auto own = [&](int i) -> double& { return ownS[i][threadIdx.x]; };
     const T* from = rowLogits<T>(p, reads ? g : 0, reads ? k : 0);
     const uint8_t* allowed = rowMask(p, reads ? g : 0, reads ? k : 0);
 #pragma unroll
     for (int q = 0; q < ACTION_LOGITS; q++) x(q) = reads && (!allowed || allowed[q]) ? toFloat(from[q]) : NEG_INF;
 
     JointKey best[N];
+    bool again = false, anyAgain = false;  // the group's second pass, and the warp's
     for (int pass = 0; pass < 2; pass++)
     {
         // The normaliser (NaN or +inf among the logits makes it NaN, an empty head -inf),
@@ -1320,59 +1327,69 @@ __global__ void __launch_bounds__(JOINT_THREADS) jointSelectKernel(BeamParams p,
         }
         if (over) best[0] = JointKey{ score > NEG_INF ? (double)score : (double)NEG_INF, k * JOINT_ACTIONS };
 
-        // The group's: every lane of it ends with the same list.  `out` is the best that
-        // another beam lost its place with.
-        JointKey out{ NEG_INF, 0 };
+        // The group's: every lane of it ends with the same list.  A beam's own totals stay in
+        // shared memory, to tell what it has left behind the last place.
+        if (pass == 0)
+        {
+#pragma unroll
+            for (int i = 0; i < N; i++) own(i) = best[i].v;
+        }
         for (int m = 1; m < lanes; m *= 2)
         {
             JointKey other[N];
 #pragma unroll
             for (int i = 0; i < N; i++)
                 other[i] = JointKey{ __shfl_xor_sync(FULL, best[N - 1 - i].v, m), __shfl_xor_sync(FULL, best[N - 1 - i].i, m) };
-            JointKey lost{ NEG_INF, 0 };
+#pragma unroll
+            for (int i = 0; i < N; i++) best[i] = pick(ahead(other[i], best[i]), other[i], best[i]);
+            settle(best);
+        }
+        // Two kept places in a row of different beams, or the last one and the best that another
+        // beam has left, may be in the wrong order if they are near.  Any other two of different
+        // beams that are near have such a pair between them.
+        if (pass == 0)
+        {
+            bool near = false;
+            int kept = 0;  // of this beam
+            JointKey last = best[0];
 #pragma unroll
             for (int i = 0; i < N; i++)
             {
-                const bool take = ahead(other[i], best[i]);
-                const JointKey drop = pick(take, best[i], other[i]);
-                best[i] = pick(take, other[i], best[i]);
-                lost = pick(drop.v > lost.v, drop, lost);
+                if (i >= p.width) continue;
+                if (i > 0)
+                    near |= last.v - best[i].v <= NEAR_JOINT && best[i].v > NEG_INF
+                            && last.i / JOINT_ACTIONS != best[i].i / JOINT_ACTIONS;
+                last = best[i];
+                kept += last.i / JOINT_ACTIONS == k;
             }
-            settle(best);
-            const JointKey theirs{ __shfl_xor_sync(FULL, out.v, m), __shfl_xor_sync(FULL, out.i, m) };
-            out = pick(theirs.v > out.v, theirs, out);
-            out = pick(lost.v > out.v, lost, out);
+            const double left = kept < N ? own(kept) : (double)NEG_INF;
+            near |= last.v - left <= NEAR_JOINT && left > NEG_INF && last.i / JOINT_ACTIONS != k;
+            const unsigned votes = __ballot_sync(FULL, near), group = (lanes < 32 ? (1u << lanes) - 1 : FULL) << (lane - k);
+            again = votes & group;
+            anyAgain = votes != 0;
         }
-        if (pass == 1) break;
-        bool near = false;
-#pragma unroll
-        for (int i = 0; i < N; i++)
+        // A group's result does not depend on whether others beside it need the second pass.
+        if (g < p.groups && again == (pass == 1))
         {
-            if (i >= p.width) continue;
-            const bool edge = i + 1 >= N;
-            const JointKey next = edge ? out : best[i + 1 < N ? i + 1 : i];
-            near |= best[i].v - next.v <= NEAR_JOINT && next.v > NEG_INF && best[i].i / JOINT_ACTIONS != next.i / JOINT_ACTIONS;
-        }
-        if (!__any_sync(FULL, near)) break;
-    }
-
-    if (g >= p.groups) return;
 #pragma unroll
-    for (int i = 0; i < N; i++)
-    {
-        if (i >= p.width || (i & (lanes - 1)) != k) continue;
-        const bool some = best[i].v > NEG_INF;
-        const long long o = g * p.width + i;
-        const int beam = best[i].i / JOINT_ACTIONS;
-        p.outScores[o] = (float)best[i].v;
-        p.outParents[o] = some ? beam : i % K;
-        int rest = some ? best[i].i - beam * JOINT_ACTIONS : 0;
+            for (int i = 0; i < N; i++)
+            {
+                if (i >= p.width || (i & (lanes - 1)) != k) continue;
+                const bool some = best[i].v > NEG_INF;
+                const long long o = g * p.width + i;
+                const int beam = best[i].i / JOINT_ACTIONS;
+                p.outScores[o] = (float)best[i].v;
+                p.outParents[o] = some ? beam : i % K;
+                int rest = some ? best[i].i - beam * JOINT_ACTIONS : 0;
 #pragma unroll
-        for (int h = HEADS - 1; h >= 0; h--)
-        {
-            p.outActions[o * HEADS + h] = rest % headSize(h);
-            rest /= headSize(h);
+                for (int h = HEADS - 1; h >= 0; h--)
+                {
+                    p.outActions[o * HEADS + h] = rest % headSize(h);
+                    rest /= headSize(h);
+                }
+            }
         }
+        if (!anyAgain) break;
     }
 }
 

@@ -276,6 +276,72 @@ def test_joint_near_totals_are_ranked_in_64_bits(K, width):
     _check(torch.from_numpy(x), torch.full((40, K), -2.0), None, None, width, HEADS, sum_error=JOINT_SUM_ERROR)
 
 
+def _check_beside_rounding(x, s, width):
+    """The joint selection where scores and logits of two beams may differ and their totals be the same real number
+    (score -2 and a sum of 3, score -3 and a sum of 4, equal normalisers): which of these comes first is then a matter
+    of how each side rounds.  Whole logits are at most 2 and scores 3, so a normaliser, a base and a total are below 32
+    and round by at most 2^-49 each; seven tops and logarithms added up, the base and the total make 16 roundings a
+    side, 2.9e-14, and two totals on two sides 1.2e-13.  A beam's own continuations have exact sums and keep their order."""
+    from carl_b200.action import CARLActionCodec
+
+    ROUNDING = 1.2e-13
+    G, K, _ = x.shape
+    best = CARLActionCodec().beam_select(x.cuda(), s.cuda(), width=width)
+    x, s = x.double().numpy(), s.double().numpy()
+    sums, norm, at = np.zeros((G, K, 1)), 0.0, 0
+    for h in HEADS:
+        row = x[..., at:at + h]
+        top = row.max(-1, keepdims=True)
+        norm = norm + top[..., 0] + np.log(np.exp(row - top).sum(-1))
+        sums = (sums[..., None] + row[:, :, None, :]).reshape(G, K, -1)
+        at += h
+    totals = (s - norm)[..., None] + sums
+    want = -np.sort(-totals.reshape(G, -1), -1)[:, :width]
+    parents = best.parents.cpu().numpy()
+    actions = np.ravel_multi_index(tuple(np.moveaxis(best.actions.cpu().numpy(), -1, 0)), HEADS)
+    got = totals[np.arange(G)[:, None], parents, actions]
+    assert (np.abs(got - want) <= ROUNDING).all()
+    assert (np.abs(best.scores.cpu().double().numpy() - want) <= JOINT_SUM_ERROR + ROUNDING + 2.0 ** -24 * np.abs(want)).all()
+    order = np.argsort(-totals, -1, kind="stable")           # a beam's continuations are taken in order
+    for g in range(G):
+        for k in np.unique(parents[g]):
+            taken = actions[g][parents[g] == k]
+            assert (taken == order[g, k, :taken.size]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("K", [2, 3, 8, 32])
+@pytest.mark.parametrize("width", [1, 2, 3, 5, 8, 16, 32])
+def test_joint_near_totals_behind_ties(dtype, K, width):
+    """Whole logits tie within a beam, so that the first near total of another beam may lie far behind the last place;
+    the normalisers differ in one choice that hardly counts, down to less than float32 sums can tell."""
+    import torch
+
+    rng = np.random.default_rng(100 * K + width)
+    G = 300
+    x = np.tile(rng.integers(-1, 3, (G, 1, 18)).astype(np.float32), (1, K, 1))
+    x[:, :, 8] = x[:, :, 6:8].max(-1) - 9 - 7 * rng.random((G, K)).astype(np.float32)   # e^-9 .. e^-16 of the head's sum
+    x[200:, :, 17] = x[200:, :, 16] - 9 - 7 * rng.random((100, K)).astype(np.float32)
+    x = torch.from_numpy(x).to(getattr(torch, dtype))
+    s = torch.full((G, K), -2.0)
+    s[100:] -= torch.from_numpy(rng.integers(0, 2, (200, K)).astype(np.float32))   # some beams a whole step behind
+    _check_beside_rounding(x, s, width)
+
+
+@pytest.mark.gpu
+def test_joint_groups_do_not_depend_on_their_neighbours():
+    """A group whose totals are near is ranked again; the scores of the others in its warp keep their bits."""
+    import torch
+    from carl_b200.action import CARLActionCodec
+
+    x, s, _, _ = _inputs(64, 4, 18, "float32", False, False, 8)
+    alone = CARLActionCodec().beam_select(x.cuda(), s.cuda())
+    x[::2], s[::2] = x[::2, :1].clone(), -1.0        # equal beams: all near
+    mixed = CARLActionCodec().beam_select(x.cuda(), s.cuda())
+    assert torch.equal(alone.scores[1::2], mixed.scores[1::2]) and torch.equal(alone.actions[1::2], mixed.actions[1::2])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 def test_joint_ties_between_heads(dtype):
