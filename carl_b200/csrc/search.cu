@@ -1206,6 +1206,38 @@ __device__ __forceinline__ void settle(JointKey (&l)[N])
         }
 }
 
+// The best of a beam's totals, one after another; the first of equal ones stays in front.
+template <class X, int N>
+__device__ __forceinline__ void bestTotals(const X& x, double base, JointKey (&best)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; i++) best[i] = JointKey{ NEG_INF, 0 };
+#pragma unroll 1
+    for (int a = 0; a < JOINT_ACTIONS; a++)
+    {
+        int digit[HEADS], rest = a;
+#pragma unroll
+        for (int h = HEADS - 1; h >= 0; h--)
+        {
+            digit[h] = rest % headSize(h);
+            rest /= headSize(h);
+        }
+        double sum = 0.0;
+        int at = 0;
+#pragma unroll
+        for (int h = 0; h < HEADS; h++)
+        {
+            sum += (double)x(at + digit[h]);
+            at += headSize(h);
+        }
+        const JointKey key{ base + sum, a };  // NaN (a base of +inf, a sum of -inf) goes before nothing
+        if (!(sum > NEG_INF && key.v > best[N - 1].v)) continue;
+#pragma unroll
+        for (int i = N - 1; i > 0; i--) best[i] = key.v > best[i - 1].v ? best[i - 1] : key.v > best[i].v ? key : best[i];
+        if (key.v > best[0].v) best[0] = key;
+    }
+}
+
 // As for the flat selection, for normalisers over seven heads: per head d averages at
 // most log(3), with two additions (1.1 * 2.25 + 6) u = 8.5 u; six products; and logf's
 // last place of at most 6.5, 8 u.  Together 74 u = 4.5e-6 a beam.
@@ -1225,8 +1257,15 @@ constexpr int jointBlocks(int n) { return n == 8 ? 7 : n == 16 ? 5 : 0; }
 // of two).  The best N joint actions of a beam are found head by head: the list of
 // the best sums so far plus each choice of the next head, merged.  A choice that is
 // the r-th best of its head (from 0) can only continue the first N / (r + 1) sums.
-// Sums of logits are in 64 bits, so they are exact for logits within 29 binades;
-// normalisers are in 32 bits first, and in 64 where two beams' totals are near.
+// Sums of logits are in 64 bits; normalisers are in 32 bits first, and in 64 where two
+// beams' totals are near.
+//
+// Lists of sums are in the order of the totals, equal ones by their action, where sums that
+// differ make totals that do.  A logit is a whole multiple of its last bit's value, and so
+// is a sum of the last bit q of the smallest logit (2^-23 of its binade).  While the sums and
+// the base stay below 2^52 q, sums are exact, differ by q at least and are apart by a unit in
+// the last place of any total.  A beam beyond that (a logit 29 binades below the total, or a
+// score of +inf) has its 648 totals looked through in turn, in the second pass.
 template <class T, int N>
 __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKernel(BeamParams p, int lanes)
 {
@@ -1255,6 +1294,8 @@ __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKern
         // The normaliser (NaN or +inf among the logits makes it NaN, an empty head -inf),
         // and the beam's best joint actions.
         double tops = 0.0, base = NEG_INF;
+        unsigned least = 0xffffffffu;  // image of the smallest logit's size, less one (0 wraps)
+        float most = 0.f;              // largest logit's size
         float product = 1.f;
         double product64 = 1.0;
 #pragma unroll
@@ -1269,6 +1310,12 @@ __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKern
             at += size;
             const float top = fmaxf(fmaxf(v[0], v[1]), v[2]);
             tops += (double)top;
+#pragma unroll
+            for (int q = 0; q < 3; q++)
+            {
+                least = min(least, (__float_as_uint(v[q]) & 0x7fffffffu) - 1);
+                most = fmaxf(most, v[q] > NEG_INF ? fabsf(v[q]) : 0.f);
+            }
             if (pass == 0)
             {
                 float sum = 0.f;
@@ -1319,10 +1366,14 @@ __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKern
         if (tops > NEG_INF)
             base = (double)score - (tops + (pass == 0 ? (double)logf(product) : log(product64)));
         const bool live = reads && base > NEG_INF;
+        // 2^52 q, the exponent's field of q being that of the smallest logit less 23.
+        const double limit = __longlong_as_double((long long)(max((int)(least >> 23), 1) - 98 + 1023) << 52);
+        const bool merges = live && !(fabs(base) + 7.0 * (double)most < limit);
+        if (pass == 1 && merges) bestTotals(x, base, best);
 #pragma unroll
         for (int i = 0; i < N; i++)
         {
-            best[i].v = live ? base + best[i].v : (double)NEG_INF;
+            if (pass == 0 || !merges) best[i].v = live ? base + best[i].v : (double)NEG_INF;
             best[i].i += k * JOINT_ACTIONS;
         }
         if (over) best[0] = JointKey{ score > NEG_INF ? (double)score : (double)NEG_INF, k * JOINT_ACTIONS };
@@ -1349,7 +1400,7 @@ __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKern
         // beams that are near have such a pair between them.
         if (pass == 0)
         {
-            bool near = false;
+            bool near = merges;
             int kept = 0;  // of this beam
             JointKey last = best[0];
 #pragma unroll

@@ -329,6 +329,60 @@ def test_joint_near_totals_behind_ties(dtype, K, width):
     _check_beside_rounding(x, s, width)
 
 
+@pytest.mark.filterwarnings("ignore:invalid value")
+@pytest.mark.gpu
+@pytest.mark.parametrize("K, width", [(1, 1), (1, 8), (1, 32), (2, 4), (3, 16), (8, 8), (32, 32)])
+def test_joint_equal_totals_of_unequal_sums(K, width):
+    """Sums of logits that differ and round to one 64-bit total (or to one sum) go to the lower action: scores that
+    swallow the logits, logits that swallow others, and scores of +inf."""
+    import torch
+
+    rng = np.random.default_rng(10 * K + width)
+    x = rng.normal(0, 2, (40, K, 18)).astype(np.float32)
+    s = -20.0 - 4.0 * rng.random((40, K)).astype(np.float32)
+    s[:5] = -1e30                                    # every total is the score
+    s[5:8, K // 2] = -1e30                           # one beam's are
+    x[8:12] = 0.0
+    x[8:12, :, 17] = 1e-20                           # below the last bit of any total
+    x[12:16] = rng.integers(-1, 2, (4, K, 18))
+    x[12:16, :, 0], x[12:16, :, 4] = 1e-20, -1e-25
+    x[16:20, :, 2], x[16:18, :, 10] = 1e20, -1e20    # the other heads vanish beside it
+    x[20:24] = x[20:24] * 1e-42                      # subnormal logits
+    s[24:27] = np.inf
+    s[27:30, K - 1] = np.inf
+    x[24:30, :, [1, 5, 9]] = -np.inf
+    x[30:33, :, 3:6] = 0.0, 1e-20, 2e-20
+    s[33:36] = 0.0
+    x[33:36] = -0.0
+    x[33:36, :, 0] = -3e38
+    x, s = torch.from_numpy(x), torch.from_numpy(s)
+    m = torch.rand(40, K, 18, generator=torch.Generator().manual_seed(K)) < 0.9
+    m[33:36] = True                                  # equal beams: their normalisers too
+    for mask in (None, m):
+        best = _check(x, s, mask, None, width, HEADS, sum_error=JOINT_SUM_ERROR)
+        got = best.scores.cpu()
+        assert not torch.isnan(got).any() and not (got[:24] == math.inf).any() and not (got[30:] == math.inf).any()
+        if mask is None:
+            assert (got[24:30, 0] == math.inf).all()
+
+
+@pytest.mark.filterwarnings("ignore:invalid value")
+@pytest.mark.gpu
+def test_flat_scores_of_infinity():
+    """A beam whose score is +inf wins with every action it has, in their order."""
+    import torch
+
+    for V, width in ((40, 16), (648, 8), (30011, 64), (9001, 100)):
+        x, s, m, _ = _inputs(6, 4, V, "float32", True, False, V)
+        s[:3, 2] = math.inf
+        s[3] = math.inf
+        x[0, 2, 3:], x[1, 2, ::2] = -math.inf, -math.inf
+        m[0, 2, 0] = True
+        best = _check(x, s, m, None, width)
+        got = best.scores.cpu()
+        assert not torch.isnan(got).any() and (got[:4, 0] == math.inf).all()
+
+
 @pytest.mark.gpu
 def test_joint_groups_do_not_depend_on_their_neighbours():
     """A group whose totals are near is ranked again; the scores of the others in its warp keep their bits."""
