@@ -1501,7 +1501,8 @@ __device__ void reorderTile(const ReorderParams& p, const ReorderArray& a, char*
     const int gt = (int)(b % a.groupTiles);
     const long long outer = b / a.groupTiles;
     const int g0 = gt * a.groupsPerTile, ng = min(a.groupsPerTile, p.groups - g0), rows = ng * K;
-    const int rowUnits = (int)(a.inner / sizeof(U)), u0 = ut * a.units, nu = min(a.units, rowUnits - u0);
+    const long long rowUnits = a.inner / (long long)sizeof(U), u0 = (long long)ut * a.units;
+    const int nu = (int)min((long long)a.units, rowUnits - u0);
     for (int r = tid; r < rows; r += REORDER_THREADS) takenS[r] = 0;
     __syncthreads();
     for (int r = tid; r < rows; r += REORDER_THREADS)
@@ -1516,13 +1517,13 @@ __device__ void reorderTile(const ReorderParams& p, const ReorderArray& a, char*
     for (int i = tid; i < rows * nu; i += REORDER_THREADS)
     {
         const int r = i / nu, u = i - r * nu;
-        if (takenS[r]) t[i] = data[(long long)r * rowUnits + u];
+        if (takenS[r]) t[i] = data[r * rowUnits + u];
     }
     __syncthreads();
     for (int i = tid; i < rows * nu; i += REORDER_THREADS)
     {
         const int r = i / nu, u = i - r * nu, s = parentS[r];
-        if (s != r) data[(long long)r * rowUnits + u] = t[s * nu + u];
+        if (s != r) data[r * rowUnits + u] = t[s * nu + u];
     }
 }
 
@@ -1626,7 +1627,7 @@ __global__ void __launch_bounds__(COLUMN_THREADS) reorderRowsKernel(ReorderParam
     const ReorderArray a = arrayOf(p);
     const int tid = threadIdx.x, K = p.beams;
     const long long b = blockIdx.x - a.firstBlock, og = b / a.unitTiles, outer = og / p.groups, g = og - outer * p.groups;
-    const int ut = (int)(b - og * a.unitTiles), columns = (int)(a.inner / 16);
+    const long long columns = a.inner / 16, c0 = (b - og * a.unitTiles) * a.units, c1 = min(columns, c0 + a.units);
     if (tid == 0) takenS = 0;
     __syncthreads();
     if (tid < K)
@@ -1639,18 +1640,18 @@ __global__ void __launch_bounds__(COLUMN_THREADS) reorderRowsKernel(ReorderParam
     const unsigned taken = takenS;
     if (!taken) return;
     uint4* data = reinterpret_cast<uint4*>(a.data + outer * a.outerStride + g * K * a.inner);
-    for (int c = ut * a.units + tid; c < min(columns, (ut + 1) * a.units); c += COLUMN_THREADS)
+    for (long long c = c0 + tid; c < c1; c += COLUMN_THREADS)
     {
         uint4 held[BEAMS];
 #pragma unroll
         for (int k = 0; k < BEAMS; k++)
-            if (taken >> k & 1) held[k] = data[(long long)k * columns + c];
+            if (taken >> k & 1) held[k] = data[k * columns + c];
 #pragma unroll
         for (int k = 0; k < BEAMS; k++)
         {
             if (!(taken >> k & 1)) continue;
             for (int j = 0; j < K; j++)  // the same for the whole block
-                if (parentS[j] == k && j != k) data[(long long)j * columns + c] = held[k];
+                if (parentS[j] == k && j != k) data[j * columns + c] = held[k];
         }
     }
 }

@@ -598,6 +598,30 @@ def test_reorder_beyond_32_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("row, unit", [(2 ** 31 + 17, 1), (2 ** 32 + 2, 2)])
+def test_reorder_rows_of_more_units_than_an_int(row, unit):
+    """Rows of more than 2^31 bytes, or pairs of bytes, that no wider unit divides: every byte moves, none around."""
+    import torch
+    from carl_b200.search import reorder_states
+
+    assert row % (2 * unit) and row // unit > 2 ** 31
+    store = torch.zeros(2 * row + 128, dtype=torch.uint8, device="cuda")
+    t = store[64:64 + 2 * row].view(2, row)
+    at = torch.tensor([0, 1, 16383, 16384, 2 ** 30 + 5, 2 ** 31 - 1, 2 ** 31, row - 18, row - 2, row - 1], device="cuda")
+    t[0] = 1
+    t[1] = 2
+    for k in range(2):
+        t[k, at] = (10 * k + 20 + torch.arange(10, device="cuda")).to(torch.uint8)
+    want = t[:, at].flip(0)
+    reorder_states([t], torch.tensor([[1, 0]], device="cuda"))
+    for k in range(2):
+        assert torch.equal(t[k, at], want[k])
+        t[k, at] = 2 - k
+        assert bool((t[k] == 2 - k).all())
+    assert not store[:64].any() and not store[-64:].any()
+
+
+@pytest.mark.gpu
 def test_env_reorder(tmp_path, monkeypatch):
     """Every persistent field and output buffer of a sim becomes its parent's; copies go on alike."""
     import torch
