@@ -1774,6 +1774,7 @@ void launchJointSelect(const BeamParams& p, LogitType type, cudaStream_t s)
 void launchReorder(const StateArray* arrays, int count, const long long* parents, int groups, int beams, cudaStream_t s)
 {
     enum Form { TILES, RUNS, ROWS, FORMS };
+    constexpr long long MOST_BLOCKS = 0x7fffffff;
     ReorderParams p[FORMS] = {};
     long long blocks[FORMS] = {};
     const auto flush = [&](int f) {
@@ -1802,28 +1803,27 @@ void launchReorder(const StateArray* arrays, int count, const long long* parents
         const StateArray& in = arrays[k];
         if (in.inner == 0 || in.outer == 0) continue;
         ReorderArray a{};
-        a.data = static_cast<char*>(in.data);
-        a.outer = in.outer;
         a.outerStride = in.outerStride;
         a.inner = in.inner;
         const unsigned long long base = reinterpret_cast<uintptr_t>(in.data) | (in.outer > 1 ? (unsigned long long)in.outerStride : 0);
         const unsigned long long bits = base | (unsigned long long)in.inner;
         int form = TILES;
-        long long n = 0;
+        long long slabs = 1, perSlabs = 0;  // blocks of so many slabs
         if (!small && bits % 16 == 0 && in.inner >= 256 && beams <= COLUMN_BEAMS)
         {
             form = ROWS;
             a.units = 4 * COLUMN_THREADS;
             a.unitTiles = (int)((in.inner / 16 + a.units - 1) / a.units);
-            n = in.outer * groups * a.unitTiles;
+            perSlabs = (long long)groups * a.unitTiles;
         }
         else if (!small && base % 16 == 0 && in.inner % 4 == 0 && in.inner / 4 * beams <= RUN_WORDS / 4)
         {
             form = RUNS;
             const int words = (int)(in.inner / 4) * beams;
             a.groupsPerTile = RUN_WORDS / words / 4 * 4;  // tiles start at whole vectors
-            a.groupTiles = (groups + a.groupsPerTile - 1) / a.groupsPerTile;
-            n = (in.outer + RUN_SLABS - 1) / RUN_SLABS * a.groupTiles;
+            a.groupTiles = (int)(((long long)groups + a.groupsPerTile - 1) / a.groupsPerTile);
+            slabs = RUN_SLABS;
+            perSlabs = a.groupTiles;
         }
         else
         {
@@ -1836,17 +1836,25 @@ void launchReorder(const StateArray* arrays, int count, const long long* parents
             if (a.unitTiles == 1)
                 a.groupsPerTile = (int)std::max<long long>(
                     1, std::min<long long>(REORDER_TILE / (beams * in.inner), BEAM_MAX_BEAMS / beams));
-            a.groupTiles = (groups + a.groupsPerTile - 1) / a.groupsPerTile;
-            n = in.outer * a.groupTiles * a.unitTiles;
+            a.groupTiles = (int)(((long long)groups + a.groupsPerTile - 1) / a.groupsPerTile);
+            perSlabs = (long long)a.groupTiles * a.unitTiles;
         }
+        // A launch takes MOST_BLOCKS; an array of more (many small slabs) is split at its slabs.
+        const long long most = std::max(1ll, MOST_BLOCKS / perSlabs) * slabs;
         ReorderParams& q = p[form];
-        if (q.count == REORDER_ARRAYS || blocks[form] + n > 0x7fffffff) flush(form);
-        q.parents = parents;
-        q.groups = groups;
-        q.beams = beams;
-        a.firstBlock = blocks[form];
-        q.a[q.count++] = a;
-        blocks[form] += n;
+        for (long long s0 = 0; s0 < in.outer; s0 += most)
+        {
+            a.data = static_cast<char*>(in.data) + s0 * in.outerStride;
+            a.outer = std::min(most, in.outer - s0);
+            const long long n = (a.outer + slabs - 1) / slabs * perSlabs;
+            if (q.count == REORDER_ARRAYS || blocks[form] + n > MOST_BLOCKS) flush(form);
+            q.parents = parents;
+            q.groups = groups;
+            q.beams = beams;
+            a.firstBlock = blocks[form];
+            q.a[q.count++] = a;
+            blocks[form] += n;
+        }
     }
     for (int f = 0; f < FORMS; f++) flush(f);
 }

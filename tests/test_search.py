@@ -622,6 +622,19 @@ def test_reorder_rows_of_more_units_than_an_int(row, unit):
 
 
 @pytest.mark.gpu
+def test_reorder_more_slabs_than_a_launch_has_blocks():
+    import torch
+    from carl_b200.search import reorder_states
+
+    slabs = 2 ** 31 + 3
+    t = torch.empty(slabs, 2, dtype=torch.uint8, device="cuda")
+    t[:, 0], t[:, 1] = 1, 2
+    other = torch.arange(6, device="cuda").view(3, 2)
+    reorder_states([t, other], torch.tensor([[1, 0]], device="cuda"), dim=1)
+    assert bool((t[:, 0] == 2).all()) and bool((t[:, 1] == 1).all()) and other.tolist() == [[1, 0], [3, 2], [5, 4]]
+
+
+@pytest.mark.gpu
 def test_env_reorder(tmp_path, monkeypatch):
     """Every persistent field and output buffer of a sim becomes its parent's; copies go on alike."""
     import torch
