@@ -374,8 +374,8 @@ __global__ void __launch_bounds__(THREADS) appendWriteKernel(HistoryView h, Appe
     const Job job{ j.x, j.y, j.z, j.w };
     if (job.kind == ROW_IDLE) return;
     const int col = job.length / h.pageLen, slot = job.length - col * h.pageLen;
-    const int s0 = part * perItem, s1 = min(s0 + perItem, slot);
-    const bool own = s0 <= slot && slot < s0 + perItem, copies = job.kind == ROW_COPY && s0 < s1;
+    const int s0 = part * perItem, s1 = s0 + min(perItem, slot - s0);  // s0 + perItem may pass 2^31
+    const bool own = s0 <= slot && slot - s0 < perItem, copies = job.kind == ROW_COPY && s0 < s1;
     if (!own && !copies && part != 0) return;
     int target = job.kind == ROW_IN_PLACE ? job.held : -1;
     if (job.kind == ROW_NEW_PAGE || job.kind == ROW_COPY)
@@ -686,7 +686,7 @@ cudaError_t launchHistoryAppend(const HistoryView& h, const char* records, long 
     const AppendWork w = planAppend(h, workspace, nullptr, &zero);
     const int unit = unitOf(reinterpret_cast<uintptr_t>(h.pages) | reinterpret_cast<uintptr_t>(records)
                             | (unsigned long long)h.recordBytes | (unsigned long long)recordStride);
-    const int perItem = itemRecords(h.recordBytes, h.pageLen), items = (h.pageLen + perItem - 1) / perItem;
+    const int perItem = itemRecords(h.recordBytes, h.pageLen), items = (h.pageLen - 1) / perItem + 1;
     if (h.nRows <= SMALL_ROWS && h.nPages <= SMALL_PAGES && h.nRows * h.recordBytes * h.pageLen <= SMALL_COPY)
     {
         appendSmallKernel<<<1, SMALL_THREADS, 0, s>>>(h, mask, w, records, recordStride, unit, perItem, items, dropped);
@@ -741,7 +741,7 @@ void launchHistoryRead(const HistoryView& h, const long long* rows, int n, int s
     if (n <= 0 || steps <= 0) return;
     const int unit = unitOf(reinterpret_cast<uintptr_t>(h.pages) | reinterpret_cast<uintptr_t>(out)
                             | (unsigned long long)h.recordBytes);
-    const int perItem = itemRecords(h.recordBytes, std::min(32, steps)), items = (steps + perItem - 1) / perItem;
+    const int perItem = itemRecords(h.recordBytes, std::min(32, steps)), items = (steps - 1) / perItem + 1;
     const unsigned n32 = blocks((long long)n * items * 32, THREADS);
     switch (unit)
     {

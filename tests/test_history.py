@@ -271,6 +271,25 @@ def test_pages_beyond_32_bits():
 
 
 @pytest.mark.gpu
+def test_pages_of_nearly_two_to_the_31_records():
+    import torch
+    from carl_b200.history import PagedHistory
+
+    P = 2 ** 31 - 1
+    h = PagedHistory.empty(1, 1, 1, P, (), torch.uint8)              # 2 GB
+    h.append(torch.tensor([5], dtype=torch.uint8, device="cuda"))
+    for last, value in ((P - 4097, 6), (P - 1, 7)):
+        h.lengths[0] = last
+        h.append(torch.tensor([value], dtype=torch.uint8, device="cuda"))
+        assert h.lengths.tolist() == [last + 1]
+        out, counts = h.read(2)
+        assert counts.tolist() == [2] and out.tolist() == [[0, value]]
+    assert h.pages[0, 0] == 5 and h.pages[0, P - 4097] == 6 and h.pages[0, -1] == 7
+    h.append(torch.tensor([8], dtype=torch.uint8, device="cuda"))
+    assert h.lengths.tolist() == [P] and int(h.dropped) == 1 and h.pages[0, -1] == 7
+
+
+@pytest.mark.gpu
 def test_history_in_graphs():
     """Two captured graphs that fork back and forth between two histories, replayed against lists."""
     import torch
