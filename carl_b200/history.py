@@ -163,6 +163,8 @@ class PagedHistory:
             raise TypeError(f"{name} must be an int64 tensor")
         if indices.device != self._device:
             raise ValueError(f"{name} must be on {self._device}")
+        if indices.numel() > 0x7fffffff:
+            raise ValueError(f"too many {name}")
         return indices if indices.is_contiguous() else indices.contiguous()
 
     def fork(self, parents: torch.Tensor, out: PagedHistory | None = None) -> PagedHistory:
@@ -179,8 +181,6 @@ class PagedHistory:
         p = self._indices(parents, "parents")
         v, n, counter = self._view, p.numel(), None
         if out is None:
-            if n > 0x7fffffff:
-                raise ValueError("too many rows, pages or records of a row")
             entries = n * v.row_pages
             book = torch.empty(entries + n + v.n_pages + 1, dtype=torch.int32, device=self._device)
             out = PagedHistory.__new__(PagedHistory)
@@ -255,7 +255,7 @@ class PagedHistory:
         shape = torch.Size((self._view.n_rows,)) if r is None else r.shape
         counts = torch.empty(shape, dtype=torch.int32, device=self._device)
         n = counts.numel()
-        if n * steps > 1 << 33:
+        if n * steps > 1 << 33 or steps > 0x7fffffff:
             raise ValueError("too many records")
         out = torch.empty((*shape, steps, *self._pages.shape[2:]), dtype=self._pages.dtype, device=self._device)
         if n:

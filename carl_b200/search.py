@@ -180,6 +180,8 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, dim: i
     if parents.dim() < 1 or not 1 <= parents.shape[-1] <= capi.BEAM_MAX_BEAMS:
         raise ValueError(f"parents must have shape [..., beams] with 1 to {capi.BEAM_MAX_BEAMS} beams")
     device, rows, beams, count = parents.device, parents.numel(), parents.shape[-1], len(states)
+    if rows // beams > 0x7fffffff:
+        raise ValueError("too many groups")
     grad = torch.is_grad_enabled()
     arrays = (capi.StateArray * max(1, count))()
     p = parents if parents.is_contiguous() else parents.contiguous()

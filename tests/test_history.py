@@ -290,6 +290,22 @@ def test_pages_of_nearly_two_to_the_31_records():
 
 
 @pytest.mark.gpu
+def test_sizes_beyond_32_bits_are_refused():
+    """Counts that the entry points take as int32: the host refuses what would wrap, before it allocates."""
+    import torch
+    from carl_b200.history import PagedHistory
+    from carl_b200.search import reorder_states
+
+    h = PagedHistory.empty(2, 2, 3, 4, (), torch.uint8)
+    many = torch.zeros(1, dtype=torch.int64, device="cuda").expand(2 ** 32 + 2)
+    for call in (lambda: h.read(2 ** 32 + 5, many[:1]), lambda: h.read(2 ** 31, many[:1]), lambda: h.read(1, many),
+                 lambda: h.fork(many), lambda: h.fork(many, out=h),
+                 lambda: reorder_states([torch.zeros(4, device="cuda")], many[:, None])):
+        with pytest.raises(ValueError, match="too many"):
+            call()
+
+
+@pytest.mark.gpu
 def test_history_in_graphs():
     """Two captured graphs that fork back and forth between two histories, replayed against lists."""
     import torch
