@@ -56,14 +56,17 @@ class PagedHistory:
 
     def __init__(self, pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
                  dropped: torch.Tensor | None = None):
-        for name, t in (("pages", pages), ("table", table), ("lengths", lengths), ("refs", refs)):
+        books = [("table", table), ("lengths", lengths), ("refs", refs)]
+        if dropped is not None:
+            books.append(("dropped", dropped))
+        for name, t in (("pages", pages), *books):
             if not isinstance(t, torch.Tensor):
                 raise TypeError(f"{name} must be a tensor")
         device, shape, rows = pages.device, pages.shape, table.shape
-        for name, t in (("table", table), ("lengths", lengths), ("refs", refs)):
+        for name, t in books:
             if t.dtype is not torch.int32:
                 raise TypeError(f"{name} must have dtype int32")
-        for name, t in (("pages", pages), ("table", table), ("lengths", lengths), ("refs", refs)):
+        for name, t in (("pages", pages), *books):
             if not t.is_cuda:
                 raise ValueError(f"{name} must be on a CUDA device")
             if t.device != device:
@@ -76,6 +79,8 @@ class PagedHistory:
             raise ValueError("pages must have shape [n_pages, page_len, *record] without empty dimensions")
         if len(rows) != 2 or rows[1] < 1 or lengths.shape != rows[:1] or refs.shape != shape[:1]:
             raise ValueError("table must be [n_rows, row_pages], lengths [n_rows] and refs [n_pages]")
+        if dropped is not None and dropped.numel() != 1:
+            raise ValueError("dropped must have one element")
         if rows[1] * shape[1] > 0x7fffffff or max(shape[0], rows[0]) > 0x7fffffff:
             raise ValueError("too many rows, pages or records of a row")
         record_bytes = pages.element_size()

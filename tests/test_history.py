@@ -74,6 +74,33 @@ def test_python_refuses_cpu_tensors():
         PagedHistory.empty(4, 0, 8, 4, device="cpu")
 
 
+def test_python_refuses_a_counter_of_another_type():
+    """The counter is written to by its address, as the books are."""
+    import torch
+    from carl_b200.history import PagedHistory
+
+    i32 = dict(dtype=torch.int32)
+    args = torch.zeros(3, 2, 4), torch.zeros(2, 2, **i32), torch.zeros(2, **i32), torch.zeros(3, **i32)
+    for bad in (torch.zeros(1, dtype=torch.int64), torch.zeros(1), 0):
+        with pytest.raises(TypeError, match="dropped"):
+            PagedHistory(*args, bad)
+
+
+@pytest.mark.gpu
+def test_counters_that_cannot_be_written_are_refused():
+    import torch
+    from carl_b200.history import PagedHistory
+
+    h = PagedHistory.empty(2, 2, 3, 4, (2,))
+    args = h.pages, h.table, h.lengths, h.refs
+    for bad in (torch.zeros(1, dtype=torch.int32), torch.zeros(0, dtype=torch.int32, device="cuda"),
+                torch.zeros(2, dtype=torch.int32, device="cuda")):
+        with pytest.raises(ValueError, match="dropped"):
+            PagedHistory(*args, bad)
+    counter = torch.full((1,), 3, dtype=torch.int32, device="cuda")
+    assert PagedHistory(*args, counter).dropped is counter
+
+
 # ---- against lists ------------------------------------------------------------------------
 
 
