@@ -182,9 +182,9 @@ class PagedHistory:
         in it.  The result replaces this history, which is void once the result is
         appended to or compacted.  `out` takes the result instead of a new history: one
         over the same pages with a table, lengths and refs of its own (two histories
-        used in turn, for instance by captured graphs)."""
+        used in turn, for instance by captured graphs); it takes over this one's `dropped`."""
         p = self._indices(parents, "parents")
-        v, n, counter = self._view, p.numel(), None
+        v, n, counter, dropped = self._view, p.numel(), None, None
         if out is None:
             entries = n * v.row_pages
             book = torch.empty(entries + n + v.n_pages + 1, dtype=torch.int32, device=self._device)
@@ -199,7 +199,11 @@ class PagedHistory:
         elif (out._view.pages != v.pages or out._pages.shape != self._pages.shape or out._pages.dtype != self._pages.dtype
               or (out._view.n_rows, out._view.row_pages) != (n, v.row_pages)):
             raise ValueError("out must be over the same pages, with a row for every parent")
+        else:
+            dropped = self.dropped
         capi.check(capi.load().carlb_history_fork(v, out._view, p.data_ptr(), counter, self._stream()))
+        if dropped is not None:
+            out._dropped = dropped
         return out
 
     def append(self, records: torch.Tensor, mask: torch.Tensor | None = None) -> None:

@@ -366,6 +366,36 @@ def test_history_in_graphs():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("counted", [False, True])
+def test_forks_go_on_with_the_dropped_records(counted):
+    """Into a new history and into one with a counter of its own, back and forth."""
+    import torch
+    from carl_b200.history import PagedHistory
+
+    def books():
+        i32 = dict(dtype=torch.int32, device="cuda")
+        return torch.full((3, 1), -1, **i32), torch.zeros(3, **i32), torch.zeros(8, **i32)
+
+    pages = torch.zeros(8, 2, device="cuda")
+    counter = lambda k: torch.full((1,), k, dtype=torch.int32, device="cuda") if counted else None  # noqa: E731
+    a, b = PagedHistory(pages, *books(), counter(2)), PagedHistory(pages, *books(), counter(100))
+    parents, rec = torch.arange(3, device="cuda"), torch.ones(3, device="cuda")
+    want = 2 if counted else 0
+    for step in range(4):                               # two records fit; three rows are dropped from then on
+        a.append(rec)
+        want += 3 * (step >= 2)
+        assert int(a.dropped) == want
+        a = a.fork(parents)
+        assert int(a.dropped) == want
+        a.fork(parents, out=b)
+        assert int(b.dropped) == want
+        a, b = b, PagedHistory(pages, *books(), counter(100))
+    fresh = PagedHistory(pages, *books())               # without a counter, not looked at before
+    fresh.fork(parents, out=a)
+    assert int(a.dropped) == 0
+
+
+@pytest.mark.gpu
 def test_a_search_with_an_env(tmp_path, monkeypatch):
     """The operators together, as a search uses them: mask, select, reorder, fork, append, step, harvest."""
     import torch
