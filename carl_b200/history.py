@@ -151,6 +151,11 @@ class PagedHistory:
             self._dropped = torch.zeros(1, dtype=torch.int32, device=self._device)
         return self._dropped
 
+    def _written(self, *tensors: torch.Tensor) -> None:
+        # The kernels write by address; a backward pass that has saved a tensor must not use it.
+        books = self._books if isinstance(self._books, tuple) else (self._books,)
+        torch.autograd.graph.increment_version((*books, *tensors))
+
     def _stream(self) -> int:
         return capi.current_stream(self._device.index)
 
@@ -204,6 +209,7 @@ class PagedHistory:
         capi.check(capi.load().carlb_history_fork(v, out._view, p.data_ptr(), counter, self._stream()))
         if dropped is not None:
             out._dropped = dropped
+            out._written()
         return out
 
     def append(self, records: torch.Tensor, mask: torch.Tensor | None = None) -> None:
@@ -235,12 +241,14 @@ class PagedHistory:
         capi.check(lib.carlb_history_append(v, records.data_ptr(), records.stride(0) * records.element_size(),
                                             None if m is None else m.data_ptr(), self.dropped.data_ptr(),
                                             work.data_ptr(), size, self._stream()))
+        self._written(self._pages, self._dropped)
 
     def free(self, mask: torch.Tensor) -> None:
         """Empties the rows with mask[r]; a page is free when no row names it any more."""
         m = self._mask(mask, "mask")
         if self._view.n_rows:
             capi.check(capi.load().carlb_history_free(self._view, m.data_ptr(), self._stream()))
+            self._written()
 
     def compact(self) -> torch.Tensor:
         """Moves the live pages to the front and returns their number, int32 [1] on the
@@ -251,6 +259,7 @@ class PagedHistory:
         work = torch.empty(size, dtype=torch.uint8, device=self._device)
         live = torch.empty(1, dtype=torch.int32, device=self._device)
         capi.check(capi.load().carlb_history_compact(v, live.data_ptr(), work.data_ptr(), size, self._stream()))
+        self._written(self._pages)
         return live
 
     def read(self, steps: int, rows: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:

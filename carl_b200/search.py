@@ -169,7 +169,8 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, dim: i
 
     Row g * beams + j takes the content that row g * beams + parents[g, j] had; a value
     outside [0, beams) leaves its row as it is.  The tensors must not overlap one
-    another or parents.  Up to 1024 beams.
+    another or parents.  To autograd it is an in-place operation: a backward pass that
+    has saved one of the states raises.  Up to 1024 beams.
     """
     if isinstance(states, torch.Tensor):
         raise TypeError("states must be a sequence of tensors")
@@ -218,3 +219,4 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, dim: i
         raise ValueError("states must not overlap one another or parents")
     capi.check(capi.load().carlb_reorder_states(arrays, count, p.data_ptr(), rows // beams, beams, device.index,
                                                 capi.current_stream(device.index)))
+    torch.autograd.graph.increment_version(states)  # a backward pass that has saved one must not use it

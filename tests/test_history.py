@@ -396,6 +396,38 @@ def test_forks_go_on_with_the_dropped_records(counted):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("change", ["append", "compact", "free", "fork", "count"])
+def test_a_backward_pass_does_not_use_a_changed_history(change):
+    import torch
+    from carl_b200.history import PagedHistory
+
+    for forked in (False, True):                         # books of their own, or in one tensor
+        h = PagedHistory.empty(3, 2, 9, 2, (4,))
+        spare = PagedHistory(h.pages, torch.full_like(h.table, -1), torch.zeros_like(h.lengths), torch.zeros_like(h.refs))
+        if forked:
+            h = h.fork(torch.arange(3, device="cuda"))
+        h.append(torch.ones(3, 4, device="cuda"))
+        w = torch.ones(4, device="cuda", requires_grad=True)
+        table = torch.ones(10, device="cuda", requires_grad=True)
+        which = {"append": h.pages, "compact": h.pages, "free": h.lengths, "fork": spare.lengths, "count": h.dropped}[change]
+        if which is h.pages:
+            loss = (h.pages[0] * w).sum()
+        else:
+            loss = table.index_select(0, which).sum()    # saves the indices
+        calls = {"append": lambda: h.append(torch.ones(3, 4, device="cuda")), "compact": h.compact,
+                 "free": lambda: h.free(torch.ones(3, dtype=torch.bool, device="cuda")),
+                 "fork": lambda: h.fork(torch.arange(3, device="cuda"), out=spare),
+                 "count": lambda: h.append(torch.ones(3, 4, device="cuda"))}
+        calls[change]()
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+        records, _ = h.read(2)                           # a copy
+        loss = (records * w).sum()
+        h.append(torch.ones(3, 4, device="cuda"))
+        loss.backward()
+
+
+@pytest.mark.gpu
 def test_a_search_with_an_env(tmp_path, monkeypatch):
     """The operators together, as a search uses them: mask, select, reorder, fork, append, step, harvest."""
     import torch

@@ -586,6 +586,24 @@ def test_reorder_many_arrays_and_neighbours():
 
 
 @pytest.mark.gpu
+def test_a_backward_pass_does_not_use_reordered_states():
+    """A state that a backward pass has saved (for a weight's gradient) is changed: the pass refuses, as after copy_."""
+    import torch
+    from carl_b200.search import reorder_states
+
+    w = torch.ones(5, device="cuda", requires_grad=True)
+    saved, other = torch.randn(6, 5, device="cuda"), torch.randn(6, 5, device="cuda")
+    parents = torch.tensor([[1, 0, 2], [2, 2, 2]], device="cuda")
+    loss, free = (saved * w).sum(), (other.clone() * w).sum()
+    reorder_states([other, saved[:]], parents)           # a view of it counts too
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    free.backward()
+    with torch.inference_mode():
+        reorder_states([torch.zeros(6, 2, device="cuda"), saved], parents)
+
+
+@pytest.mark.gpu
 def test_reorder_beyond_32_bits():
     import torch
     from carl_b200.search import reorder_states
