@@ -89,6 +89,7 @@ class PagedHistory:
         self._pages, self._books, self._dropped, self._device = pages, (table, lengths, refs), dropped, device
         self._view = capi.History(pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), record_bytes,
                                   rows[0], rows[1], shape[0], shape[1], device.index)
+        self._own = tuple((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for _, t in (("pages", pages), *books))
 
     @classmethod
     def empty(cls, n_rows: int, row_pages: int, n_pages: int, page_len: int, record_shape: tuple = (),
@@ -199,6 +200,7 @@ class PagedHistory:
             lengths = at + 4 * entries
             refs = lengths + 4 * n
             out._view = capi.History(v.pages, at, lengths, refs, v.record_bytes, n, v.row_pages, v.n_pages, v.page_len, v.device)
+            out._own = self._own[0], (at, refs + 4 * v.n_pages + 4)  # the pages; the books and a counter
             if out._dropped is None:
                 out._dropped, counter = book[-1:], refs + 4 * v.n_pages
         elif (out._view.pages != v.pages or out._pages.shape != self._pages.shape or out._pages.dtype != self._pages.dtype
@@ -231,15 +233,21 @@ class PagedHistory:
         m = None if mask is None else self._mask(mask, "mask")
         if n == 0:
             return
+        counter = self.dropped.data_ptr()
         if not records.is_contiguous() and not records[0].is_contiguous():
             records = records.detach().contiguous()
-        elif v.pages is not None and v.pages <= records.data_ptr() < v.pages + v.record_bytes * v.page_len * v.n_pages:
-            records = records.clone()  # records of this history: their pages are written to
+        else:
+            at = records.data_ptr()
+            end = at + (n - 1) * records.stride(0) * records.element_size() + v.record_bytes
+            for low, high in (*self._own, (counter, counter + 4)):
+                if at < high and low < end:
+                    records = records.clone()  # the history's own memory, which is written to
+                    break
         lib = capi.load()
         size = _workspaces(n, v.row_pages, v.n_pages, v.page_len)[0]
         work = torch.empty(size, dtype=torch.uint8, device=self._device)
         capi.check(lib.carlb_history_append(v, records.data_ptr(), records.stride(0) * records.element_size(),
-                                            None if m is None else m.data_ptr(), self.dropped.data_ptr(),
+                                            None if m is None else m.data_ptr(), counter,
                                             work.data_ptr(), size, self._stream()))
         self._written(self._pages, self._dropped)
 

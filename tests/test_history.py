@@ -428,6 +428,40 @@ def test_a_backward_pass_does_not_use_a_changed_history(change):
 
 
 @pytest.mark.gpu
+def test_records_in_the_historys_own_memory():
+    """Rows that begin in front of the pages and run into them, the lengths, the table: taken as they were before."""
+    import torch
+    from carl_b200.history import PagedHistory
+
+    n, P = 600, 2
+    i32 = dict(dtype=torch.int32, device="cuda")
+    store = torch.arange(1500 * P * 3, **i32).view(1500, P, 3)
+    pages = store[500:]
+    h = PagedHistory(pages, torch.full((n, 3), -1, **i32), torch.zeros(n, **i32), torch.zeros(1000, **i32))
+    ref = _mirror(h)
+    for records in (store[400:1000, 1], store[:600, 0], h.table, store[400:1000, 1]):
+        want = records.cpu().numpy()
+        h.append(records)
+        ref.append(want)
+        _same(h, ref)
+    one = PagedHistory(torch.zeros(900, 4, **i32), torch.full((n, 2), -1, **i32), torch.zeros(n, **i32), torch.zeros(900, **i32))
+    ref = _mirror(one)
+    for records in (one.lengths, one.lengths, one.refs[100:100 + n], one.dropped.expand(n), one.lengths,
+                    one.dropped.expand(n)):                  # a third of the rows drop theirs by then
+        want = records.cpu().numpy()
+        one.append(records)
+        ref.append(want)
+        _same(one, ref)
+    one = one.fork(torch.arange(n, device="cuda"))           # books in one tensor
+    ref = ref.fork(np.arange(n))
+    for _ in range(3):
+        want = one.lengths.cpu().numpy()
+        one.append(one.lengths)
+        ref.append(want)
+        _same(one, ref)
+
+
+@pytest.mark.gpu
 def test_a_search_with_an_env(tmp_path, monkeypatch):
     """The operators together, as a search uses them: mask, select, reorder, fork, append, step, harvest."""
     import torch
