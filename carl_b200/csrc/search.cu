@@ -876,15 +876,21 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
             place += c.total > mine.total || (c.total == mine.total && c.index < mine.index);
             near |= c.beam != mine.beam && fabs(c.total - mine.total) <= NEAR_TOTALS;
         }
-        if (tid < n && near && place < p.width + 1) sh.repair = 1;
+        // Only what is near one of the first `width` places counts: the set of beams that are
+        // summed again, and with it every score, depends on the totals alone and not on how
+        // low the bar came to be.
+        near &= tid < n && place < p.width;
+        if (near) sh.repair = 1;
         sync();
         if (sh.repair)
         {
             clear();
-            for (int i = 0; tid < n && i < n; i++)
+            for (int i = 0; near && i < n; i++)
             {
                 const Candidate c = sh.found[i];
-                if (c.beam != mine.beam && fabs(c.total - mine.total) <= NEAR_TOTALS) mark(mine.beam);
+                if (c.beam == mine.beam || !(fabs(c.total - mine.total) <= NEAR_TOTALS)) continue;
+                mark(mine.beam);
+                mark(c.beam);
             }
             sync();
             repair();
@@ -907,6 +913,20 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
         return;
     }
 
+    // The elements of lane l's chunk of a segment, 32 at a time (all lanes take part; -inf is none).
+    const auto eachElement = [&](const Row<T>& row, int begin, int end, int l, auto use) {
+        const int elements = max(0, (end - begin - l + 31) / 32) * VE;
+        for (int e0 = 0; e0 < elements; e0 += 32)
+        {
+            const int e = e0 + lane, action = row.head + (begin + l + e / VE * 32) * VE + e % VE;
+            const bool has = e < elements && (!row.allowed || row.allowed[action]);
+            use(has ? toFloat(row.x[action]) : NEG_INF, action);
+        }
+        float x = NEG_INF;
+        const int action = begin == 0 && lane == l ? row.edge(x) : -1;
+        use(x, action);
+    };
+
     // Every element, chunk by chunk: a warp leaves out the chunks whose largest total, at
     // the lowest index it could have, would come behind its list's last place.  Rows of
     // equal logits so end after the chunks that hold their first few.
@@ -927,22 +947,10 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
             {
                 const int l = __ffs(left) - 1;
                 left &= left - 1;
-                const int elements = max(0, (end - begin - l + 31) / 32) * VE;
-                for (int e0 = 0; e0 < elements; e0 += 32)
-                {
-                    const int e = e0 + lane, action = row.head + (begin + l + e / VE * 32) * VE + e % VE;
-                    GroupKey key{};
-                    if (e < elements && (!row.allowed || row.allowed[action]))
-                    {
-                        const float x = toFloat(row.x[action]);
-                        if (x > NEG_INF) key = GroupKey{ ordered64(b + (double)x), ~((unsigned)k * p.vocab + action) };
-                    }
-                    list.push(key.t && better(key, list.bar), key);
-                }
-                float x = NEG_INF;
-                const int action = begin == 0 && lane == l ? row.edge(x) : -1;
-                const GroupKey key{ ordered64(b + (double)x), ~((unsigned)k * p.vocab + action) };
-                list.push(x > NEG_INF && better(key, list.bar), key);
+                eachElement(row, begin, end, l, [&](float x, int action) {
+                    const GroupKey key{ ordered64(b + (double)x), ~((unsigned)k * p.vocab + action) };
+                    list.push(x > NEG_INF && better(key, list.bar), key);
+                });
             }
             k += stepBeams;
             seg += stepSegs;
@@ -1012,10 +1020,27 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
     for (int c = tid; !every && c < n; c += THREADS) nearEdge(sh.found[c].total, sh.found[c].beam);
     if (every && last.t)
     {
-        // Any beam with a chunk that comes up to the last place may have an element there.
+        // Of the other elements those that are near the last place: largest ones of their chunks,
+        // and others in the chunks whose largest is in front (fewer than `width` of them).
+        if (tid == 0) sh.chunks = 0;
+        sync();
         eachChunk([&](double total, int c) {
-            if (total > NEG_INF && total >= edge - NEAR_TOTALS) nearEdge(edge, (c >> 5) / segs);
+            const int k = (c >> 5) / segs;
+            if (!(total >= edge - NEAR_TOTALS) || k == kl) return;
+            if (total <= edge + NEAR_TOTALS)
+                nearEdge(total, k);
+            else
+                sh.chunk[atomicAdd(&sh.chunks, 1)] = c;
         });
+        sync();
+        for (int j = warp; j < sh.chunks; j += Shared::WARPS)
+        {
+            const int c = sh.chunk[j], k = (c >> 5) / segs, begin = THREADS == 32 ? 0 : ((c >> 5) - k * segs) * segVectors;
+            const Row<T> row(p, g, k, lane);
+            eachElement(row, begin, min(row.vectors, begin + segVectors), c & 31, [&](float x, int) {
+                if (x > NEG_INF) nearEdge(base[k] + (double)x, k);
+            });
+        }
         for (int k = tid; p.finished && k < K; k += THREADS) nearEdge((double)overOf(k), k);
     }
     sync();

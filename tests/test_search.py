@@ -243,6 +243,65 @@ def test_one_beam_has_all_the_best(G, K, V, width):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("K, V, width, spread", [(8, 30011, 64, 1e-1), (8, 30011, 64, 1e-3), (16, 9000, 128, 1e-2),
+                                                 (6, 648, 16, 1e-3), (64, 5000, 32, 1e-2)])
+def test_scores_do_not_depend_on_what_was_found_first(K, V, width, spread):
+    """More reaches the bar than there is room for, so that the next bar depends on what came first.  Beams 3 and 4 have
+    one of the best places each, and near totals of theirs lie at many places behind the last; beams 1 and 2 are
+    near in front.  The scores near zero show the last bits of a normaliser."""
+    import torch
+    from carl_b200.search import beam_select
+
+    rng = np.random.default_rng(V + K)
+    G = 24
+    x = rng.normal(0, 1, (G, K, V)).astype(np.float32)
+    dense = V // 3
+    x[:, 0, :dense] = np.linspace(9, 9 + spread, dense, dtype=np.float32)
+    at = rng.permutation(V)[:43]
+    for k, top in ((1, 2e-3), (2, 2e-3 + 2e-6), (3, 1e-3), (4, 5e-4)):
+        x[:, k, at[0]] = 8.9 + 0.001 * k + top
+    # Totals of beams 3 and 4 down beam 0's, from a fifth of the way behind the last place on.
+    down = np.linspace(dense - 1.2 * width, max(0, dense - 12 * width), 42).astype(int)
+    for g in range(G):
+        for j, place in enumerate(down):
+            for k in (3, 4):
+                x[g, k, at[1 + j]] = (x[g, 0, place] - 9.5) + 8.9 + 0.001 * k
+    zero = 8.9 + 0.001 * np.arange(K)                # the logit that makes a total of 0
+    zero[0] = 9.5                                    # beam 0's dense totals begin at -0.5
+    s = (np.log(np.exp(x.astype(np.float64)).sum(-1)) - zero).astype(np.float32)
+    x, s = torch.from_numpy(x).cuda(), torch.from_numpy(s).cuda()
+    first = beam_select(x, s, width=width)
+    assert all(set(range(5)) <= set(row) for row in first.parents.tolist())
+    for _ in range(60):
+        again = beam_select(x, s, width=width)
+        assert torch.equal(again.scores, first.scores) and torch.equal(again.parents, first.parents)
+        assert torch.equal(again.actions, first.actions)
+    _check(x.cpu(), s.cpu(), None, None, width)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V, width", [(30012, 64), (9000, 16), (200000, 128)])
+def test_near_totals_behind_the_best_of_a_chunk(V, width):
+    """A beam of equal logits, and one with four legal neighbours: one far in front, three within a few float32 steps
+    of the equal ones, before or behind them."""
+    import torch
+
+    G = 9
+    x, m = np.zeros((G, 2, V), np.float32), np.ones((G, 2, V), bool)
+    at = V // 8 * 4
+    m[:, 1] = False
+    m[:, 1, at:at + 4] = True
+    x[:, 1, at + 1] = 5
+    s = np.zeros((G, 2), np.float32)
+    s[:, 1] = np.log(np.exp(5.0) + 3) - np.log(V)
+    for g in range(G):
+        for _ in range(abs(g - 4)):
+            s[g, 1] = np.nextafter(s[g, 1], np.float32(np.sign(g - 4) * 100), dtype=np.float32)
+    best = _check(torch.from_numpy(x), torch.from_numpy(s), torch.from_numpy(m), None, width)
+    assert sorted(set((best.parents == 1).sum(-1).tolist())) == [1, 4]
+
+
+@pytest.mark.gpu
 def test_near_totals_are_ranked_in_64_bits():
     """Beams whose normalisers differ by less than float32 sums can tell."""
     import torch
