@@ -7,11 +7,14 @@ lineages share their past, so records lie in pages of `page_len` that a table
 assigns to rows; a page is shared until a row writes to it::
 
     history = PagedHistory.empty(n_rows, row_pages, n_pages, page_len, (obs_dim,))
+    torch.cuda.current_stream().wait_stream(torch.cuda.ExternalStream(env.stream))
     history.append(env.get_obs().view(n_rows, obs_dim))     # one record per row
     history.free(done)                                      # rows of ended episodes
     history = history.fork(parents)                         # rows become their parents
     history.compact()                                       # live pages to the front
     records, counts = history.read(steps)                   # the last records, dense
+
+An env writes its outputs on its own stream, hence the wait before they are read.
 
 Everything runs on torch's current stream of the pages' device, without a host
 synchronisation, and can be captured into CUDA graphs; two calls on one history (or

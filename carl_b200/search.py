@@ -3,11 +3,21 @@
 A group is one planning problem; a beam is one candidate of it, with a score (the
 sum of its actions' log-probabilities) and a sim of an env.  A step of a search::
 
-    best = codec.beam_select(logits, scores, codec.mask(obs), finished=done)
+    torch_stream.wait_stream(env_stream)           # the outputs are written on the env's stream
+    obs = env.get_obs()[:, 0].contiguous()
+    best = codec.beam_select(policy(obs).view(...), scores, codec.mask(obs).view(...))
     env.reorder(best.parents)                      # the kept beams' sims
     reorder_states([hidden], best.parents)         # the caller's own per-beam state
     history = history.fork(best.parents + first)   # the kept beams' records
+    history.append(best.actions ...)
     env.step(best.actions ...)
+
+with ``env_stream = torch.cuda.ExternalStream(env.stream)``: the env's inputs are
+ordered after torch's current stream, but nothing orders torch after the env, so what
+reads an env's output, or writes to a tensor that an env call still reads, has to wait.
+At the root all beams but one start with a score of -inf: copies of one sim with equal
+scores tie everywhere, which says the same several times and is slow (near totals are
+ranked in 64 bits, row by row).
 
 The kernels run on torch's current stream of the inputs' device, neither
 synchronise nor read values on the host, and can be captured into CUDA graphs.

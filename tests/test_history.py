@@ -516,3 +516,65 @@ def test_a_search_with_an_env(tmp_path, monkeypatch):
     records, _ = history.read(5, torch.arange(0, n, K, device="cuda"))
     assert records.tolist() == [p[0] for p in paths]
     env.close()
+
+
+@pytest.mark.gpu
+def test_the_documented_search_loop(tmp_path, monkeypatch):
+    """The loop of the integration guide as it stands there, with an env that is slow to step (a delay on its stream
+    before every step) and one that is waited for after every call: the same observations, choices and records.
+    """
+    import re
+    import torch
+    from pathlib import Path
+
+    from box_arena import write_box
+    from carl_b200 import carl
+    from carl_b200.action import CARLActionCodec
+
+    guide = (Path(__file__).resolve().parents[1] / "INTEGRATION.md").read_text()
+    loop, = [c for c in re.findall(r"```python\n(.*?)```", guide, re.S) if "codec.beam_select" in c]
+    monkeypatch.setenv("CARL_ARENA_OBJ", str(write_box(tmp_path / "box.obj")))
+    G, K, depth = 5, 4, 6
+    n = G * K
+    codec = CARLActionCodec()
+    gen = torch.Generator("cuda").manual_seed(1)
+    idx = torch.arange(0, n, K, device="cuda")
+
+    def run(slow):
+        env = carl.Env(n, 1, 1, 7)
+        stream = torch.cuda.ExternalStream(env.stream)
+        seen = []
+        weight = torch.randn(env.obs_dim, 18, device="cuda", generator=gen.manual_seed(1)) * 0.01
+        delay = torch.zeros(1 << 26, device="cuda")
+
+        def step(actions):
+            if slow:
+                with torch.cuda.stream(stream):
+                    for _ in range(40):              # a few milliseconds, in which an early read sees the old outputs
+                        delay.add_(1.0)
+            env_step(actions)
+            if not slow:
+                torch.cuda.synchronize()
+
+        env_step, env.step = env.step, step
+
+        def policy(obs):
+            seen.append(obs.clone())
+            return obs @ weight
+
+        scope = dict(torch=torch, env=env, codec=codec, policy=policy, groups=G, beams=K, depth=depth, row_pages=4,
+                     n_pages=3 * n, page_len=2, hidden=torch.arange(n, device="cuda"))
+        exec(loop, scope)
+        torch.cuda.synchronize()
+        records, counts = scope["history"].read(8)
+        env.close()
+        return dict(obs=torch.stack(seen), scores=scope["scores"], hidden=scope["hidden"],
+                    records=records, counts=counts)
+
+    want, got = run(False), run(True)
+    for name in want:
+        assert torch.equal(want[name], got[name]), name
+    assert (want["obs"][1:] != want["obs"][:-1]).flatten(1).any(1).all()         # every step is seen
+    assert torch.equal(want["hidden"].view(G, K), idx[:, None].expand(G, K))     # all from the root's first beam
+    assert (want["counts"] == depth).all()
+    assert torch.isfinite(want["scores"]).all()
