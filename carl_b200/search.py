@@ -4,12 +4,14 @@ A group is one planning problem; a beam is one candidate of it, with a score (th
 sum of its actions' log-probabilities) and a sim of an env.  A step of a search::
 
     torch_stream.wait_stream(env_stream)           # the outputs are written on the env's stream
+    over = over | env.get_dones().view(over.shape) # an env step resets a sim that is done
     obs = env.get_obs()[:, 0].contiguous()
-    best = codec.beam_select(policy(obs).view(...), scores, codec.mask(obs).view(...))
+    best = codec.beam_select(policy(obs).view(...), scores, codec.mask(obs).view(...), finished=over)
     env.reorder(best.parents)                      # the kept beams' sims
     reorder_states([hidden], best.parents)         # the caller's own per-beam state
     history = history.fork(best.parents + first)   # the kept beams' records
-    history.append(best.actions ...)
+    over = over.gather(1, best.parents)            # a lineage that is over stays so
+    history.append(best.actions ..., ~over ...)
     env.step(best.actions ...)
 
 with ``env_stream = torch.cuda.ExternalStream(env.stream)``: the env's inputs are

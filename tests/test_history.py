@@ -522,7 +522,7 @@ def test_a_search_with_an_env(tmp_path, monkeypatch):
 def test_the_documented_search_loop(tmp_path, monkeypatch):
     """The loop of the integration guide as it stands there, with an env that is slow to step (a delay on its stream
     before every step) and one that is waited for after every call: the same observations, choices and records.
-    """
+    Episodes end on the way, and a lineage that is over keeps its score and its records."""
     import re
     import torch
     from pathlib import Path
@@ -542,12 +542,16 @@ def test_the_documented_search_loop(tmp_path, monkeypatch):
 
     def run(slow):
         env = carl.Env(n, 1, 1, 7)
+        env.max_ticks = 1000
         stream = torch.cuda.ExternalStream(env.stream)
-        seen = []
+        seen, steps = [], []
         weight = torch.randn(env.obs_dim, 18, device="cuda", generator=gen.manual_seed(1)) * 0.01
+        zeros = torch.zeros(G, dtype=torch.int32, device="cuda")
         delay = torch.zeros(1 << 26, device="cuda")
 
         def step(actions):
+            # One beam of every group ends with this step.
+            env_set(zeros + 1, zeros, zeros + 999, idx + len(steps) % K)   # (a tie would go on)
             if slow:
                 with torch.cuda.stream(stream):
                     for _ in range(40):              # a few milliseconds, in which an early read sees the old outputs
@@ -555,8 +559,9 @@ def test_the_documented_search_loop(tmp_path, monkeypatch):
             env_step(actions)
             if not slow:
                 torch.cuda.synchronize()
+            steps.append(None)
 
-        env_step, env.step = env.step, step
+        env_step, env_set, env.step = env.step, env.set_match_state, step
 
         def policy(obs):
             seen.append(obs.clone())
@@ -568,7 +573,7 @@ def test_the_documented_search_loop(tmp_path, monkeypatch):
         torch.cuda.synchronize()
         records, counts = scope["history"].read(8)
         env.close()
-        return dict(obs=torch.stack(seen), scores=scope["scores"], hidden=scope["hidden"],
+        return dict(obs=torch.stack(seen), scores=scope["scores"], over=scope["over"], hidden=scope["hidden"],
                     records=records, counts=counts)
 
     want, got = run(False), run(True)
@@ -576,5 +581,6 @@ def test_the_documented_search_loop(tmp_path, monkeypatch):
         assert torch.equal(want[name], got[name]), name
     assert (want["obs"][1:] != want["obs"][:-1]).flatten(1).any(1).all()         # every step is seen
     assert torch.equal(want["hidden"].view(G, K), idx[:, None].expand(G, K))     # all from the root's first beam
-    assert (want["counts"] == depth).all()
+    counts, over = want["counts"].view(G, K), want["over"]
+    assert over.any() and (counts[~over] == depth).all() and (counts[over] < depth).any()
     assert torch.isfinite(want["scores"]).all()
