@@ -187,13 +187,6 @@ def action_mask(obs, rows: int, obs_dim: int, previous_controls: bool, mask, str
         raise CarlbError(st, lib.carlb_last_error(None).decode())
 
 
-def current_stream(device: int) -> int:
-    """torch's current CUDA stream of a device, as an address."""
-    import torch
-
-    return torch._C._cuda_getCurrentRawStream(device)
-
-
 def check(st: int) -> None:
     """Raises the error of an entry point that has no env: ValueError for arguments,
     CarlbError (a RuntimeError) otherwise."""

@@ -59,19 +59,22 @@ class PagedHistory:
 
     def __init__(self, pages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
                  dropped: torch.Tensor | None = None):
-        books = [("table", table), ("lengths", lengths), ("refs", refs)]
+        books = (("table", table), ("lengths", lengths), ("refs", refs))
         if dropped is not None:
-            books.append(("dropped", dropped))
-        for name, t in (("pages", pages), *books):
+            books += ("dropped", dropped),
+        if not isinstance(pages, torch.Tensor):
+            raise TypeError("pages must be a tensor")
+        for name, t in books:
             if not isinstance(t, torch.Tensor):
                 raise TypeError(f"{name} must be a tensor")
-        device, shape, rows = pages.device, pages.shape, table.shape
-        for name, t in books:
             if t.dtype is not torch.int32:
                 raise TypeError(f"{name} must have dtype int32")
-        for name, t in (("pages", pages), *books):
-            if not t.is_cuda:
-                raise ValueError(f"{name} must be on a CUDA device")
+        device, shape, rows = pages.device, pages.shape, table.shape
+        if not pages.is_cuda:
+            raise ValueError("pages must be on a CUDA device")
+        if not pages.is_contiguous():
+            raise ValueError("pages must be contiguous")
+        for name, t in books:
             if t.device != device:
                 raise ValueError(f"{name} must be on {device}")
             if not t.is_contiguous():
@@ -90,9 +93,10 @@ class PagedHistory:
         for n in shape[2:]:
             record_bytes *= n
         self._pages, self._books, self._dropped, self._device = pages, (table, lengths, refs), dropped, device
-        self._view = capi.History(pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), record_bytes,
-                                  rows[0], rows[1], shape[0], shape[1], device.index)
-        self._own = tuple((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for _, t in (("pages", pages), *books))
+        at, t, n, r = pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), refs.data_ptr()
+        self._view = capi.History(at, t, n, r, record_bytes, rows[0], rows[1], shape[0], shape[1], device.index)
+        self._own = ((at, at + record_bytes * shape[0] * shape[1]), (t, t + 4 * rows[0] * rows[1]), (n, n + 4 * rows[0]),
+                     (r, r + 4 * shape[0]))  # what the operators write to
 
     @classmethod
     def empty(cls, n_rows: int, row_pages: int, n_pages: int, page_len: int, record_shape: tuple = (),
@@ -161,7 +165,7 @@ class PagedHistory:
         torch.autograd.graph.increment_version((*books, *tensors))
 
     def _stream(self) -> int:
-        return capi.current_stream(self._device.index)
+        return torch._C._cuda_getCurrentRawStream(self._view.device)
 
     def _mask(self, mask, name: str) -> torch.Tensor:
         if not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool:
@@ -236,22 +240,23 @@ class PagedHistory:
         m = None if mask is None else self._mask(mask, "mask")
         if n == 0:
             return
-        counter = self.dropped.data_ptr()
         if not records.is_contiguous() and not records[0].is_contiguous():
             records = records.detach().contiguous()
+        at, step, counter = records.data_ptr(), records.stride(0) * records.element_size(), self.dropped.data_ptr()
+        end = at + (n - 1) * step + v.record_bytes
+        for low, high in self._own:
+            if at < high and low < end:
+                break
         else:
-            at = records.data_ptr()
-            end = at + (n - 1) * records.stride(0) * records.element_size() + v.record_bytes
-            for low, high in (*self._own, (counter, counter + 4)):
-                if at < high and low < end:
-                    records = records.clone()  # the history's own memory, which is written to
-                    break
+            low, high = counter, counter + 4
+        if at < high and low < end:
+            records = records.clone()  # the history's own memory, which is written to
+            at, step = records.data_ptr(), records.stride(0) * records.element_size()
         lib = capi.load()
         size = _workspaces(n, v.row_pages, v.n_pages, v.page_len)[0]
         work = torch.empty(size, dtype=torch.uint8, device=self._device)
-        capi.check(lib.carlb_history_append(v, records.data_ptr(), records.stride(0) * records.element_size(),
-                                            None if m is None else m.data_ptr(), counter,
-                                            work.data_ptr(), size, self._stream()))
+        capi.check(lib.carlb_history_append(v, at, step, None if m is None else m.data_ptr(), counter, work.data_ptr(), size,
+                                            self._stream()))
         self._written(self._pages, self._dropped)
 
     def free(self, mask: torch.Tensor) -> None:

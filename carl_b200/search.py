@@ -144,14 +144,14 @@ def select(logits, scores, mask, width, finished, *, joint: bool) -> BeamStep:
                          device.index)
     lib = capi.load()
     if joint:
-        capi.check(lib.carlb_joint_select(args, capi.current_stream(device.index)))
+        capi.check(lib.carlb_joint_select(args, torch._C._cuda_getCurrentRawStream(device.index)))
         return best
     size = ctypes.c_int64()
     capi.check(lib.carlb_beam_workspace(args, size))
     if size.value:
         work = torch.empty(size.value, dtype=torch.uint8, device=device)
         args.workspace, args.workspace_bytes = work.data_ptr(), size.value
-    capi.check(lib.carlb_beam_select(args, capi.current_stream(device.index)))
+    capi.check(lib.carlb_beam_select(args, torch._C._cuda_getCurrentRawStream(device.index)))
     return best
 
 
@@ -230,5 +230,5 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, dim: i
     if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
         raise ValueError("states must not overlap one another or parents")
     capi.check(capi.load().carlb_reorder_states(arrays, count, p.data_ptr(), rows // beams, beams, device.index,
-                                                capi.current_stream(device.index)))
+                                                torch._C._cuda_getCurrentRawStream(device.index)))
     torch.autograd.graph.increment_version(states)  # a backward pass that has saved one must not use it
