@@ -1231,35 +1231,56 @@ __device__ __forceinline__ void settle(JointKey (&l)[N])
         }
 }
 
+// A logit's last bit, in binades below its first.
+template <class T>
+__device__ constexpr int lastBit();
+template <>
+__device__ constexpr int lastBit<float>() { return 23; }
+template <>
+__device__ constexpr int lastBit<__nv_bfloat16>() { return 7; }
+template <>
+__device__ constexpr int lastBit<__half>() { return 10; }
+
 // The best of a beam's totals, one after another; the first of equal ones stays in front.
+// The six choices of the last two heads side by side: 24576 groups of 8 such beams take 154
+// us (36 if they were not looked through; an action at a time took 399), and 70 where five of
+// them have one (41 without: the time of the warp that comes last).
 template <class X, int N>
 __device__ __forceinline__ void bestTotals(const X& x, double base, JointKey (&best)[N])
 {
 #pragma unroll
     for (int i = 0; i < N; i++) best[i] = JointKey{ NEG_INF, 0 };
+    double low[3], last[2];
+#pragma unroll
+    for (int q = 0; q < 3; q++) low[q] = (double)x(13 + q);
+#pragma unroll
+    for (int q = 0; q < 2; q++) last[q] = (double)x(16 + q);
 #pragma unroll 1
-    for (int a = 0; a < JOINT_ACTIONS; a++)
+    for (int a = 0; a < JOINT_ACTIONS / 6; a++)
     {
-        int digit[HEADS], rest = a;
+        const int a2 = a >> 2, a1 = a2 / 3, a0 = a1 / 3;
+        const double sum = (double)x(a0) + (double)x(3 + a1 - 3 * a0) + (double)x(6 + a2 - 3 * a1) + (double)x(9 + (a >> 1 & 1))
+                           + (double)x(11 + (a & 1));
+        double total[6];
+        bool any = false;
 #pragma unroll
-        for (int h = HEADS - 1; h >= 0; h--)
+        for (int q = 0; q < 6; q++)
         {
-            digit[h] = rest % headSize(h);
-            rest /= headSize(h);
+            // -inf (an action not allowed) and NaN (that, and a base of +inf) go before nothing.
+            total[q] = base + (sum + low[q / 2] + last[q % 2]);
+            any |= total[q] > best[N - 1].v;
         }
-        double sum = 0.0;
-        int at = 0;
-#pragma unroll
-        for (int h = 0; h < HEADS; h++)
+        if (!any) continue;
+#pragma unroll 1
+        for (int q = 0; q < 6; q++)
         {
-            sum += (double)x(at + digit[h]);
-            at += headSize(h);
-        }
-        const JointKey key{ base + sum, a };  // NaN (a base of +inf, a sum of -inf) goes before nothing
-        if (!(sum > NEG_INF && key.v > best[N - 1].v)) continue;
+            const double v = q == 0 ? total[0] : q == 1 ? total[1] : q == 2 ? total[2] : q == 3 ? total[3] : q == 4 ? total[4] : total[5];
+            const JointKey key{ v, 6 * a + q };
+            if (!(v > best[N - 1].v)) continue;
 #pragma unroll
-        for (int i = N - 1; i > 0; i--) best[i] = key.v > best[i - 1].v ? best[i - 1] : key.v > best[i].v ? key : best[i];
-        if (key.v > best[0].v) best[0] = key;
+            for (int i = N - 1; i > 0; i--) best[i] = v > best[i - 1].v ? best[i - 1] : v > best[i].v ? key : best[i];
+            if (v > best[0].v) best[0] = key;
+        }
     }
 }
 
@@ -1287,10 +1308,11 @@ constexpr int jointBlocks(int n) { return n == 8 ? 7 : n == 16 ? 5 : 0; }
 //
 // Lists of sums are in the order of the totals, equal ones by their action, where sums that
 // differ make totals that do.  A logit is a whole multiple of its last bit's value, and so
-// is a sum of the last bit q of the smallest logit (2^-23 of its binade).  While the sums and
-// the base stay below 2^52 q, sums are exact, differ by q at least and are apart by a unit in
-// the last place of any total.  A beam beyond that (a logit 29 binades below the total, or a
-// score of +inf) has its 648 totals looked through in turn, in the second pass.
+// is a sum of the last bit q of the smallest logit (2^-23 of its binade, in the 16-bit types
+// 2^-10 and 2^-7).  While the sums and the base stay below 2^52 q, sums are exact, differ by
+// q at least and are apart by a unit in the last place of any total.  A beam beyond that (a
+// float32 logit 29 binades below the total, or a score of +inf) has its 648 totals looked
+// through in turn, in the second pass.
 template <class T, int N>
 __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKernel(BeamParams p, int lanes)
 {
@@ -1391,8 +1413,8 @@ __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKern
         if (tops > NEG_INF)
             base = (double)score - (tops + (pass == 0 ? (double)logf(product) : log(product64)));
         const bool live = reads && base > NEG_INF;
-        // 2^52 q, the exponent's field of q being that of the smallest logit less 23.
-        const double limit = __longlong_as_double((long long)(max((int)(least >> 23), 1) - 98 + 1023) << 52);
+        // 2^52 q, the exponent's field of q being that of the smallest logit less its bits.
+        const double limit = __longlong_as_double((long long)(max((int)(least >> 23), 1) - 75 - lastBit<T>() + 1023) << 52);
         const bool merges = live && !(fabs(base) + 7.0 * (double)most < limit);
         if (pass == 1 && merges) bestTotals(x, base, best);
 #pragma unroll
