@@ -523,6 +523,14 @@ __global__ void __launch_bounds__(ROW_THREADS) selectRowsKernel(BeamParams p)
 // twice that are in order.  Nearer ones are decided by normalisers in 64 bits.
 constexpr double NEAR_TOTALS = 8e-6;
 
+// Far from zero a score and a normaliser round to one of two neighbours, whatever the
+// normaliser's error: totals within a few units of the last place are near as well.
+__device__ __forceinline__ bool nearTotals(double a, double b, double error)
+{
+    const double d = fabs(a - b);
+    return d <= error || (d <= 0x1p-50 * fabs(b) && d < INFINITY);
+}
+
 // A continuation that reaches the group's bar.
 struct Candidate
 {
@@ -874,7 +882,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
         {
             const Candidate c = sh.found[i];
             place += c.total > mine.total || (c.total == mine.total && c.index < mine.index);
-            near |= c.beam != mine.beam && fabs(c.total - mine.total) <= NEAR_TOTALS;
+            near |= c.beam != mine.beam && nearTotals(c.total, mine.total, NEAR_TOTALS);
         }
         // Only what is near one of the first `width` places counts: the set of beams that are
         // summed again, and with it every score, depends on the totals alone and not on how
@@ -888,7 +896,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
             for (int i = 0; near && i < n; i++)
             {
                 const Candidate c = sh.found[i];
-                if (c.beam == mine.beam || !(fabs(c.total - mine.total) <= NEAR_TOTALS)) continue;
+                if (c.beam == mine.beam || !nearTotals(c.total, mine.total, NEAR_TOTALS)) continue;
                 mark(mine.beam);
                 mark(c.beam);
             }
@@ -1004,7 +1012,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
     for (int i = tid; i + 1 < p.width; i += THREADS)
     {
         const GroupKey a = list[i], b = list[i + 1];
-        if (!a.t || !b.t || fromOrdered64(a.t) - fromOrdered64(b.t) > NEAR_TOTALS) continue;
+        if (!a.t || !b.t || !nearTotals(fromOrdered64(a.t), fromOrdered64(b.t), NEAR_TOTALS)) continue;
         const int ka = ~a.i / p.vocab, kb = ~b.i / p.vocab;
         if (ka == kb) continue;
         mark(ka);
@@ -1013,7 +1021,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
     const double edge = last.t ? fromOrdered64(last.t) : (double)INFINITY;
     const int kl = ~last.i / p.vocab;
     const auto nearEdge = [&](double total, int beam) {
-        if (beam == kl || !(fabs(total - edge) <= NEAR_TOTALS)) return;
+        if (beam == kl || !nearTotals(total, edge, NEAR_TOTALS)) return;
         mark(beam);
         mark(kl);
     };
@@ -1026,10 +1034,10 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
         sync();
         eachChunk([&](double total, int c) {
             const int k = (c >> 5) / segs;
-            if (!(total >= edge - NEAR_TOTALS) || k == kl) return;
-            if (total <= edge + NEAR_TOTALS)
+            if (k == kl) return;
+            if (nearTotals(total, edge, NEAR_TOTALS))
                 nearEdge(total, k);
-            else
+            else if (total > edge)
                 sh.chunk[atomicAdd(&sh.chunks, 1)] = c;
         });
         sync();
@@ -1447,7 +1455,7 @@ __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKern
         // beams that are near have such a pair between them.
         if (pass == 0)
         {
-            bool near = merges;
+            bool near = false;
             int kept = 0;  // of this beam
             JointKey last = best[0];
 #pragma unroll
@@ -1455,13 +1463,14 @@ __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKern
             {
                 if (i >= p.width) continue;
                 if (i > 0)
-                    near |= last.v - best[i].v <= NEAR_JOINT && best[i].v > NEG_INF
+                    near |= nearTotals(last.v, best[i].v, NEAR_JOINT) && best[i].v > NEG_INF
                             && last.i / JOINT_ACTIONS != best[i].i / JOINT_ACTIONS;
                 last = best[i];
                 kept += last.i / JOINT_ACTIONS == k;
             }
             const double left = kept < N ? own(kept) : (double)NEG_INF;
-            near |= last.v - left <= NEAR_JOINT && left > NEG_INF && last.i / JOINT_ACTIONS != k;
+            near |= nearTotals(last.v, left, NEAR_JOINT) && left > NEG_INF && last.i / JOINT_ACTIONS != k;
+            near |= merges && kept > 0;  // the values of such a list are right, their actions may not be
             const unsigned votes = __ballot_sync(FULL, near), group = (lanes < 32 ? (1u << lanes) - 1 : FULL) << (lane - k);
             again = votes & group;
             anyAgain = votes != 0;

@@ -335,20 +335,26 @@ def test_joint_near_totals_are_ranked_in_64_bits(K, width):
     _check(torch.from_numpy(x), torch.full((40, K), -2.0), None, None, width, HEADS, sum_error=JOINT_SUM_ERROR)
 
 
-def _check_beside_rounding(x, s, width):
-    """The joint selection where scores and logits of two beams may differ and their totals be the same real number
-    (score -2 and a sum of 3, score -3 and a sum of 4, equal normalisers): which of these comes first is then a matter
-    of how each side rounds.  Whole logits are at most 2 and scores 3, so a normaliser, a base and a total are below 32
-    and round by at most 2^-49 each; seven tops and logarithms added up, the base and the total make 16 roundings a
-    side, 2.9e-14, and two totals on two sides 1.2e-13.  A beam's own continuations have exact sums and keep their order."""
+def _check_beside_rounding(x, s, width, mask=None, heads=HEADS):
+    """A selection where scores and logits of two beams may differ and their totals be the same real number (score -2
+    and a sum of 3, score -3 and a sum of 4, or the same logits in another order): which of these comes first is then a
+    matter of how each side rounds.  Logits are whole and at most 12, scores 3e8 or more or at most 4: where totals are
+    below 32, a normaliser, a base and a total round by at most 2^-49 each; seven tops and logarithms added up (or a sum
+    of exponentials whose terms and partial sums are off by as much in relation), the base and the total make 16
+    roundings a side, 2.9e-14, and two totals on two sides 1.2e-13.  Far from zero (from 1e3 on) a normaliser's last
+    bit vanishes in the score, and totals are equal.  A beam's own continuations have exact sums and keep their order."""
     from carl_b200.action import CARLActionCodec
+    from carl_b200.search import beam_select
 
     ROUNDING = 1.2e-13
     G, K, _ = x.shape
-    best = CARLActionCodec().beam_select(x.cuda(), s.cuda(), width=width)
+    joint = heads is HEADS
+    fn = CARLActionCodec().beam_select if joint else beam_select
+    best = fn(x.cuda(), s.cuda(), None if mask is None else mask.cuda(), width=width)
     x, s = x.double().numpy(), s.double().numpy()
+    x = x if mask is None else np.where(mask.numpy(), x, -np.inf)
     sums, norm, at = np.zeros((G, K, 1)), 0.0, 0
-    for h in HEADS:
+    for h in heads:
         row = x[..., at:at + h]
         top = row.max(-1, keepdims=True)
         norm = norm + top[..., 0] + np.log(np.exp(row - top).sum(-1))
@@ -356,16 +362,21 @@ def _check_beside_rounding(x, s, width):
         at += h
     totals = (s - norm)[..., None] + sums
     want = -np.sort(-totals.reshape(G, -1), -1)[:, :width]
+    rounding = np.where(np.abs(want) < 1e3, ROUNDING, 0.0)
     parents = best.parents.cpu().numpy()
-    actions = np.ravel_multi_index(tuple(np.moveaxis(best.actions.cpu().numpy(), -1, 0)), HEADS)
+    actions = best.actions.cpu().numpy()
+    actions = np.ravel_multi_index(tuple(np.moveaxis(actions, -1, 0)), HEADS) if joint else actions
     got = totals[np.arange(G)[:, None], parents, actions]
-    assert (np.abs(got - want) <= ROUNDING).all()
-    assert (np.abs(best.scores.cpu().double().numpy() - want) <= JOINT_SUM_ERROR + ROUNDING + 2.0 ** -24 * np.abs(want)).all()
+    assert (np.abs(got - want) <= rounding).all()
+    error = JOINT_SUM_ERROR if joint else SUM_ERROR
+    assert (np.abs(best.scores.cpu().double().numpy() - want) <= error + rounding + 2.0 ** -24 * np.abs(want)).all()
     order = np.argsort(-totals, -1, kind="stable")           # a beam's continuations are taken in order
     for g in range(G):
         for k in np.unique(parents[g]):
             taken = actions[g][parents[g] == k]
             assert (taken == order[g, k, :taken.size]).all()
+        for i in range(1, width):                            # and of totals that are equal far from zero the lower beam's
+            assert want[g, i] < want[g, i - 1] or want[g, i] > -1e3 or parents[g, i] >= parents[g, i - 1]
 
 
 @pytest.mark.gpu
@@ -440,6 +451,30 @@ def test_flat_scores_of_infinity():
         best = _check(x, s, m, None, width)
         got = best.scores.cpu()
         assert not torch.isnan(got).any() and (got[:4, 0] == math.inf).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("joint", [False, True])
+@pytest.mark.parametrize("score", [-1e6, -3e8, -1e10, -1e11, -3e11, -1e12, -1e14, -1e16, -1e20])
+def test_scores_far_from_zero(joint, score):
+    """Totals whose unit in the last place is from far below to far above a normaliser's error: score - normaliser is
+    one of two neighbours, and beams of equal scores differ by that.  Logits are whole, so no total is half way; the
+    beams of a group differ in one of them, by 1e-5 and less in the normaliser."""
+    import torch
+
+    rng = np.random.default_rng(int(-10 * np.log10(-score)) + 1000)
+    G, K = 800, 8
+    for V, width in [(18, 8)] if joint else [(40, 8), (40, 16), (1500, 20)]:
+        x = np.tile(rng.integers(-3, 4, (G, 1, V)).astype(np.float32), (1, K, 1))
+        x[:, :, 8] = -8 - 4 * rng.random((G, K))
+        s = np.full((G, K), score, np.float32)
+        s[G // 2:, ::2] = -4.0                       # some beams near zero; the others are reached where few logits are left
+        m = np.ones((G, K, V), bool)
+        if not joint:
+            m[G // 2:, ::2, 1:8] = False
+            m[G // 2:, ::2, 9:] = False
+        _check_beside_rounding(torch.from_numpy(x), torch.from_numpy(s), width, torch.from_numpy(m),
+                               HEADS if joint else (V,))
 
 
 @pytest.mark.gpu
