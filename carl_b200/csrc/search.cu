@@ -524,12 +524,9 @@ __global__ void __launch_bounds__(ROW_THREADS) selectRowsKernel(BeamParams p)
 constexpr double NEAR_TOTALS = 8e-6;
 
 // Far from zero a score and a normaliser round to one of two neighbours, whatever the
-// normaliser's error: totals within a few units of the last place are near as well.
-__device__ __forceinline__ bool nearTotals(double a, double b, double error)
-{
-    const double d = fabs(a - b);
-    return d <= error || (d <= 0x1p-50 * fabs(b) && d < INFINITY);
-}
+// normaliser's error: totals within a few units of the last place are near as well.  (A
+// total of +inf is near nothing.)
+__device__ __forceinline__ double nearness(double total) { return NEAR_TOTALS + fmin(0x1p-50 * fabs(total), 1e300); }
 
 // A continuation that reaches the group's bar.
 struct Candidate
@@ -877,12 +874,13 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
         if (tid < n) mine = sh.found[tid];
         int place = 0;
         bool near = false;
+        const double range = nearness(mine.total);
 #pragma unroll 4
         for (int i = 0; i < n; i++)
         {
             const Candidate c = sh.found[i];
             place += c.total > mine.total || (c.total == mine.total && c.index < mine.index);
-            near |= c.beam != mine.beam && nearTotals(c.total, mine.total, NEAR_TOTALS);
+            near |= c.beam != mine.beam && fabs(c.total - mine.total) <= range;
         }
         // Only what is near one of the first `width` places counts: the set of beams that are
         // summed again, and with it every score, depends on the totals alone and not on how
@@ -896,7 +894,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
             for (int i = 0; near && i < n; i++)
             {
                 const Candidate c = sh.found[i];
-                if (c.beam == mine.beam || !nearTotals(c.total, mine.total, NEAR_TOTALS)) continue;
+                if (c.beam == mine.beam || !(fabs(c.total - mine.total) <= range)) continue;
                 mark(mine.beam);
                 mark(c.beam);
             }
@@ -1012,16 +1010,19 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
     for (int i = tid; i + 1 < p.width; i += THREADS)
     {
         const GroupKey a = list[i], b = list[i + 1];
-        if (!a.t || !b.t || !nearTotals(fromOrdered64(a.t), fromOrdered64(b.t), NEAR_TOTALS)) continue;
+        if (!a.t || !b.t) continue;
+        const double total = fromOrdered64(a.t);
+        if (!(total - fromOrdered64(b.t) <= nearness(total))) continue;
         const int ka = ~a.i / p.vocab, kb = ~b.i / p.vocab;
         if (ka == kb) continue;
         mark(ka);
         mark(kb);
     }
     const double edge = last.t ? fromOrdered64(last.t) : (double)INFINITY;
+    const double edgeRange = nearness(edge);
     const int kl = ~last.i / p.vocab;
     const auto nearEdge = [&](double total, int beam) {
-        if (beam == kl || !nearTotals(total, edge, NEAR_TOTALS)) return;
+        if (beam == kl || !(fabs(total - edge) <= edgeRange)) return;
         mark(beam);
         mark(kl);
     };
@@ -1035,7 +1036,7 @@ __device__ __forceinline__ void finishGroup(const BeamParams& p, long long g, in
         eachChunk([&](double total, int c) {
             const int k = (c >> 5) / segs;
             if (k == kl) return;
-            if (nearTotals(total, edge, NEAR_TOTALS))
+            if (fabs(total - edge) <= edgeRange)
                 nearEdge(total, k);
             else if (total > edge)
                 sh.chunk[atomicAdd(&sh.chunks, 1)] = c;
@@ -1463,13 +1464,13 @@ __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKern
             {
                 if (i >= p.width) continue;
                 if (i > 0)
-                    near |= nearTotals(last.v, best[i].v, NEAR_JOINT) && best[i].v > NEG_INF
+                    near |= last.v - best[i].v <= NEAR_JOINT + 0x1p-50 * fabs(last.v) && best[i].v > NEG_INF
                             && last.i / JOINT_ACTIONS != best[i].i / JOINT_ACTIONS;
                 last = best[i];
                 kept += last.i / JOINT_ACTIONS == k;
             }
             const double left = kept < N ? own(kept) : (double)NEG_INF;
-            near |= nearTotals(last.v, left, NEAR_JOINT) && left > NEG_INF && last.i / JOINT_ACTIONS != k;
+            near |= last.v - left <= NEAR_JOINT + 0x1p-50 * fabs(last.v) && left > NEG_INF && last.i / JOINT_ACTIONS != k;
             near |= merges && kept > 0;  // the values of such a list are right, their actions may not be
             const unsigned votes = __ballot_sync(FULL, near), group = (lanes < 32 ? (1u << lanes) - 1 : FULL) << (lane - k);
             again = votes & group;
