@@ -1340,8 +1340,16 @@ __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKern
     const auto own = [&](int i) -> double& { return ownS[i][threadIdx.x]; };
     const T* from = rowLogits<T>(p, reads ? g : 0, reads ? k : 0);
     const uint8_t* allowed = rowMask(p, reads ? g : 0, reads ? k : 0);
+    unsigned least = 0xffffffffu;  // image of the smallest logit's size, less one (0 wraps)
+    float most = 0.f;              // largest logit's size
 #pragma unroll
-    for (int q = 0; q < ACTION_LOGITS; q++) x(q) = reads && (!allowed || allowed[q]) ? toFloat(from[q]) : NEG_INF;
+    for (int q = 0; q < ACTION_LOGITS; q++)
+    {
+        const float v = reads && (!allowed || allowed[q]) ? toFloat(from[q]) : NEG_INF;
+        least = min(least, (__float_as_uint(v) & 0x7fffffffu) - 1);
+        most = fmaxf(most, v > NEG_INF ? fabsf(v) : 0.f);
+        x(q) = v;
+    }
 
     JointKey best[N];
     bool again = false, anyAgain = false;  // the group's second pass, and the warp's
@@ -1350,8 +1358,6 @@ __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKern
         // The normaliser (NaN or +inf among the logits makes it NaN, an empty head -inf),
         // and the beam's best joint actions.
         double tops = 0.0, base = NEG_INF;
-        unsigned least = 0xffffffffu;  // image of the smallest logit's size, less one (0 wraps)
-        float most = 0.f;              // largest logit's size
         float product = 1.f;
         double product64 = 1.0;
 #pragma unroll
@@ -1366,12 +1372,6 @@ __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKern
             at += size;
             const float top = fmaxf(fmaxf(v[0], v[1]), v[2]);
             tops += (double)top;
-#pragma unroll
-            for (int q = 0; q < 3; q++)
-            {
-                least = min(least, (__float_as_uint(v[q]) & 0x7fffffffu) - 1);
-                most = fmaxf(most, v[q] > NEG_INF ? fabsf(v[q]) : 0.f);
-            }
             if (pass == 0)
             {
                 float sum = 0.f;
