@@ -491,9 +491,10 @@ constexpr int ROW_WARPS = 8;
 constexpr int ROW_THREADS = ROW_WARPS * 32;
 
 // One warp per segment of a row, results to the workspace.  Bound by memory in float32
-// (64 x 16 rows of 131072: 104 us with the finishing kernel, 5.2 TB/s); in the 16-bit types
-// by issue and the exponential unit at about eight logits a clock and SM (128 x 16 rows:
-// 135 us, 4.0 TB/s).  Loading eight vectors at a time, or none ahead, measured the same.
+// (64 x 16 rows of 131072: 104 us with the finishing kernel, 5.2 TB/s, where no totals are
+// near); in the 16-bit types by issue (56 % of its slots) and the exponential unit at about
+// eight logits a clock and SM (128 x 16 rows: 132 us, 4.1 TB/s).  Loading eight vectors at a
+// time, or none ahead, measured the same.
 template <class T, bool MASKED>
 __global__ void __launch_bounds__(ROW_THREADS) selectRowsKernel(BeamParams p)
 {
@@ -1186,9 +1187,10 @@ __device__ __forceinline__ void finishRows(const BeamParams& p, long long g, int
         r.base, sh);
 }
 
-// A block reads a group's rows, its first warp finishes.  Bound by issue: about 600
-// instructions of a warp a row and 1000 a group (4096 groups of 8 beams over 648 with a
-// mask: 43 us; the bytes alone would take 14).
+// A block reads a group's rows, its first warp finishes.  Bound by latency: 4096 groups of 8
+// beams over 648 with a mask take 45 us, their 18.8 M instructions 17 us of issue and the
+// bytes 14.  A warp waits for its next row's score, then for the row, and 26 % of the warps'
+// places are taken.
 template <class T, bool MASKED>
 __global__ void __launch_bounds__(GROUP_WARPS * 32, 3) selectGroupKernel(BeamParams p)
 {
@@ -1304,9 +1306,10 @@ constexpr int JOINT_THREADS = 128;
 // lists of 4 and 32 are the faster without one.
 constexpr int jointBlocks(int n) { return n == 8 ? 7 : n == 16 ? 5 : 0; }
 
-// Bound by issue (196608 rows of 18 logits in 24576 groups: 43 us, of which 7 for the few
-// warps that take the 64-bit pass; the bytes alone would take 3.7).  Blocks of 64 threads
-// measured the same, a limit of 48 registers 46 us, outputs through shared memory 50 us.
+// 196608 rows of 18 logits in 24576 groups: 43 us.  25.5 M instructions are 22 us of issue
+// and the bytes 4; the rest is waiting for the 64-bit pipe and for loads with a third of the
+// warps' places taken, and the few warps that take the 64-bit pass.  Blocks of 64 threads
+// measured the same, a limit of 48 registers 3 us more, outputs through shared memory 7.
 //
 // A thread per beam, the beams of a group side by side in a warp (padded to a power
 // of two).  The best N joint actions of a beam are found head by head: the list of
@@ -1504,9 +1507,11 @@ __global__ void __launch_bounds__(JOINT_THREADS, jointBlocks(N)) jointSelectKern
 // ---- state reordering --------------------------------------------------------------------
 //
 // Every byte of a moved row is read and written once; the kernels differ in how a block
-// finds them.  Bound by memory: the word-major state of 32768 sims of 3v3, whose 24-byte
-// rows fill every 32-byte sector, is 188 MB of sectors in 35 us (5.4 TB/s; 77 us row by
-// row in the largest unit).  Rows of whole 16-byte columns go through registers (reorderRowsKernel);
+// finds them.  The word-major state of 32768 sims of 3v3, whose 24-byte rows fill every
+// 32-byte sector, is 188 MB of sectors in 36 us (77 us row by row in the largest unit): 5.3
+// TB/s at the L2 cache, of which 129 MB reach memory (3.9 TB/s).  It waits for loads and at
+// the barrier of a slab.  Rows of whole 16-byte columns go through registers (reorderRowsKernel: 32768 sims'
+// observations, hidden states and actions, 53.6 us of bytes at the copy rate, in 73);
 // short rows, as the simulator's words of a few cars, through shared memory as one dense
 // run of whole groups (reorderRunsKernel); anything else, and what is too small for more
 // than one launch to pay, in the row's largest unit (reorderTilesKernel).

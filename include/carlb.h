@@ -380,7 +380,10 @@ carlb_status carlb_beam_workspace(const carlb_beam_args* args, int64_t* bytes);
 /* The `width` best continuations of each group, best first: the total of action v
  * of beam k is scores[k] + logits[k][v] - log(sum over the allowed u of
  * exp(logits[k][u])), and equal totals go to the lower k * vocab + v.  Totals are
- * compared as if computed in 64 bits and returned rounded to float32.
+ * compared as if computed in 64 bits, but returned from logarithms that are off by up
+ * to 3.5e-6 (joint: 4.5e-6) unless the order needs them more exactly, and rounded to
+ * float32; the same call gives the same bits.  Logits of a beam that differ by less
+ * than the last bit of a 64-bit total are ranked by how the totals round.
  * A finished beam has one continuation, action 0 at its own score.  Not allowed:
  * actions with mask 0 (whatever their logit), logits of -inf, every action of a
  * beam whose score is -inf or NaN or whose allowed logits hold a NaN or +inf.
