@@ -1301,9 +1301,11 @@ __device__ __forceinline__ void bestTotals(const X& x, double base, JointKey (&b
 constexpr double NEAR_JOINT = 1e-5;
 
 constexpr int JOINT_THREADS = 128;
-// Blocks of an SM (0: no limit): without these limits the lists of 8 take 72 registers and 49 us where 64
-// take 47 (24576 groups of 8 beams), those of 16 118 and 111 us where 96 take 94 (12288 of 16);
-// lists of 4 and 32 are the faster without one.
+// Blocks that an SM has to hold (0: no limit).  Lists of 8 take 72 registers and 43.1 us with
+// the limit, 80 and 44.0 without (24576 groups of 8 beams; one group 8.2 and 9.4); of 16, 96 and
+// 93, 128 and 107 (12288 of 16).  For lists of 32 a limit of two blocks costs 312 us, none 248
+// (6144 of 32), and for lists of 4 one of nine 24.5, none 25.2, but 19.7 against 19.0 where a
+// group is one beam.
 constexpr int jointBlocks(int n) { return n == 8 ? 7 : n == 16 ? 5 : 0; }
 
 // 196608 rows of 18 logits in 24576 groups: 43 us.  25.5 M instructions are 22 us of issue
